@@ -527,6 +527,45 @@ int32_t oxz_loader_seek(oxz_loader* loader, oxz_data_position pos);
  * loader, the buffers are recycled in its order. */
 int32_t oxz_loader_next_batch_async(oxz_loader* loader, void* stream, int64_t** inputs, int64_t** targets, uint64_t* rows);
 
+/* ------------------------------------------------------------------ the token embedding
+ *
+ * The first operator of a model and its gradient, between the loader's batch and the flat gradient buffer: the table is
+ * work + offsets[embed_tokens] of a plan, its gradient goes to grads + offsets[embed_tokens] (embed_tokens, [vocab, hidden],
+ * src/model.rs:3905-3953; tied models share the tensor with the head, so its gradient is then added to the head's).
+ *
+ *   lookup     out[i] = scale * table[ids[i]]
+ *   gradient   d_table[v] = scale * sum over i with ids[i] = v of d_out[i]      (+ what d_table held, when accumulating)
+ *
+ * Sums run in f32, in the order of the tokens, whatever the launch: equal inputs give equal bits. Each result is rounded once
+ * to its type. An id outside [0, vocab) reads as a row of zeros and receives no gradient.
+ * The handle holds the workspace of the gradient. It is used by one thread at a time; calls on different streams are ordered by
+ * the handle, but graphs captured from its gradient calls share the workspace, so their replays must not overlap each other or
+ * other gradient calls of the handle. No call allocates, synchronises or copies to the host. */
+typedef struct oxz_embed oxz_embed;
+typedef struct oxz_embed_desc {
+    uint64_t max_tokens;  /* the most tokens of one call, below 2^31 */
+    uint64_t hidden;      /* elements of a row */
+    uint64_t vocab;       /* rows of the table, below 2^31 */
+    double scale;         /* factor of the embedding (1: none); applied in f32 */
+    int32_t dtype;        /* oxz_dtype of the table, the rows looked up and their gradients */
+    int32_t grad_dtype;   /* oxz_dtype of the table's gradient: dtype or OXZ_F32 */
+    int32_t device;       /* CUDA device ordinal */
+    int32_t reserved;     /* 0 */
+} oxz_embed_desc;
+int32_t oxz_embed_create(const oxz_embed_desc* desc, oxz_embed** out); /* host only: runs without a GPU */
+/* Allocates the gradient's workspace on the device; *workspace_bytes (may be NULL) receives its size. A handle that is only
+ * looked up through needs none. */
+int32_t oxz_embed_alloc(oxz_embed* embed, uint64_t* workspace_bytes);
+int32_t oxz_embed_destroy(oxz_embed* embed);
+/* n tokens (0: nothing is done). ids: device i64, as the loader hands its inputs. out: rows of `hidden` elements, out_stride
+ * elements apart (0: hidden). Pointers are aligned to their element; rows that start on 16 bytes move in 16-byte pieces. */
+int32_t oxz_embed_lookup_async(const oxz_embed* embed, const int64_t* ids, uint64_t n, const void* table, void* out,
+                               uint64_t out_stride, void* stream);
+/* accumulate 0: every row of d_table is written, rows without a token with zeros. accumulate 1: the sums are added in f32 to
+ * what the rows of d_table hold, and rows without a token are left alone (n 0: nothing is done). d_out must not overlap d_table. */
+int32_t oxz_embed_grads_async(oxz_embed* embed, const int64_t* ids, uint64_t n, const void* d_out, uint64_t d_out_stride,
+                              void* d_table, int32_t accumulate, void* stream);
+
 /* StepWeighting::over_ranks applied to the summed counts (src/dp/weighting.rs:46-61): counts = {scored, masked ranks}
  * after oxz_allreduce_i64x2. *global_scored = -1 for an unmasked step. Mixed masks are OXZ_ERR_INVALID on every rank. */
 int32_t oxz_step_weighting(uint64_t local_micro_batches, int32_t world, const int64_t counts[2],

@@ -102,6 +102,11 @@ class BatchMasks(C.Structure):
                 ("scored", C.POINTER(C.c_uint64)), ("n_segments", C.POINTER(C.c_uint64))]
 
 
+class EmbedDesc(C.Structure):
+    _fields_ = [("max_tokens", C.c_uint64), ("hidden", C.c_uint64), ("vocab", C.c_uint64), ("scale", C.c_double),
+                ("dtype", C.c_int32), ("grad_dtype", C.c_int32), ("device", C.c_int32), ("reserved", C.c_int32)]
+
+
 RankBody = C.CFUNCTYPE(C.c_int32, C.c_int32, C.c_int32, C.c_void_p)
 
 # name -> (restype, argtypes): one row per declaration of include/oxz_dpstep.h
@@ -203,6 +208,11 @@ SIGNATURES = {
     "oxz_loader_position": (C.c_int32, [vp, C.POINTER(DataPositionC)]),
     "oxz_loader_seek": (C.c_int32, [vp, DataPositionC]),
     "oxz_loader_next_batch_async": (C.c_int32, [vp, vp, C.POINTER(vp), C.POINTER(vp), u64p]),
+    "oxz_embed_create": (C.c_int32, [C.POINTER(EmbedDesc), C.POINTER(vp)]),
+    "oxz_embed_alloc": (C.c_int32, [vp, u64p]),
+    "oxz_embed_destroy": (C.c_int32, [vp]),
+    "oxz_embed_lookup_async": (C.c_int32, [vp, vp, C.c_uint64, vp, vp, C.c_uint64, vp]),
+    "oxz_embed_grads_async": (C.c_int32, [vp, vp, C.c_uint64, vp, C.c_uint64, vp, C.c_int32, vp]),
     "oxz_step_weighting": (C.c_int32, [C.c_uint64, C.c_int32, i64p, u64p, i64p]),
 }
 

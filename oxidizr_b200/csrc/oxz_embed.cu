@@ -1,0 +1,490 @@
+// The token embedding (oxz_embed_*): a scaled row lookup, and its gradient by sorted tokens.
+//
+//   out[i] = c * T[id_i]            dT[v] = c * sum_{i : id_i = v} dY_i   (+ dT[v])
+//
+// Both are bound by memory: the lookup reads and writes n rows; the gradient reads n rows and writes either the whole table
+// (overwriting) or the rows that have tokens, read and written (accumulating). The gradient adds no atomics: the tokens are
+// sorted (stable, so equal tokens keep their order), every sum runs in f32 in that order, and equal inputs give equal bits.
+#include <algorithm>
+#include <cmath>
+
+#include <cooperative_groups.h>
+
+#include "oxz_elem.cuh"
+#include "oxz_internal.h"
+
+namespace cg = cooperative_groups;
+
+struct oxz_embed {
+    oxz_embed_desc d{};
+    bool allocated = false;
+    uint64_t bytes = 0;
+    unsigned long long* sorted[2] = {nullptr, nullptr};  // token << 32 | position, max_tokens each
+    float* carry = nullptr;                              // [chunks][2][hidden]: partial sums of the tokens that cross chunks
+    oxz::StreamOrder order;
+};
+
+namespace oxz {
+namespace {
+
+constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_CLUSTER = 8;
+constexpr int DIGIT_BITS = 9, BINS = 1 << DIGIT_BITS;
+constexpr uint32_t CHUNK = 16;  // sorted tokens a warp sums on its own
+
+// ---- lookup: a warp takes a piece of 32 x 4 vectors of one row
+template <typename T, int N>
+__global__ void __launch_bounds__(256) k_embed_lookup(const int64_t* __restrict__ ids, uint64_t n, const T* __restrict__ table,
+                                                      T* __restrict__ out, uint64_t out_stride, uint32_t hidden, uint64_t vocab,
+                                                      float scale, uint32_t pieces) {
+    for (uint64_t unit = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; unit < n * pieces; unit += (uint64_t)gridDim.x * 8) {
+        const uint64_t row = unit / pieces;
+        const uint32_t first = (uint32_t)(unit - row * pieces) * 32 * 4 * N + (threadIdx.x & 31) * N;
+        const int64_t id = ids[row];
+        const bool known = (uint64_t)id < vocab;
+        const T* src = table + (known ? (uint64_t)id * hidden : 0);
+        T* dst = out + row * out_stride;
+        Vec<T, N> v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (known && first + k * 32 * N < hidden) v[k].load(src + first + k * 32 * N);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (first + k * 32 * N >= hidden) break;
+#pragma unroll
+            for (int j = 0; j < N; j++) v[k].e[j] = from_f32<T>(known ? to_f32<T>(v[k].e[j]) * scale : 0.f);
+            v[k].store(dst + first + k * 32 * N);
+        }
+    }
+}
+
+// ---- gradient, first launch. Cluster 0 sorts the tokens; when the table is overwritten the other clusters fill it with zeros
+// meanwhile, which hides the sort behind the fill (the longer of the two wherever the table is worth filling).
+//
+// The sort is a least-significant-digit radix sort by digits of at most 9 bits. A block owns a contiguous run of the items, a
+// warp a contiguous run of the block's, and walks it 32 at a time: __match_any_sync ranks equal digits within the 32, a
+// histogram of the warp's own counts the ones before. Bases come from the blocks' histograms, read through distributed shared
+// memory, so that a pass is: count, cluster barrier, place, cluster barrier. Ids outside the table get the key `vocab`, sort
+// behind every token and are not summed.
+struct SortShared {
+    uint32_t mine[SORT_WARPS][BINS];  // per warp: items of each digit seen (first walk), then the next place (second walk)
+    uint32_t block[BINS];             // the block's histogram, read by the other blocks
+    uint32_t scan[SORT_WARPS];
+};
+
+__device__ void sort_tokens(cg::cluster_group& cl, SortShared& sh, const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab,
+                            int passes, int bits, unsigned long long* a, unsigned long long* b) {
+    const uint32_t rank = cl.block_rank(), blocks = cl.num_blocks();
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t bins = 1u << bits;
+    // runs are multiples of 32 items so that only the last warp with items meets a part of 32
+    const uint32_t per_warp = (((n + blocks * SORT_WARPS - 1) / (blocks * SORT_WARPS)) + 31) & ~31u;
+    const uint64_t begin = (uint64_t)(rank * SORT_WARPS + warp) * per_warp;
+    const uint32_t lo = (uint32_t)min(begin, (uint64_t)n), hi = (uint32_t)min(begin + per_warp, (uint64_t)n);
+    unsigned long long *src = a, *dst = b;
+    for (int pass = 0; pass < passes; pass++) {
+        const int shift = pass * bits;
+        auto item = [&](uint32_t i) -> unsigned long long {
+            if (pass == 0) {
+                const int64_t id = ids[i];
+                return (unsigned long long)((uint64_t)id < vocab ? (uint32_t)id : vocab) << 32 | i;
+            }
+            return src[i];
+        };
+        for (uint32_t i = threadIdx.x; i < SORT_WARPS * bins; i += SORT_THREADS) sh.mine[i / bins][i % bins] = 0;
+        __syncthreads();
+        for (uint32_t i0 = lo; i0 < hi; i0 += 32) {
+            const bool have = i0 + lane < hi;
+            const uint32_t digit = have ? (uint32_t)(item(i0 + lane) >> (32 + shift)) & (bins - 1) : bins;
+            const uint32_t same = __match_any_sync(0xffffffffu, digit);
+            if (have && lane == (uint32_t)(__ffs(same) - 1)) sh.mine[warp][digit] += __popc(same);
+            __syncwarp();
+        }
+        __syncthreads();
+        for (uint32_t d = threadIdx.x; d < bins; d += SORT_THREADS) {
+            uint32_t sum = 0;
+            for (int w = 0; w < SORT_WARPS; w++) sum += sh.mine[w][d];
+            sh.block[d] = sum;
+        }
+        cl.sync();
+        // thread d: the items of its digit in all blocks, and in the blocks before this one
+        uint32_t total = 0, before = 0;
+        if (threadIdx.x < bins) {
+            for (uint32_t r = 0; r < blocks; r++) {
+                const uint32_t c = cl.map_shared_rank(sh.block, r)[threadIdx.x];
+                total += c;
+                before += r < rank ? c : 0;
+            }
+        }
+        // exclusive scan of the totals over the digits
+        uint32_t inc = total;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += up;
+        }
+        if (lane == 31) sh.scan[warp] = inc;
+        __syncthreads();
+        if (warp == 0) {
+            uint32_t w = sh.scan[lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, w, o);
+                if (lane >= (uint32_t)o) w += up;
+            }
+            sh.scan[lane] = w;
+        }
+        __syncthreads();
+        if (threadIdx.x < bins) {
+            uint32_t place = inc - total + (warp ? sh.scan[warp - 1] : 0) + before;
+            for (int w = 0; w < SORT_WARPS; w++) {
+                const uint32_t c = sh.mine[w][threadIdx.x];
+                sh.mine[w][threadIdx.x] = place;
+                place += c;
+            }
+        }
+        __syncthreads();
+        for (uint32_t i0 = lo; i0 < hi; i0 += 32) {
+            const bool have = i0 + lane < hi;
+            const unsigned long long it = have ? item(i0 + lane) : 0;
+            const uint32_t digit = have ? (uint32_t)(it >> (32 + shift)) & (bins - 1) : bins;
+            const uint32_t same = __match_any_sync(0xffffffffu, digit);
+            uint32_t place = 0;
+            if (have) place = sh.mine[warp][digit] + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (have && lane == (uint32_t)(__ffs(same) - 1)) sh.mine[warp][digit] += __popc(same);
+            __syncwarp();
+            if (have) dst[place] = it;
+        }
+        cl.sync();  // the items are in place for every block, and nobody reads this pass's histograms any more
+        unsigned long long* t = src;
+        src = dst;
+        dst = t;
+    }
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) k_embed_sort(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, int passes,
+                                                             int bits, unsigned long long* a, unsigned long long* b,
+                                                             unsigned char* fill, uint64_t fill_bytes) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    cg::cluster_group cl = cg::this_cluster();
+    const uint32_t blocks = cl.num_blocks();
+    if (blockIdx.x < blocks) {
+        if (n) sort_tokens(cl, *reinterpret_cast<SortShared*>(raw), ids, n, vocab, passes, bits, a, b);
+        if (gridDim.x > blocks) return;  // others fill
+    }
+    const bool alone = gridDim.x <= blocks;
+    const uint64_t first = alone ? blockIdx.x : blockIdx.x - blocks, step = alone ? gridDim.x : gridDim.x - blocks;
+    // up to 15 bytes either side of the 16-byte pieces (a table whose rows are not whole pieces)
+    unsigned char* lo = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fill) + 15) & ~(uintptr_t)15);
+    const uint64_t head = min((uint64_t)(lo - fill), fill_bytes), pieces = (fill_bytes - head) / 16;
+    const uint64_t tail = fill_bytes - head - pieces * 16;
+    if (first == 0) {
+        if (threadIdx.x < head) fill[threadIdx.x] = 0;
+        if (threadIdx.x < tail) lo[pieces * 16 + threadIdx.x] = 0;
+    }
+    uint4* q = reinterpret_cast<uint4*>(lo);
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (uint64_t i = first * SORT_THREADS + threadIdx.x; i < pieces; i += step * SORT_THREADS) q[i] = zero;
+}
+
+__device__ __forceinline__ uint32_t key_of(unsigned long long it) { return (uint32_t)(it >> 32); }
+
+template <typename G, int N>
+__device__ __forceinline__ void write_row(G* dst, const float (&sum)[N], float scale, bool accumulate) {
+    Vec<G, N> v;
+    if (accumulate) v.load_coherent(dst);
+#pragma unroll
+    for (int j = 0; j < N; j++) v.e[j] = from_f32<G>(accumulate ? to_f32<G>(v.e[j]) + sum[j] * scale : sum[j] * scale);
+    v.store(dst);
+}
+
+// ---- gradient, second launch: a warp sums one chunk of CHUNK sorted tokens for 32 x N columns. Tokens that lie inside the
+// chunk are written; the sums of a token that goes on from the chunk before or into the chunk after go to the carries:
+// carry[chunk][0] for the token the chunk begins with, carry[chunk][1] for one that begins in the chunk and leaves it.
+template <typename T, typename G, int N>
+__global__ void __launch_bounds__(256) k_embed_sums(const unsigned long long* __restrict__ sorted, uint32_t n, uint32_t vocab,
+                                                    const T* __restrict__ d_out, uint64_t stride, uint32_t hidden, G* d_table,
+                                                    float* __restrict__ carry, float scale, int accumulate, uint32_t slices) {
+    const uint64_t chunks = (n + CHUNK - 1) / CHUNK;
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint64_t unit = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; unit < chunks * slices; unit += (uint64_t)gridDim.x * 8) {
+        const uint32_t chunk = (uint32_t)(unit / slices);
+        const uint64_t c0 = (uint64_t)chunk * CHUNK;
+        const uint32_t col = (uint32_t)(unit - (uint64_t)chunk * slices) * 32 * N + lane * N;
+        const uint32_t count = (uint32_t)min((uint64_t)CHUNK, n - c0);
+        // lane k holds item k; lane CHUNK the item after the chunk
+        unsigned long long it = (unsigned long long)vocab << 32;
+        if (lane < count || (lane == count && c0 + count < n)) it = sorted[c0 + lane];
+        const uint32_t first_key = __shfl_sync(0xffffffffu, key_of(it), 0);
+        const bool from_left = c0 > 0 && key_of(sorted[c0 - 1]) == first_key;
+        const bool live = col < hidden;
+        float sum[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) sum[j] = 0.f;
+        uint32_t begin = 0;  // where the current token's run begins in the chunk
+        constexpr int AHEAD = 8;
+        for (uint32_t k0 = 0; k0 < count; k0 += AHEAD) {
+            Vec<T, N> v[AHEAD];
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++) {
+                const unsigned long long x = __shfl_sync(0xffffffffu, it, (k0 + a) & 31);
+                if (live && k0 + a < count && key_of(x) < vocab) v[a].load(d_out + (uint64_t)(uint32_t)x * stride + col);
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++) {
+                const uint32_t k = k0 + a;
+                const uint32_t key = __shfl_sync(0xffffffffu, key_of(it), k & 31), next = __shfl_sync(0xffffffffu, key_of(it), (k + 1) & 31);
+                if (k >= count || key >= vocab) continue;
+                if (live) {
+#pragma unroll
+                    for (int j = 0; j < N; j++) sum[j] += to_f32<T>(v[a].e[j]);
+                }
+                const bool ends = k + 1 < count ? next != key : !(c0 + count < n && next == key);
+                if (!ends && k + 1 < count) continue;
+                const bool left = begin == 0 && from_left;
+                if (live) {
+                    if (ends && !left) {
+                        write_row<G, N>(d_table + (uint64_t)key * hidden + col, sum, scale, accumulate != 0);
+                    } else {
+                        float* c = carry + ((uint64_t)chunk * 2 + (left ? 0 : 1)) * hidden + col;
+#pragma unroll
+                        for (int j = 0; j < N; j++) c[j] = sum[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < N; j++) sum[j] = 0.f;
+                begin = k + 1;
+            }
+        }
+    }
+}
+
+// ---- gradient, third launch: the tokens that cross chunks. The block of the chunk a token begins in adds the token's carries:
+// its 8 warps take contiguous parts of the chunks, and the parts are added in order.
+template <typename G, int N>
+__global__ void __launch_bounds__(256) k_embed_join(const unsigned long long* __restrict__ sorted, uint32_t n, uint32_t vocab,
+                                                    uint32_t hidden, G* d_table, const float* __restrict__ carry, float scale,
+                                                    int accumulate) {
+    __shared__ float part[8][32 * N];
+    const uint32_t chunk = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint64_t c0 = (uint64_t)chunk * CHUNK, c1 = c0 + CHUNK;
+    if (c1 >= n) return;  // nothing leaves the last chunk
+    const uint32_t key = key_of(sorted[c1 - 1]);
+    if (key >= vocab || key_of(sorted[c1]) != key) return;
+    if (key_of(sorted[c0]) == key && c0 > 0 && key_of(sorted[c0 - 1]) == key) return;  // began further left
+    // one past the token's last item
+    uint32_t lo = (uint32_t)c1, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (key_of(sorted[mid]) <= key) lo = mid + 1;
+        else hi = mid;
+    }
+    const uint32_t last = (lo - 1) / CHUNK, parts = last - chunk;  // carries [0] of chunks chunk + 1 .. last
+    const uint32_t col = blockIdx.y * 32 * N + lane * N;
+    const uint32_t each = (parts + 7) / 8, p0 = min(parts, warp * each), p1 = min(parts, p0 + each);
+    float sum[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) sum[j] = 0.f;
+    if (col < hidden) {
+        if (warp == 0) {
+#pragma unroll
+            for (int j = 0; j < N; j++) sum[j] = carry[((uint64_t)chunk * 2 + 1) * hidden + col + j];
+        }
+#pragma unroll 4
+        for (uint32_t p = p0; p < p1; p++) {
+            const float* c = carry + (uint64_t)(chunk + 1 + p) * 2 * hidden + col;
+#pragma unroll
+            for (int j = 0; j < N; j++) sum[j] += c[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) part[warp][lane * N + j] = sum[j];
+    __syncthreads();
+    if (warp || col >= hidden) return;
+    for (int w = 1; w < 8; w++) {
+#pragma unroll
+        for (int j = 0; j < N; j++) sum[j] += part[w][lane * N + j];
+    }
+    write_row<G, N>(d_table + (uint64_t)key * hidden + col, sum, scale, accumulate != 0);
+}
+
+bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) % to) != 0; }
+
+template <typename T, int N>
+void lookup(const oxz_embed_desc& d, const int64_t* ids, uint64_t n, const void* table, void* out, uint64_t stride, cudaStream_t s) {
+    const uint32_t pieces = (uint32_t)((d.hidden + 128 * N - 1) / (128 * N));
+    const uint64_t blocks = std::min<uint64_t>((n * pieces + 7) / 8, 1u << 30);
+    k_embed_lookup<T, N><<<(unsigned)blocks, 256, 0, s>>>(ids, n, static_cast<const T*>(table), static_cast<T*>(out), stride,
+                                                         (uint32_t)d.hidden, d.vocab, (float)d.scale, pieces);
+}
+
+template <typename T, typename G, int N>
+void sums(oxz_embed* e, uint32_t n, const unsigned long long* sorted, const void* d_out, uint64_t stride, void* d_table,
+             int32_t accumulate, cudaStream_t s) {
+    const oxz_embed_desc& d = e->d;
+    const uint32_t chunks = (n + CHUNK - 1) / CHUNK, slices = (uint32_t)((d.hidden + 32 * N - 1) / (32 * N));
+    const uint64_t blocks = std::min<uint64_t>(((uint64_t)chunks * slices + 7) / 8, 1u << 30);
+    k_embed_sums<T, G, N><<<(unsigned)blocks, 256, 0, s>>>(sorted, n, (uint32_t)d.vocab, static_cast<const T*>(d_out), stride,
+                                                           (uint32_t)d.hidden, static_cast<G*>(d_table), e->carry, (float)d.scale,
+                                                           accumulate, slices);
+    if (chunks > 1)
+        k_embed_join<G, N><<<dim3(chunks - 1, slices), 256, 0, s>>>(sorted, n, (uint32_t)d.vocab, (uint32_t)d.hidden,
+                                                                   static_cast<G*>(d_table), e->carry, (float)d.scale, accumulate);
+}
+
+}  // namespace
+}  // namespace oxz
+
+using namespace oxz;
+
+extern "C" {
+
+int32_t oxz_embed_create(const oxz_embed_desc* desc, oxz_embed** out) {
+    return guarded("oxz_embed_create", [&]() -> int32_t {
+        if (!desc || !out) return fail(OXZ_ERR_INVALID, "oxz_embed_create: null argument");
+        *out = nullptr;
+        const oxz_embed_desc& d = *desc;
+        if (d.max_tokens == 0 || d.max_tokens > 0x7fffffffull)
+            return fail(OXZ_ERR_INVALID, "oxz_embed_create: max_tokens %llu is outside 1..2^31-1", (unsigned long long)d.max_tokens);
+        if (d.vocab == 0 || d.vocab > 0x7fffffffull)
+            return fail(OXZ_ERR_INVALID, "oxz_embed_create: vocab %llu is outside 1..2^31-1", (unsigned long long)d.vocab);
+        if (d.hidden == 0 || d.hidden > (1u << 20))
+            return fail(OXZ_ERR_INVALID, "oxz_embed_create: hidden %llu is outside 1..2^20", (unsigned long long)d.hidden);
+        if (!std::isfinite((float)d.scale)) return fail(OXZ_ERR_INVALID, "oxz_embed_create: scale %g is not a finite f32", d.scale);
+        if (d.dtype != OXZ_F32 && d.dtype != OXZ_BF16 && d.dtype != OXZ_F16)
+            return fail(OXZ_ERR_INVALID, "oxz_embed_create: dtype %d is none of f32, bf16, f16", d.dtype);
+        if (d.grad_dtype != d.dtype && d.grad_dtype != OXZ_F32)
+            return fail(OXZ_ERR_INVALID, "oxz_embed_create: grad_dtype %d is neither the dtype (%d) nor f32", d.grad_dtype, d.dtype);
+        if (d.device < 0) return fail(OXZ_ERR_INVALID, "oxz_embed_create: device %d", d.device);
+        oxz_embed* e = new oxz_embed();
+        e->d = d;
+        *out = e;
+        return OXZ_OK;
+    });
+}
+
+int32_t oxz_embed_alloc(oxz_embed* e, uint64_t* workspace_bytes) {
+    return guarded("oxz_embed_alloc", [&]() -> int32_t {
+        if (!e) return fail(OXZ_ERR_INVALID, "oxz_embed_alloc: null handle");
+        if (!e->allocated) {
+            DeviceGuard dev;
+            OXZ_TRY(dev.enter(e->d.device));
+            const uint64_t chunks = (e->d.max_tokens + CHUNK - 1) / CHUNK;
+            const uint64_t items = e->d.max_tokens * 8, carry = chunks * 2 * e->d.hidden * 4;
+            // what a failed attempt left behind is kept and used by the next one
+            for (int i = 0; i < 2; i++)
+                if (!e->sorted[i]) OXZ_CUDA(cudaMalloc((void**)&e->sorted[i], items));
+            if (!e->carry) OXZ_CUDA(cudaMalloc((void**)&e->carry, carry));
+            OXZ_TRY(e->order.create());
+            OXZ_CUDA(cudaFuncSetAttribute(k_embed_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared)));
+            e->bytes = 2 * items + carry;
+            e->allocated = true;
+        }
+        if (workspace_bytes) *workspace_bytes = e->bytes;
+        return OXZ_OK;
+    });
+}
+
+int32_t oxz_embed_destroy(oxz_embed* e) {
+    return guarded("oxz_embed_destroy", [&]() -> int32_t {
+        if (!e) return OXZ_OK;
+        DeviceGuard dev;
+        if (e->sorted[0] || e->carry) dev.enter(e->d.device);
+        e->order.destroy();
+        for (int i = 0; i < 2; i++)
+            if (e->sorted[i]) cudaFree(e->sorted[i]);
+        if (e->carry) cudaFree(e->carry);
+        delete e;
+        return OXZ_OK;
+    });
+}
+
+int32_t oxz_embed_lookup_async(const oxz_embed* e, const int64_t* ids, uint64_t n, const void* table, void* out, uint64_t out_stride,
+                               void* stream) {
+    return guarded("oxz_embed_lookup_async", [&]() -> int32_t {
+        if (!e) return fail(OXZ_ERR_INVALID, "oxz_embed_lookup_async: null handle");
+        if (n == 0) return OXZ_OK;
+        if (!ids || !table || !out) return fail(OXZ_ERR_INVALID, "oxz_embed_lookup_async: null argument");
+        const oxz_embed_desc& d = e->d;
+        if (n > d.max_tokens)
+            return fail(OXZ_ERR_INVALID, "oxz_embed_lookup_async: %llu tokens, the handle was made for %llu", (unsigned long long)n, (unsigned long long)d.max_tokens);
+        if (out_stride == 0) out_stride = d.hidden;
+        if (out_stride < d.hidden || out_stride > (1ull << 31))
+            return fail(OXZ_ERR_INVALID, "oxz_embed_lookup_async: out_stride %llu with rows of %llu", (unsigned long long)out_stride, (unsigned long long)d.hidden);
+        const size_t es = dtype_size(d.dtype);
+        if (misaligned(ids, 8) || misaligned(table, es) || misaligned(out, es))
+            return fail(OXZ_ERR_INVALID, "oxz_embed_lookup_async: a pointer is not aligned to its element");
+        DeviceGuard dev;
+        OXZ_TRY(dev.enter(d.device));
+        cudaStream_t s = (cudaStream_t)stream;
+        const bool wide = !misaligned(table, 16) && !misaligned(out, 16) && d.hidden * es % 16 == 0 && out_stride * es % 16 == 0;
+        if (d.dtype == OXZ_F32) wide ? lookup<float, 4>(d, ids, n, table, out, out_stride, s) : lookup<float, 1>(d, ids, n, table, out, out_stride, s);
+        else if (d.dtype == OXZ_BF16) wide ? lookup<__nv_bfloat16, 8>(d, ids, n, table, out, out_stride, s) : lookup<__nv_bfloat16, 1>(d, ids, n, table, out, out_stride, s);
+        else wide ? lookup<__half, 8>(d, ids, n, table, out, out_stride, s) : lookup<__half, 1>(d, ids, n, table, out, out_stride, s);
+        OXZ_CUDA(cudaGetLastError());
+        return OXZ_OK;
+    });
+}
+
+int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, const void* d_out, uint64_t d_out_stride, void* d_table,
+                              int32_t accumulate, void* stream) {
+    return guarded("oxz_embed_grads_async", [&]() -> int32_t {
+        if (!e) return fail(OXZ_ERR_INVALID, "oxz_embed_grads_async: null handle");
+        const oxz_embed_desc& d = e->d;
+        if (!d_table || (n && (!ids || !d_out))) return fail(OXZ_ERR_INVALID, "oxz_embed_grads_async: null argument");
+        if (n > d.max_tokens)
+            return fail(OXZ_ERR_INVALID, "oxz_embed_grads_async: %llu tokens, the handle was made for %llu", (unsigned long long)n, (unsigned long long)d.max_tokens);
+        if (d_out_stride == 0) d_out_stride = d.hidden;
+        if (d_out_stride < d.hidden || d_out_stride > (1ull << 31))
+            return fail(OXZ_ERR_INVALID, "oxz_embed_grads_async: d_out_stride %llu with rows of %llu", (unsigned long long)d_out_stride, (unsigned long long)d.hidden);
+        const size_t es = dtype_size(d.dtype), gs = dtype_size(d.grad_dtype);
+        if (misaligned(ids, 8) || misaligned(d_out, es) || misaligned(d_table, gs))
+            return fail(OXZ_ERR_INVALID, "oxz_embed_grads_async: a pointer is not aligned to its element");
+        if (!e->allocated) return fail(OXZ_ERR_STATE, "oxz_embed_grads_async: no workspace: call oxz_embed_alloc first");
+        if (n == 0 && accumulate) return OXZ_OK;
+        DeviceGuard dev;
+        OXZ_TRY(dev.enter(d.device));
+        cudaStream_t s = (cudaStream_t)stream;
+        OXZ_TRY(e->order.begin(s));
+        // keys run to vocab itself (ids outside the table): as few passes of at most DIGIT_BITS bits as hold them, of equal width
+        int key_bits = 1;
+        while ((d.vocab >> key_bits) != 0) key_bits++;
+        const int passes = (key_bits + DIGIT_BITS - 1) / DIGIT_BITS, bits = (key_bits + passes - 1) / passes;
+        int sms = 0;
+        OXZ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d.device));
+        // a cluster no larger than the tokens need: a warp walks 32 at a time
+        unsigned cluster = 1;
+        while (cluster < (unsigned)SORT_CLUSTER && (uint64_t)cluster * SORT_THREADS < n) cluster *= 2;
+        const uint64_t fill_bytes = accumulate ? 0 : d.vocab * d.hidden * gs;
+        unsigned grid = cluster;
+        if (fill_bytes > (1u << 20)) grid = (unsigned)(sms * 2) / cluster * cluster;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(SORT_THREADS);
+        cfg.dynamicSmemBytes = sizeof(SortShared);
+        cfg.stream = s;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {cluster, 1, 1};
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        OXZ_CUDA(cudaLaunchKernelEx(&cfg, k_embed_sort, ids, (uint32_t)n, (uint32_t)d.vocab, passes, bits, e->sorted[0], e->sorted[1],
+                                    static_cast<unsigned char*>(d_table), fill_bytes));
+        if (n) {
+            const unsigned long long* sorted = e->sorted[passes & 1];
+            const bool wide = !misaligned(d_out, 16) && !misaligned(d_table, 16) && d.hidden * es % 16 == 0 && d_out_stride * es % 16 == 0;
+            const uint32_t m = (uint32_t)n;
+            const uint64_t st = d_out_stride;
+            const bool f32g = d.grad_dtype == OXZ_F32;
+            if (d.dtype == OXZ_F32) wide ? (sums<float, float, 4>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<float, float, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
+            else if (d.dtype == OXZ_BF16 && !f32g) wide ? (sums<__nv_bfloat16, __nv_bfloat16, 8>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<__nv_bfloat16, __nv_bfloat16, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
+            else if (d.dtype == OXZ_BF16) wide ? (sums<__nv_bfloat16, float, 8>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<__nv_bfloat16, float, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
+            else if (!f32g) wide ? (sums<__half, __half, 8>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<__half, __half, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
+            else wide ? (sums<__half, float, 8>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<__half, float, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
+        }
+        OXZ_CUDA(cudaGetLastError());
+        return e->order.end(s);
+    });
+}
+
+}  // extern "C"

@@ -48,6 +48,62 @@ inline int32_t guarded(const char* who, F&& body) noexcept {
         if (s__ != OXZ_OK) return s__; \
     } while (0)
 
+// Makes `device` current for the calling thread until the end of the scope, then puts back what was.
+struct DeviceGuard {
+    int before = -1;
+    int32_t enter(int device) {
+        int now = -1;
+        OXZ_CUDA(cudaGetDevice(&now));
+        if (now == device) return OXZ_OK;
+        const cudaError_t e = cudaSetDevice(device);
+        if (e != cudaSuccess) {
+            (void)cudaGetLastError();  // the refusal is reported here, not again by a later call
+            return fail(OXZ_ERR_CUDA, "device %d cannot be used: %s", device, cudaGetErrorString(e));
+        }
+        before = now;
+        return OXZ_OK;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// Orders the calls of a handle whose workspace they share: a call waits for the one before it, whatever stream that used. A
+// call that is being captured into a graph is left out: an event of the running stream cannot be waited for in a capture, and a
+// replay's place is the replaying program's business.
+struct StreamOrder {
+    cudaEvent_t done = nullptr;
+    bool used = false;
+    int32_t create() {
+        if (!done) OXZ_CUDA(cudaEventCreateWithFlags(&done, cudaEventDisableTiming));
+        return OXZ_OK;
+    }
+    void destroy() {
+        if (done) cudaEventDestroy(done);
+        done = nullptr;
+    }
+    static int32_t capturing(cudaStream_t s, bool* yes) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        OXZ_CUDA(cudaStreamIsCapturing(s, &st));
+        *yes = st != cudaStreamCaptureStatusNone;
+        return OXZ_OK;
+    }
+    int32_t begin(cudaStream_t s) {
+        bool captured = false;
+        OXZ_TRY(capturing(s, &captured));
+        if (!captured && used) OXZ_CUDA(cudaStreamWaitEvent(s, done, 0));
+        return OXZ_OK;
+    }
+    int32_t end(cudaStream_t s) {
+        bool captured = false;
+        OXZ_TRY(capturing(s, &captured));
+        if (captured) return OXZ_OK;
+        OXZ_CUDA(cudaEventRecord(done, s));
+        used = true;
+        return OXZ_OK;
+    }
+};
+
 constexpr uint32_t TILE = 256;           // elements per tile: one 8-element vector per lane of a warp
 constexpr uint32_t MAX_GROUPS = 8;       // distinct (lr_scale, decay) groups a plan may hold
 constexpr uint32_t PAD_TILE = 0xFFFFFFFFu;  // tile_meta of a tile past the last tensor

@@ -487,6 +487,55 @@ class LitDataLoader:
             self._h = C.c_void_p()
 
 
+# ------------------------------------------------------------------ the token operators
+def _ptr(address: int | None):
+    return C.c_void_p(address) if address else None
+
+
+class TokenEmbedding:
+    """The token embedding and its gradient (embed_tokens, [vocab, hidden]): ``out[i] = scale * table[ids[i]]`` and
+    ``d_table[v] = scale * sum of d_out[i] over the tokens i with ids[i] = v``. All arguments are device addresses; sums run
+    in f32 in the order of the tokens, so equal inputs give equal bits. An id outside the table reads as zeros and receives
+    no gradient."""
+
+    def __init__(self, vocab: int, hidden: int, max_tokens: int, dtype: int = BF16, grad_dtype: int | None = None,
+                 scale: float = 1.0, device: int = 0, allocate: bool = True):
+        self.vocab, self.hidden, self.max_tokens, self.scale = vocab, hidden, max_tokens, scale
+        self.dtype, self.grad_dtype, self.device = dtype, dtype if grad_dtype is None else grad_dtype, device
+        desc = ffi.EmbedDesc(max_tokens, hidden, vocab, scale, dtype, self.grad_dtype, device, 0)
+        self._h = C.c_void_p()
+        check(lib().oxz_embed_create(C.byref(desc), C.byref(self._h)))
+        self.workspace_bytes = 0
+        if allocate:
+            self.alloc()
+
+    def alloc(self) -> None:
+        """The workspace of the gradient; a handle that only looks up needs none."""
+        v = C.c_uint64()
+        check(lib().oxz_embed_alloc(self._h, C.byref(v)))
+        self.workspace_bytes = v.value
+
+    def lookup(self, ids: int, n: int, table: int, out: int, out_stride: int = 0, stream: int | None = None) -> None:
+        check(lib().oxz_embed_lookup_async(self._h, _ptr(ids), n, _ptr(table), _ptr(out), out_stride, _ptr(stream)))
+
+    def grads(self, ids: int, n: int, d_out: int, d_table: int, accumulate: bool = False, d_out_stride: int = 0,
+              stream: int | None = None) -> None:
+        """accumulate False writes every row of d_table (zeros where no token is), True adds to the rows that have tokens."""
+        check(lib().oxz_embed_grads_async(self._h, _ptr(ids), n, _ptr(d_out), d_out_stride, _ptr(d_table), int(accumulate),
+                                          _ptr(stream)))
+
+    def destroy(self) -> None:
+        if self._h:
+            lib().oxz_embed_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
 # ------------------------------------------------------------------ the checkpoint meta's keys on this path
 @dataclass
 class SpikeGuardState:

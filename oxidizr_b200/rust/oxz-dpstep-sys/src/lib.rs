@@ -79,6 +79,11 @@ pub struct oxz_loader {
     _private: [u8; 0],
 }
 
+#[repr(C)]
+pub struct oxz_embed {
+    _private: [u8; 0],
+}
+
 /// `run_ranks` body: called once per rank with (rank, world, user); non-zero = that rank failed.
 pub type oxz_rank_body = Option<unsafe extern "C" fn(rank: i32, world: i32, user: *mut c_void) -> i32>;
 
@@ -256,6 +261,19 @@ pub struct oxz_batch_masks {
     pub cu_seqlens: *const i32,
     pub scored: *const u64,
     pub n_segments: *const u64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct oxz_embed_desc {
+    pub max_tokens: u64,
+    pub hidden: u64,
+    pub vocab: u64,
+    pub scale: f64,
+    pub dtype: i32,
+    pub grad_dtype: i32,
+    pub device: i32,
+    pub reserved: i32,
 }
 
 extern "C" {
@@ -551,6 +569,28 @@ extern "C" {
         inputs: *mut *mut i64,
         targets: *mut *mut i64,
         rows: *mut u64,
+    ) -> i32;
+    pub fn oxz_embed_create(desc: *const oxz_embed_desc, out: *mut *mut oxz_embed) -> i32;
+    pub fn oxz_embed_alloc(embed: *mut oxz_embed, workspace_bytes: *mut u64) -> i32;
+    pub fn oxz_embed_destroy(embed: *mut oxz_embed) -> i32;
+    pub fn oxz_embed_lookup_async(
+        embed: *const oxz_embed,
+        ids: *const i64,
+        n: u64,
+        table: *const c_void,
+        out: *mut c_void,
+        out_stride: u64,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn oxz_embed_grads_async(
+        embed: *mut oxz_embed,
+        ids: *const i64,
+        n: u64,
+        d_out: *const c_void,
+        d_out_stride: u64,
+        d_table: *mut c_void,
+        accumulate: i32,
+        stream: *mut c_void,
     ) -> i32;
     pub fn oxz_step_weighting(
         local_micro_batches: u64,
