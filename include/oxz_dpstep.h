@@ -566,6 +566,70 @@ int32_t oxz_embed_lookup_async(const oxz_embed* embed, const int64_t* ids, uint6
 int32_t oxz_embed_grads_async(oxz_embed* embed, const int64_t* ids, uint64_t n, const void* d_out, uint64_t d_out_stride,
                               void* d_table, int32_t accumulate, void* stream);
 
+/* ------------------------------------------------------------------ the loss head
+ *
+ * Softmax cross entropy over a large vocabulary on top of the last hidden states, with its gradients, without keeping the
+ * logits: the vocabulary is taken in pieces, and a piece's logits live only inside a kernel. It stands between the loader's
+ * targets and loss mask and the flat buffers: the weight is work + offsets[lm_head] (or of embed_tokens where the two are
+ * tied, src/model.rs:3798-3802), its gradient goes to grads + offsets[lm_head], the loss is what a training step is given
+ * (src/step_loss.rs, src/trainer.rs:373-502).
+ *
+ *   l[i][v]  = sum over h of hidden[i][h] * weight[v][h]
+ *   loss[i]  = log(sum over v of exp(l[i][v])) - l[i][targets[i]]
+ *   g[i][v]  = loss_mask[i] * (exp(l[i][v]) / (sum over u of exp(l[i][u])) - (v == targets[i] ? 1 : 0))
+ *   d_hidden = grad_scale * g weight          d_weight = grad_scale * g^T hidden   (+ what d_weight held, when accumulating)
+ *
+ * A row is scored when its loss_mask is not zero and its target lies in [0, vocab). Nothing of another row is used - not its
+ * hidden state either, which may hold anything - and it gets loss 0, statistics 0 and a gradient of zeros.
+ * Products are summed in f32 and softmax statistics kept in f32. g is rounded to dtype before it is multiplied (f16: scaled by a
+ * power of two into its range first); d_hidden and d_weight are rounded once. There are no atomics: equal inputs give equal bits.
+ * The handle holds the workspace. It is used by one thread at a time; calls on different streams are ordered by the handle, but
+ * graphs captured from its calls share the workspace, so their replays must not overlap each other or other calls of the
+ * handle. No call allocates, synchronises or copies to the host. */
+typedef struct oxz_head oxz_head;
+typedef struct oxz_head_desc {
+    uint64_t max_rows;     /* the most tokens of one call, below 2^31 */
+    uint64_t hidden;       /* elements of a row */
+    uint64_t vocab;        /* rows of the weight, below 2^31 */
+    uint64_t piece_bytes;  /* the most workspace for one piece's gradient of the logits; 0 = 512 MiB */
+    int32_t dtype;         /* oxz_dtype of hidden, weight and d_hidden */
+    int32_t grad_dtype;    /* oxz_dtype of d_weight: dtype or OXZ_F32 */
+    int32_t device;        /* CUDA device ordinal */
+    int32_t reserved;      /* 0 */
+} oxz_head_desc;
+int32_t oxz_head_create(const oxz_head_desc* desc, oxz_head** out); /* host only: runs without a GPU */
+/* Allocates the workspace on the device; *workspace_bytes (may be NULL) receives its size. */
+int32_t oxz_head_alloc(oxz_head* head, uint64_t* workspace_bytes);
+int32_t oxz_head_destroy(oxz_head* head);
+/* One batch. All pointers are device memory, aligned to their element (weight: to 16 bytes, as every tensor of a plan is). */
+typedef struct oxz_head_batch {
+    uint64_t rows;           /* tokens; 0 is allowed */
+    const void* hidden;      /* rows of `hidden` elements, hidden_stride elements apart */
+    uint64_t hidden_stride;  /* 0: hidden */
+    const void* weight;      /* [vocab, hidden], without gaps */
+    const int64_t* targets;  /* [rows], as the loader hands them */
+    const float* loss_mask;  /* [rows]; NULL: every row counts once */
+} oxz_head_batch;
+typedef struct oxz_head_grads {
+    void* d_hidden;            /* NULL: not wanted */
+    uint64_t d_hidden_stride;  /* 0: hidden */
+    void* d_weight;            /* [vocab, hidden] of grad_dtype, aligned to 16 bytes; NULL: not wanted */
+    double grad_scale;         /* the loss scale times the step's weight of this batch; applied in f32 */
+    int32_t accumulate;        /* d_weight: 0 = written whole, 1 = added in f32 to what it holds */
+    int32_t reserved;          /* 0 */
+} oxz_head_grads;
+/* Losses only (a held-out pass). row_loss [rows] f32, row_stats [rows][2] f32 {largest logit, sum of exp(logit - largest)} and
+ * totals [2] f32 {sum of loss_mask * loss, sum of loss_mask, over the scored rows; summed in f64} may each be NULL. */
+int32_t oxz_head_loss_async(oxz_head* head, const oxz_head_batch* batch, float* row_loss, float* row_stats, float* totals,
+                            void* stream);
+/* Gradients from the statistics that oxz_head_loss_async wrote for the same batch (when grad_scale is known only after the
+ * losses of every micro-batch). */
+int32_t oxz_head_grads_async(oxz_head* head, const oxz_head_batch* batch, const float* row_stats, const oxz_head_grads* grads,
+                             void* stream);
+/* Both in one call, with the same results. */
+int32_t oxz_head_loss_grads_async(oxz_head* head, const oxz_head_batch* batch, float* row_loss, float* row_stats, float* totals,
+                                  const oxz_head_grads* grads, void* stream);
+
 /* StepWeighting::over_ranks applied to the summed counts (src/dp/weighting.rs:46-61): counts = {scored, masked ranks}
  * after oxz_allreduce_i64x2. *global_scored = -1 for an unmasked step. Mixed masks are OXZ_ERR_INVALID on every rank. */
 int32_t oxz_step_weighting(uint64_t local_micro_batches, int32_t world, const int64_t counts[2],

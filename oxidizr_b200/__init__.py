@@ -6,7 +6,7 @@ This package binds it with ctypes and mirrors the reference's host-side interfac
 from ._ffi import BF16, F16, F32, SYNC_COPY, SYNC_NCCL, SYNC_P2P, SYNC_REPLICATED, SYNC_SINGLE, OxzError, lib  # noqa: F401
 from . import _ffi as ffi  # noqa: F401
 from .dpstep import (CheckpointMeta, MixtureRecord, check_mixture_resume, Communicator, DataPosition, DecayPlan, DpOptimizer, GradScalerState, LitDataLoader, LitTrainerStep,  # noqa: F401
-                     LossScaleConfig, LossScaler, LrPlan, RowLayout, SpikeGuard, SpikeGuardConfig, SpikeGuardState, StepConfig,
+                     LossHead, LossScaleConfig, LossScaler, LrPlan, RowLayout, SpikeGuard, SpikeGuardConfig, SpikeGuardState, StepConfig,
                      TensorInfo, TokenEmbedding, TrainerConfig, WeightDecaySpec, check_resume_world, compute_grad_norm, mixture_quotas,
                      compute_grad_norm_static, diagnose_bad_gradients, read_loss_scale_state, run_ranks, selftest_bounded_wait,
                      step_weighting)

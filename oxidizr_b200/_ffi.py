@@ -107,6 +107,21 @@ class EmbedDesc(C.Structure):
                 ("dtype", C.c_int32), ("grad_dtype", C.c_int32), ("device", C.c_int32), ("reserved", C.c_int32)]
 
 
+class HeadDesc(C.Structure):
+    _fields_ = [("max_rows", C.c_uint64), ("hidden", C.c_uint64), ("vocab", C.c_uint64), ("piece_bytes", C.c_uint64),
+                ("dtype", C.c_int32), ("grad_dtype", C.c_int32), ("device", C.c_int32), ("reserved", C.c_int32)]
+
+
+class HeadBatch(C.Structure):
+    _fields_ = [("rows", C.c_uint64), ("hidden", C.c_void_p), ("hidden_stride", C.c_uint64), ("weight", C.c_void_p),
+                ("targets", C.c_void_p), ("loss_mask", C.c_void_p)]
+
+
+class HeadGrads(C.Structure):
+    _fields_ = [("d_hidden", C.c_void_p), ("d_hidden_stride", C.c_uint64), ("d_weight", C.c_void_p), ("grad_scale", C.c_double),
+                ("accumulate", C.c_int32), ("reserved", C.c_int32)]
+
+
 RankBody = C.CFUNCTYPE(C.c_int32, C.c_int32, C.c_int32, C.c_void_p)
 
 # name -> (restype, argtypes): one row per declaration of include/oxz_dpstep.h
@@ -213,6 +228,12 @@ SIGNATURES = {
     "oxz_embed_destroy": (C.c_int32, [vp]),
     "oxz_embed_lookup_async": (C.c_int32, [vp, vp, C.c_uint64, vp, vp, C.c_uint64, vp]),
     "oxz_embed_grads_async": (C.c_int32, [vp, vp, C.c_uint64, vp, C.c_uint64, vp, C.c_int32, vp]),
+    "oxz_head_create": (C.c_int32, [C.POINTER(HeadDesc), C.POINTER(vp)]),
+    "oxz_head_alloc": (C.c_int32, [vp, u64p]),
+    "oxz_head_destroy": (C.c_int32, [vp]),
+    "oxz_head_loss_async": (C.c_int32, [vp, C.POINTER(HeadBatch), vp, vp, vp, vp]),
+    "oxz_head_grads_async": (C.c_int32, [vp, C.POINTER(HeadBatch), vp, C.POINTER(HeadGrads), vp]),
+    "oxz_head_loss_grads_async": (C.c_int32, [vp, C.POINTER(HeadBatch), vp, vp, vp, C.POINTER(HeadGrads), vp]),
     "oxz_step_weighting": (C.c_int32, [C.c_uint64, C.c_int32, i64p, u64p, i64p]),
 }
 

@@ -536,6 +536,65 @@ class TokenEmbedding:
             pass
 
 
+class LossHead:
+    """Softmax cross entropy over a large vocabulary on the last hidden states, with its gradients, without keeping the logits
+    (the step loss of src/step_loss.rs over lm_head, or over embed_tokens where the two are tied). All arguments are device
+    addresses. A row is scored when its ``loss_mask`` (None: all ones) is not zero and its target lies in ``[0, vocab)``; other
+    rows get loss 0 and a gradient of zeros, whatever their hidden state holds."""
+
+    def __init__(self, vocab: int, hidden: int, max_rows: int, dtype: int = BF16, grad_dtype: int | None = None,
+                 device: int = 0, piece_bytes: int = 0, allocate: bool = True):
+        self.vocab, self.hidden, self.max_rows = vocab, hidden, max_rows
+        self.dtype, self.grad_dtype, self.device = dtype, dtype if grad_dtype is None else grad_dtype, device
+        desc = ffi.HeadDesc(max_rows, hidden, vocab, piece_bytes, dtype, self.grad_dtype, device, 0)
+        self._h = C.c_void_p()
+        check(lib().oxz_head_create(C.byref(desc), C.byref(self._h)))
+        self.workspace_bytes = 0
+        if allocate:
+            self.alloc()
+
+    def alloc(self) -> None:
+        v = C.c_uint64()
+        check(lib().oxz_head_alloc(self._h, C.byref(v)))
+        self.workspace_bytes = v.value
+
+    def loss(self, rows: int, hidden: int, weight: int, targets: int, loss_mask: int | None = None, row_loss: int | None = None,
+             row_stats: int | None = None, totals: int | None = None, hidden_stride: int = 0, stream: int | None = None) -> None:
+        """Losses only. ``row_loss`` [rows] f32, ``row_stats`` [rows, 2] f32 and ``totals`` [2] f32 (sum of mask * loss, sum of
+        mask) are each written when given."""
+        b = ffi.HeadBatch(rows, hidden, hidden_stride, weight, targets, loss_mask)
+        check(lib().oxz_head_loss_async(self._h, C.byref(b), row_loss, row_stats, totals, stream))
+
+    def grads(self, rows: int, hidden: int, weight: int, targets: int, row_stats: int, loss_mask: int | None = None,
+              d_hidden: int | None = None, d_weight: int | None = None, grad_scale: float = 1.0, accumulate: bool = False,
+              hidden_stride: int = 0, d_hidden_stride: int = 0, stream: int | None = None) -> None:
+        """Gradients from the statistics ``loss`` wrote for the same batch. ``accumulate``: add to what ``d_weight`` holds."""
+        b = ffi.HeadBatch(rows, hidden, hidden_stride, weight, targets, loss_mask)
+        g = ffi.HeadGrads(d_hidden, d_hidden_stride, d_weight, grad_scale, int(accumulate), 0)
+        check(lib().oxz_head_grads_async(self._h, C.byref(b), row_stats, C.byref(g), stream))
+
+    def loss_and_grads(self, rows: int, hidden: int, weight: int, targets: int, loss_mask: int | None = None,
+                       row_loss: int | None = None, row_stats: int | None = None, totals: int | None = None,
+                       d_hidden: int | None = None, d_weight: int | None = None, grad_scale: float = 1.0,
+                       accumulate: bool = False, hidden_stride: int = 0, d_hidden_stride: int = 0,
+                       stream: int | None = None) -> None:
+        """``loss`` and ``grads`` in one call, with the same results."""
+        b = ffi.HeadBatch(rows, hidden, hidden_stride, weight, targets, loss_mask)
+        g = ffi.HeadGrads(d_hidden, d_hidden_stride, d_weight, grad_scale, int(accumulate), 0)
+        check(lib().oxz_head_loss_grads_async(self._h, C.byref(b), row_loss, row_stats, totals, C.byref(g), stream))
+
+    def destroy(self) -> None:
+        if self._h:
+            lib().oxz_head_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
 # ------------------------------------------------------------------ the checkpoint meta's keys on this path
 @dataclass
 class SpikeGuardState:

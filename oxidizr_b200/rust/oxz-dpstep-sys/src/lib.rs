@@ -84,6 +84,11 @@ pub struct oxz_embed {
     _private: [u8; 0],
 }
 
+#[repr(C)]
+pub struct oxz_head {
+    _private: [u8; 0],
+}
+
 /// `run_ranks` body: called once per rank with (rank, world, user); non-zero = that rank failed.
 pub type oxz_rank_body = Option<unsafe extern "C" fn(rank: i32, world: i32, user: *mut c_void) -> i32>;
 
@@ -273,6 +278,41 @@ pub struct oxz_embed_desc {
     pub dtype: i32,
     pub grad_dtype: i32,
     pub device: i32,
+    pub reserved: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct oxz_head_desc {
+    pub max_rows: u64,
+    pub hidden: u64,
+    pub vocab: u64,
+    pub piece_bytes: u64,
+    pub dtype: i32,
+    pub grad_dtype: i32,
+    pub device: i32,
+    pub reserved: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct oxz_head_batch {
+    pub rows: u64,
+    pub hidden: *const c_void,
+    pub hidden_stride: u64,
+    pub weight: *const c_void,
+    pub targets: *const i64,
+    pub loss_mask: *const f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct oxz_head_grads {
+    pub d_hidden: *mut c_void,
+    pub d_hidden_stride: u64,
+    pub d_weight: *mut c_void,
+    pub grad_scale: f64,
+    pub accumulate: i32,
     pub reserved: i32,
 }
 
@@ -590,6 +630,33 @@ extern "C" {
         d_out_stride: u64,
         d_table: *mut c_void,
         accumulate: i32,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn oxz_head_create(desc: *const oxz_head_desc, out: *mut *mut oxz_head) -> i32;
+    pub fn oxz_head_alloc(head: *mut oxz_head, workspace_bytes: *mut u64) -> i32;
+    pub fn oxz_head_destroy(head: *mut oxz_head) -> i32;
+    pub fn oxz_head_loss_async(
+        head: *mut oxz_head,
+        batch: *const oxz_head_batch,
+        row_loss: *mut f32,
+        row_stats: *mut f32,
+        totals: *mut f32,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn oxz_head_grads_async(
+        head: *mut oxz_head,
+        batch: *const oxz_head_batch,
+        row_stats: *const f32,
+        grads: *const oxz_head_grads,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn oxz_head_loss_grads_async(
+        head: *mut oxz_head,
+        batch: *const oxz_head_batch,
+        row_loss: *mut f32,
+        row_stats: *mut f32,
+        totals: *mut f32,
+        grads: *const oxz_head_grads,
         stream: *mut c_void,
     ) -> i32;
     pub fn oxz_step_weighting(
