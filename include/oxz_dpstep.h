@@ -585,7 +585,8 @@ int32_t oxz_embed_grads_async(oxz_embed* embed, const int64_t* ids, uint64_t n, 
  * power of two into its range first); d_hidden and d_weight are rounded once. There are no atomics: equal inputs give equal bits.
  * The handle holds the workspace. It is used by one thread at a time; calls on different streams are ordered by the handle, but
  * graphs captured from its calls share the workspace, so their replays must not overlap each other or other calls of the
- * handle. No call allocates, synchronises or copies to the host. */
+ * handle. No call allocates, synchronises or copies to the host. OXZ_ERR_TIMEOUT: a bounded wait inside a kernel of an earlier call
+ * ran out, its results are not valid, and the handle serves no further call. */
 typedef struct oxz_head oxz_head;
 typedef struct oxz_head_desc {
     uint64_t max_rows;     /* the most tokens of one call, below 2^31 */

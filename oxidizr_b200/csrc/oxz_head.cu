@@ -9,9 +9,13 @@
 // every product runs over the list.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
+
+#include <cuda.h>
 
 #include "oxz_elem.cuh"
 #include "oxz_internal.h"
+#include "oxz_tcgen05.cuh"
 
 namespace oxz {
 
@@ -20,6 +24,7 @@ struct HeadMeta {
     uint32_t n;          // scored rows
     uint32_t done;       // blocks of k_head_finish that have added their part (put back to 0 by the last)
     double weight_sum;   // of the scored rows
+    float up, down;      // power of two G is scaled by before it is rounded (f16 only), and its inverse
 };
 
 }  // namespace oxz
@@ -31,13 +36,22 @@ struct oxz_head {
     uint64_t piece = 0;              // columns of the vocabulary in a piece
     int32_t* row_of = nullptr;       // [max_rows] slot -> row of the batch, scored rows in order
     int32_t* slot_of = nullptr;      // [max_rows] row -> slot, -1: not scored
-    float2* part = nullptr;          // [tiles][max_rows] {max, sum of exp} of a slot over one tile of the vocabulary
+    float2* part = nullptr;          // [2 * tiles][max_rows] {max, sum of exp} of a slot over half a tile of the vocabulary
     float* target_logit = nullptr;   // [max_rows] by slot
     float2* stats = nullptr;         // [max_rows] by row, where the caller keeps none
     double* loss_part = nullptr;     // [blocks of k_head_finish]
     oxz::HeadMeta* meta = nullptr;
-    float* g = nullptr;              // [max_rows][piece]
-    float* dx = nullptr;             // [max_rows][hidden] sum over the pieces
+    uint64_t cap = 0;                // max_rows up to a multiple of a tile
+    uint32_t pitch = 0;              // elements of a packed row: hidden up to 16 bytes
+    uint32_t dx_pitch = 0;           // of a row of dx
+    int parts = 1, g_parts = 1;      // 16-bit parts of an operand, and of G
+    int clusters = 0;                // pairs of SMs the device runs at once
+    void* x = nullptr;               // [parts][cap][pitch] packed hidden states
+    void* w = nullptr;               // [parts][vocab][pitch] packed weight, where TMA cannot read the caller's
+    void* g = nullptr;               // [g_parts][cap][piece]
+    float* dx = nullptr;             // [splits][rows][dx_pitch] sums over the pieces
+    int32_t* expired = nullptr;      // mapped host memory: a bounded wait inside a kernel ran out
+    int32_t* d_expired = nullptr;
     oxz::StreamOrder order;
 };
 
@@ -45,22 +59,26 @@ namespace oxz {
 namespace {
 
 constexpr int FINISH_ROWS = 8;  // rows a block of k_head_finish takes: one per warp
+constexpr uint32_t MMA_M = 256, MMA_N = 256, MMA_K = 64;  // tile of a pair of SMs
 
 // ---- the scored rows, in order. One block: each thread counts a run of rows, a scan over the threads places them.
 __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ targets, const float* __restrict__ mask, uint32_t rows,
-                                                    uint64_t vocab, int32_t* row_of, int32_t* slot_of, HeadMeta* meta) {
+                                                    uint64_t vocab, int32_t* row_of, int32_t* slot_of, HeadMeta* meta, int f16) {
     __shared__ uint32_t scan[32];
     __shared__ double wsum[32];
+    __shared__ float wtop[32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const uint32_t each = (rows + 1023) / 1024;
     const uint32_t lo = min(rows, threadIdx.x * each), hi = min(rows, lo + each);
     uint32_t count = 0;
     double w = 0.0;
+    float top = 0.f;
     auto scored = [&](uint32_t i) { return (mask == nullptr || mask[i] != 0.f) && (uint64_t)targets[i] < vocab; };
     for (uint32_t i = lo; i < hi; i++)
         if (scored(i)) {
             count++;
             w += mask ? (double)mask[i] : 1.0;
+            top = fmaxf(top, mask ? fabsf(mask[i]) : 1.f);
         }
     uint32_t inc = count;
 #pragma unroll
@@ -69,9 +87,15 @@ __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ 
         if (lane >= (uint32_t)o) inc += up;
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    for (int o = 16; o; o >>= 1) {
+        w += __shfl_xor_sync(0xffffffffu, w, o);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
     if (lane == 31) scan[warp] = inc;
-    if (lane == 0) wsum[warp] = w;
+    if (lane == 0) {
+        wsum[warp] = w;
+        wtop[warp] = top;
+    }
     __syncthreads();
     if (warp == 0) {
         uint32_t v = scan[lane];
@@ -83,10 +107,18 @@ __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ 
         scan[lane] = v;
         if (lane == 31) {
             double total = 0.0;
-            for (int k = 0; k < 32; k++) total += wsum[k];
+            for (int k = 0; k < 32; k++) {
+                total += wsum[k];
+                top = fmaxf(top, wtop[k]);
+            }
             meta->n = v;
             meta->done = 0;
             meta->weight_sum = total;
+            // f16 holds 2^-24 .. 65504: the largest weight times one goes to 2^13 .. 2^14, so that probabilities down to 2^-27 of it
+            // stay normal numbers
+            const int up = f16 && top > 0.f && isfinite(top) ? 13 - ilogbf(top) : 0;
+            meta->up = exp2f((float)min(max(up, -100), 100));
+            meta->down = exp2f((float)-min(max(up, -100), 100));
         }
     }
     __syncthreads();
@@ -152,189 +184,528 @@ __global__ void __launch_bounds__(32 * FINISH_ROWS) k_head_finish(uint32_t rows,
     }
 }
 
-// ---- the four products, one output tile of 64 x 64 per block, summed in f32 over steps of 16
+// ---- the scored rows' hidden states, packed for the products: [part][slot][pitch] 16-bit values, zeros to the end of the pitch and
+// in the rows up to the next multiple of a tile, which the products read. An f32 is the sum of three bf16 of 8 bits each (cut, not
+// rounded, so that no part leaves the range); 16-bit values are copied.
+template <typename T, typename S>
+__device__ __forceinline__ void pack_piece(const float (&v)[8], S* out, uint64_t part_stride, int parts) {
+    float rest[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) rest[j] = v[j];
+    for (int p = 0; p < parts; p++) {
+        Vec<S, 8> o;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (sizeof(T) == 4) {
+                float hi = __uint_as_float(__float_as_uint(rest[j]) & 0xffff0000u);
+                rest[j] = isfinite(v[j]) ? rest[j] - hi : 0.f;  // an infinity or a NaN is its first part alone
+                // no part of a value is zero where the value is not: times an infinity it would make a NaN of it
+                if (hi == 0.f && isfinite(v[j]) && fabsf(v[j]) > 0x1p-100f) hi = copysignf(0x1p-126f, v[j]);
+                o.e[j] = from_f32<S>(hi);
+            } else {
+                o.e[j] = from_f32<S>(v[j]);
+            }
+        }
+        o.store(out + p * part_stride);
+    }
+}
+// rows: the packed rows (row_of null: row i is source row i, `rows` of them; else the scored ones and zeros to the next multiple of 256)
+template <typename T, typename S>
+__global__ void __launch_bounds__(256) k_head_pack(const T* __restrict__ src, uint64_t stride, uint32_t hidden, uint32_t pitch, uint64_t rows,
+                                                   const int32_t* __restrict__ row_of, const HeadMeta* __restrict__ meta, S* out,
+                                                   uint64_t part_stride, int parts, int wide) {
+    const uint32_t n = row_of ? meta->n : (uint32_t)rows, per = pitch / 8;
+    const uint64_t total = (row_of ? (uint64_t)(n + MMA_M - 1) / MMA_M * MMA_M : rows) * per;
+    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
+        const uint64_t slot = e / per;
+        const uint32_t col = (uint32_t)(e - slot * per) * 8;
+        float v[8];
+        if (slot >= n) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = 0.f;
+        } else {
+            const T* from = src + (row_of ? (uint64_t)row_of[slot] : slot) * stride + col;
+            if (wide && col + 8 <= hidden) {
+                Vec<T, 8> x;
+                x.load(from);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = to_f32<T>(x.e[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = col + j < hidden ? to_f32<T>(from[j]) : 0.f;
+            }
+        }
+        pack_piece<T, S>(v, out + slot * pitch + col, part_stride, parts);
+    }
+}
+
+// ---- the four products on the tensor cores.
+//
+// A pair of SMs works on one output tile of 256 x 256 (cta_group::2): each holds 128 rows of A and of the accumulator and half of B's
+// rows, so that a step of 64 in K costs an SM 32 KiB from L2 for 2 x 256 x 128 x 64 operations. One thread per SM keeps STAGES
+// steps of both operands in flight by TMA, one thread of the pair issues the products, eight warps per SM take the finished tile
+// from tensor memory while the other of its two buffers fills.
+//   LOGITS_STATS  l = X W^T: each row's {max, sum of exp} over half a tile's columns goes out, and the target's logit
+//   LOGITS_GRAD   the same tile, turned into G
+//   D_HIDDEN      G W, summed over the pieces in f32 (each split of K in a slab of its own)
+//   D_WEIGHT      G^T X
+// Operands come as K runs in memory: G and X are K-major in the first three, W in the first two; the others are read with K along
+// the lines of their tiles. Values of more than 16 bits come in parts; a product of such operands is the sum over `pairs` of parts.
 enum Product { LOGITS_STATS, LOGITS_GRAD, D_HIDDEN, D_WEIGHT };
+constexpr int STAGES = 6, MMA_THREADS = 320, EPILOGUE_WARPS = 8;
+constexpr uint32_t STAGE_BYTES = 4 * BOX_BYTES, MMA_SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+
 struct ProductArgs {
     const HeadMeta* meta;
     const int32_t* row_of;
-    const void* x;
-    uint64_t x_stride;
-    const void* w;
-    uint32_t hidden, vocab, first, columns, pitch, tiles;  // the piece [first, first + columns) of the vocabulary
+    uint32_t hidden, first, columns, pitch, g_pitch, dx_pitch, splits;  // the piece [first, first + columns) of the vocabulary
+    uint64_t g_part, dx_slab;
     const int64_t* targets;
     const float* mask;
     const float2* stats;
     float2* part;
     float* target_logit;
-    float* g;
+    void* g;
     float* dx;
     void* dw;
     float scale;
-    int accumulate, add;
+    int accumulate, add, bf16, n_pairs;
+    uint8_t pair_a[6], pair_b[6];
+    int32_t* expired;
 };
 
-template <typename T, typename G, int P>
-__global__ void __launch_bounds__(256) k_head_product(const ProductArgs a) {
-    __shared__ float sa[16][65], sb[16][65];
-    const uint32_t n = a.meta->n, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const uint32_t i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
+// exp(x - m). f32 results take the library's exponential. For 16-bit operands the unit's 2^x of one fused product is ample: it is
+// off by 2^-22 and by 2^-24 |m log2 e| relatively, where the operands themselves are rounded to 2^-9 or 2^-12.
+constexpr float LOG2E = 1.4426950408889634f;
+template <bool EXACT> struct ExpFrom {
+    float m;
+    __device__ __forceinline__ explicit ExpFrom(float at) : m(EXACT ? at : at * LOG2E) {}
+    __device__ __forceinline__ float operator()(float x) const {
+        if constexpr (EXACT) return expf(x - m);
+        float r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(x, LOG2E, -m)));
+        return r;
+    }
+};
+
+// T: type of the operands, S: type of the parts they come in, G: type of d_weight; PARTS: parts of G
+template <typename T, typename S, typename G, int P, int PARTS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
+    k_head_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a) {
+    constexpr bool A_LINES = P == D_WEIGHT, B_LINES = P == D_HIDDEN || P == D_WEIGHT;
+    extern __shared__ __align__(16) unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+    const uint32_t bars = base + STAGES * STAGE_BYTES;
+    auto full = [&](uint32_t i) { return bars + 8 * i; };
+    auto empty = [&](uint32_t i) { return bars + 8 * (STAGES + i); };
+    auto done = [&](uint32_t i) { return bars + 8 * (2 * STAGES + i); };       // a tile is in accumulator buffer i
+    auto taken = [&](uint32_t i) { return bars + 8 * (2 * STAGES + 2 + i); };  // ... and has been read out by both blocks
+    __shared__ uint32_t tmem_at, dead;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, rank = cluster_rank();
+    const WaitState ws{&dead, a.expired};
+
+    if (threadIdx.x == 0) {
+        dead = 0;
+        for (int i = 0; i < STAGES; i++) {
+            mbar_init(full(i), 1);
+            mbar_init(empty(i), 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(done(i), 1);
+            mbar_init(taken(i), 2 * EPILOGUE_WARPS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tma_prefetch_map(&map_a);
+        tma_prefetch_map(&map_b);
+    }
+    if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_at), 512);
+    fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_at);
+
+    const uint32_t n = a.meta->n;
     const uint32_t M = P == D_WEIGHT ? a.columns : n, N = P == LOGITS_STATS || P == LOGITS_GRAD ? a.columns : a.hidden;
     const uint32_t K = P == D_HIDDEN ? a.columns : P == D_WEIGHT ? n : a.hidden;
-    if (i0 >= M) return;
-    const T* x = static_cast<const T*>(a.x);
-    const T* w = static_cast<const T*>(a.w);
-    float acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < K; k0 += 16) {
-        for (uint32_t e = threadIdx.x; e < 1024; e += 256) {
-            // the faster index runs along memory
-            const bool k_fast = P == LOGITS_STATS || P == LOGITS_GRAD || P == D_HIDDEN;
-            const uint32_t k = k_fast ? e & 15 : e >> 6, i = k_fast ? e >> 4 : e & 63;
-            float v = 0.f;
-            if (k0 + k < K && i0 + i < M) {
-                if (P == D_HIDDEN) v = a.g[(uint64_t)(i0 + i) * a.columns + k0 + k];
-                else if (P == D_WEIGHT) v = a.g[(uint64_t)(k0 + k) * a.columns + i0 + i];
-                else v = to_f32<T>(x[(uint64_t)a.row_of[i0 + i] * a.x_stride + k0 + k]);
-            }
-            sa[k][i] = v;
-            const bool bk_fast = P == LOGITS_STATS || P == LOGITS_GRAD;
-            const uint32_t kb = bk_fast ? e & 15 : e >> 6, j = bk_fast ? e >> 4 : e & 63;
-            v = 0.f;
-            if (k0 + kb < K && j0 + j < N) {
-                if (P == D_HIDDEN) v = to_f32<T>(w[(uint64_t)(a.first + k0 + kb) * a.hidden + j0 + j]);
-                else if (P == D_WEIGHT) v = to_f32<T>(x[(uint64_t)a.row_of[k0 + kb] * a.x_stride + j0 + j]);
-                else v = to_f32<T>(w[(uint64_t)(a.first + j0 + j) * a.hidden + k0 + kb]);
-            }
-            sb[kb][j] = v;
+    const uint32_t mt = (M + 255) / 256, nt = (N + 255) / 256, steps_all = (K + 63) / 64;
+    const uint32_t splits = P == D_HIDDEN ? a.splits : 1;
+    const uint32_t tiles = mt * nt * splits, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+    struct Tile {
+        uint32_t m0, n0, width, half, k0, steps, split;
+    };
+    auto tile_at = [&](uint32_t t) {
+        Tile r;
+        uint32_t m, c;
+        if (P == LOGITS_STATS || P == LOGITS_GRAD) {  // the rows run fastest: one stretch of W serves them all
+            m = t % mt;
+            c = t / mt;
+            r.split = 0;
+        } else {
+            c = t % nt;
+            const uint32_t q = t / nt;
+            m = q % mt;
+            r.split = q / mt;
         }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; k++) {
-            float p[4], q[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                p[r] = sa[k][ty * 4 + r];
-                q[r] = sb[k][tx * 4 + r];
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) acc[r][c] = fmaf(p[r], q[c], acc[r][c]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const uint32_t i = i0 + ty * 4 + r;
-        const bool in = i < M;
-        const uint32_t row = in && P != D_WEIGHT ? (uint32_t)a.row_of[i] : 0;
-        if (P == LOGITS_STATS) {
-            const int64_t t = in ? a.targets[row] : -1;
-            float2 s = make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const uint32_t v = j0 + tx * 4 + c;
-                if (in && v < N) {
-                    s.x = fmaxf(s.x, acc[r][c]);
-                    if ((int64_t)v == t) a.target_logit[i] = acc[r][c];
+        r.m0 = m * 256;
+        r.n0 = c * 256;
+        r.width = min(256u, (N - r.n0 + 31) & ~31u);
+        r.half = r.width / 2;
+        r.k0 = (uint32_t)((uint64_t)steps_all * r.split / splits);
+        r.steps = (uint32_t)((uint64_t)steps_all * (r.split + 1) / splits) - r.k0;
+        return r;
+    };
+
+    if (warp == 0 && lane == 0) {
+        // ---- loads
+        uint32_t it = 0;
+        bool ok = true;
+        for (uint32_t t = pair; t < tiles && ok; t += pairs) {
+            const Tile c = tile_at(t);
+            const uint32_t b_boxes = c.half > 64 ? 2 : 1;
+            for (uint32_t p = 0; p < (uint32_t)a.n_pairs && ok; p++) {
+                const int32_t za = a.pair_a[p], zb = a.pair_b[p];
+                for (uint32_t k = 0; k < c.steps; k++, it++) {
+                    const uint32_t st = it % STAGES, use = it / STAGES;
+                    if (!(ok = mbar_wait(empty(st), (use & 1) ^ 1, ws))) break;
+                    const uint32_t to = base + st * STAGE_BYTES, bar = peer_smem(full(st), 0);
+                    if (rank == 0) mbar_expect(full(st), 2 * (2 + b_boxes) * BOX_BYTES);
+                    const int32_t kk = (int32_t)(c.k0 + k) * 64, m = (int32_t)(c.m0 + rank * 128);
+                    const int32_t bn = (int32_t)(c.n0 + rank * c.half + (P == LOGITS_STATS || P == LOGITS_GRAD ? a.first : 0));
+                    const int32_t bk = kk + (int32_t)(P == D_HIDDEN ? a.first : 0);
+                    for (int i = 0; i < 2; i++) {
+                        if (A_LINES) tma_load_pair(to + i * BOX_BYTES, &map_a, m + 64 * i, kk, za, bar);
+                        else tma_load_pair(to + i * BOX_BYTES, &map_a, kk, m + 64 * i, za, bar);
+                    }
+                    for (int i = 0; i < (int)b_boxes; i++) {
+                        if (B_LINES) tma_load_pair(to + (2 + i) * BOX_BYTES, &map_b, bn + 64 * i, bk, zb, bar);
+                        else tma_load_pair(to + (2 + i) * BOX_BYTES, &map_b, bk, bn + 64 * i, zb, bar);
+                    }
                 }
             }
+        }
+        // every stage has been given back before the block ends: no load and no arrival is on its way any more
+        for (uint32_t i = 1; i <= min(it, (uint32_t)STAGES) && ok; i++) ok = mbar_wait(empty((it - i) % STAGES), ((it - i) / STAGES) & 1, ws);
+        if (!ok)  // a wait ran out: what is in flight lands meanwhile
+            for (int i = 0; i < 2000; i++) __nanosleep(1000);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // ---- products
+        uint32_t it = 0, round = 0;
+        bool ok = true;
+        for (uint32_t t = pair; t < tiles && ok; t += pairs, round++) {
+            const Tile c = tile_at(t);
+            const uint32_t total = c.steps * a.n_pairs, buf = round & 1, d = tmem + buf * 256;
+            if (!(ok = mbar_wait(taken(buf), ((round >> 1) & 1) ^ 1, ws))) break;
+            fence_after_sync();
+            const uint32_t idesc = instruction(a.bf16, A_LINES, B_LINES, 256, c.width);
+            for (uint32_t k = 0; k < total; k++, it++) {
+                const uint32_t st = it % STAGES;
+                if (!(ok = mbar_wait(full(st), (it / STAGES) & 1, ws))) break;
+                fence_after_sync();
+                const uint32_t sa = base + st * STAGE_BYTES, sb = sa + 2 * BOX_BYTES;
 #pragma unroll
-            for (int o = 8; o; o >>= 1) s.x = fmaxf(s.x, __shfl_xor_sync(0xffffffffu, s.x, o));
-            const float ref = s.x == -INFINITY ? 0.f : s.x;
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (j0 + tx * 4 + c < N) s.y += expf(acc[r][c] - ref);
-#pragma unroll
-            for (int o = 8; o; o >>= 1) s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
-            if (in && tx == 0) a.part[(uint64_t)blockIdx.x * a.pitch + i] = s;
-        } else if (in) {
-            const float2 s = P == LOGITS_GRAD ? a.stats[row] : make_float2(0.f, 0.f);
-            const float weight = P == LOGITS_GRAD && a.mask ? a.mask[row] : 1.f;
-            const int64_t t = P == LOGITS_GRAD ? a.targets[row] : -1;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const uint32_t j = j0 + tx * 4 + c;
-                if (j >= N) continue;
+                for (int q = 0; q < 4; q++)  // 16 of K: 32 bytes along a line, or 16 lines
+                    mma_pair(d, operand(sa + q * (A_LINES ? 2048 : 32), A_LINES), operand(sb + q * (B_LINES ? 2048 : 32), B_LINES), idesc,
+                             k > 0 || q > 0);
+                commit_pair(empty(st));
+            }
+            commit_pair(done(buf));
+        }
+    } else if (warp >= 2) {
+        // ---- the finished tiles: a warp reads the 32 lanes of its quarter, half of the columns each
+        const uint32_t quarter = warp & 3, side = (warp - 2) / 4, row_in = quarter * 32 + lane;
+        uint32_t round = 0;
+        for (uint32_t t = pair; t < tiles; t += pairs, round++) {
+            const Tile c = tile_at(t);
+            const uint32_t buf = round & 1, i = c.m0 + rank * 128 + row_in;
+            const bool in = i < M;
+            // what the row needs is fetched while the tile is still being made
+            uint32_t target = 0xffffffffu;
+            float2 s = make_float2(0.f, 1.f);
+            float factor = 0.f;
+            if ((P == LOGITS_STATS || P == LOGITS_GRAD) && in) {
+                const uint32_t row = (uint32_t)a.row_of[i];
+                target = (uint32_t)a.targets[row] - a.first - c.n0;  // column of the tile; far outside it: another tile's
                 if (P == LOGITS_GRAD) {
-                    const float e = expf(acc[r][c] - s.x);
-                    a.g[(uint64_t)i * a.columns + j] = weight * ((int64_t)(a.first + j) == t ? (e - s.y) / s.y : e / s.y);
-                } else if (P == D_HIDDEN) {
-                    float* to = a.dx + (uint64_t)i * a.hidden + j;
-                    *to = a.add ? *to + acc[r][c] : acc[r][c];
-                } else {
-                    G* to = static_cast<G*>(a.dw) + (uint64_t)(a.first + i) * a.hidden + j;
-                    *to = from_f32<G>(a.accumulate ? to_f32<G>(*to) + acc[r][c] * a.scale : acc[r][c] * a.scale);
+                    s = a.stats[row];
+                    factor = (a.mask ? a.mask[row] : 1.f) * a.meta->up / s.y;
                 }
             }
+            const float scale = P == D_WEIGHT ? a.scale * a.meta->down : 1.f;
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(done(buf), (round >> 1) & 1, ws));
+            if (!ok) break;
+            fence_after_sync();
+            const uint32_t valid = min(256u, N - c.n0);  // columns of the tile that exist
+            const uint32_t from = side * 128, to = min(from + 128, P == LOGITS_GRAD ? (valid + 63) & ~63u : valid);
+            float2 run = make_float2(-INFINITY, 0.f);
+            for (uint32_t c0 = from; c0 < to; c0 += 32) {
+                uint32_t x[32];
+                const bool made = c.steps > 0 && c0 < c.width;
+                if (made) {
+                    tmem_load32(tmem + buf * 256 + c0 + (quarter << 21), x);
+                    tmem_wait(x);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) x[j] = 0;
+                }
+                if (P == LOGITS_STATS) {
+                    if (c0 + 32 > valid) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (c0 + j >= valid) x[j] = 0xff800000u;  // -inf: no word of the vocabulary
+                    }
+                    if (target - c0 < 32) {
+                        float tl = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; j++) tl = target - c0 == (uint32_t)j ? __uint_as_float(x[j]) : tl;
+                        a.target_logit[i] = tl;
+                    }
+                    float m = run.x;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) m = fmaxf(m, __uint_as_float(x[j]));
+                    const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf yet: exp(-inf - 0) is the zero it should be
+                    const ExpFrom<sizeof(T) == 4> ex(ref);
+                    float part[4] = {run.x == -INFINITY ? run.y : run.y * ex(run.x), 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < 32; j++) part[j & 3] += ex(__uint_as_float(x[j]));
+                    run = make_float2(m, (part[0] + part[1]) + (part[2] + part[3]));
+                } else if (P == LOGITS_GRAD) {
+                    const ExpFrom<sizeof(T) == 4> ex(s.x);
+                    float g[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) g[j] = ex(__uint_as_float(x[j])) * factor;
+                    if (target - c0 < 32) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (target - c0 == (uint32_t)j) g[j] = (ex(__uint_as_float(x[j])) - s.y) * factor;
+                    }
+                    if (!in || c0 + 32 > valid) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (!in || c0 + j >= valid) g[j] = 0.f;
+                    }
+                    S* out = static_cast<S*>(a.g) + (uint64_t)i * a.g_pitch + c.n0 + c0;
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            w[j] = pack2<S>(g[2 * j], g[2 * j + 1]);
+                            if (p + 1 < PARTS) {  // what the part leaves; nothing of an infinity or a NaN
+                                const float2 got = unpack2<S>(w[j]);
+                                g[2 * j] = isfinite(g[2 * j]) ? g[2 * j] - got.x : 0.f;
+                                g[2 * j + 1] = isfinite(g[2 * j + 1]) ? g[2 * j + 1] - got.y : 0.f;
+                            }
+                        }
+                        store32(out + p * a.g_part, w);
+                        store32(out + p * a.g_part + 16, w + 8);
+                    }
+                } else if (P == D_HIDDEN) {
+                    if (in) {
+                        float* to_dx = a.dx + c.split * a.dx_slab + (uint64_t)i * a.dx_pitch + c.n0 + c0;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            uint32_t w[8];
+                            if (a.add) load32(to_dx + 8 * q, w);
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+                                w[j] = a.add ? __float_as_uint(__uint_as_float(w[j]) + __uint_as_float(x[8 * q + j])) : x[8 * q + j];
+                            store32(to_dx + 8 * q, w);
+                        }
+                    }
+                } else if (in) {
+                    G* out = static_cast<G*>(a.dw) + (uint64_t)(a.first + i) * a.hidden + c.n0 + c0;
+                    write_span<G>(out, x, min(32u, valid - c0), scale, a.accumulate != 0);
+                }
+            }
+            if (P == LOGITS_STATS && in) a.part[(uint64_t)(2 * (c.n0 / 256) + side) * a.pitch + i] = run;
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(peer_smem(taken(buf), 0));
         }
     }
+    __syncwarp();
+    fence_before_sync();
+    __syncthreads();
+    cluster_sync();  // nobody arrives at a barrier of a block that has ended
+    fence_after_sync();
+    if (warp == 1) tmem_free_pair(tmem, 512);
 }
 
-// ---- d_hidden: the scored rows' sums times the scale, rounded; zeros for the others
+// ---- d_hidden: the scored rows' sums over the splits, in their order, times the scale, rounded; zeros for the others
 template <typename T>
-__global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t hidden, const int32_t* __restrict__ slot_of,
-                                                       const float* __restrict__ dx, float scale, T* out, uint64_t stride) {
+__global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t hidden, uint32_t dx_pitch, uint32_t splits, uint64_t dx_slab,
+                                                       const int32_t* __restrict__ slot_of, const float* __restrict__ dx,
+                                                       const HeadMeta* __restrict__ meta, float scale, T* out, uint64_t stride) {
+    scale *= meta->down;
     const uint64_t total = (uint64_t)rows * hidden;
     for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
         const uint32_t row = (uint32_t)(e / hidden), col = (uint32_t)(e - (uint64_t)row * hidden);
         const int32_t slot = slot_of[row];
-        out[(uint64_t)row * stride + col] = from_f32<T>(slot < 0 ? 0.f : dx[(uint64_t)slot * hidden + col] * scale);
+        float sum = 0.f;
+        if (slot >= 0)
+            for (uint32_t k = 0; k < splits; k++) sum += dx[k * dx_slab + (uint64_t)slot * dx_pitch + col];
+        out[(uint64_t)row * stride + col] = from_f32<T>(slot < 0 ? 0.f : sum * scale);
     }
 }
 
 bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) % to) != 0; }
 
-template <typename T, typename G, int P>
-void product(const ProductArgs& a, uint64_t m, uint64_t n, cudaStream_t s) {
-    if (m && n) k_head_product<T, G, P><<<dim3((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64)), 256, 0, s>>>(a);
+using Encode = decltype(&cuTensorMapEncodeTiled);
+int32_t encoder(Encode* out) {
+    static Encode fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult st;
+        OXZ_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &st));
+        if (st != cudaDriverEntryPointSuccess || !p) return fail(OXZ_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+        fn = reinterpret_cast<Encode>(p);
+    }
+    *out = fn;
+    return OXZ_OK;
 }
 
-template <typename T, typename G>
-int32_t run(oxz_head* h, const oxz_head_batch& b, float* row_loss, float2* row_stats, bool want_loss, float* totals, const oxz_head_grads* gr,
-            cudaStream_t s) {
-    const oxz_head_desc& d = h->d;
-    k_head_rows<<<1, 1024, 0, s>>>(b.targets, b.loss_mask, (uint32_t)b.rows, d.vocab, h->row_of, h->slot_of, h->meta);
-    ProductArgs a{};
-    a.meta = h->meta;
-    a.row_of = h->row_of;
-    a.x = b.hidden;
-    a.x_stride = b.hidden_stride;
-    a.w = b.weight;
-    a.hidden = (uint32_t)d.hidden;
-    a.vocab = (uint32_t)d.vocab;
-    a.pitch = (uint32_t)d.max_rows;
-    a.targets = b.targets;
-    a.mask = b.loss_mask;
-    a.part = h->part;
-    a.target_logit = h->target_logit;
-    a.g = h->g;
-    a.dx = h->dx;
-    float2* stats = row_stats ? row_stats : h->stats;
-    if (want_loss) {
-        a.columns = (uint32_t)d.vocab;
-        product<T, G, LOGITS_STATS>(a, b.rows, d.vocab, s);
-        const unsigned blocks = std::max<unsigned>(1, (unsigned)((b.rows + FINISH_ROWS - 1) / FINISH_ROWS));
-        k_head_finish<<<blocks, 32 * FINISH_ROWS, 0, s>>>((uint32_t)b.rows, a.pitch, (uint32_t)((d.vocab + 63) / 64), h->slot_of, h->part,
-                                                          h->target_logit, b.loss_mask, stats, row_loss, h->loss_part, h->meta, totals);
+// [parts][lines][pitch] 16-bit values as boxes of 64 x 64, 128-byte swizzle; what lies outside reads as zeros
+int32_t tensor_map(CUtensorMap* m, bool bf16, const void* base, uint64_t pitch, uint64_t lines, uint64_t parts, uint64_t part_stride) {
+    Encode encode = nullptr;
+    OXZ_TRY(encoder(&encode));
+    const cuuint64_t dims[3] = {pitch, lines, parts}, strides[2] = {pitch * 2, part_stride * 2};
+    const cuuint32_t box[3] = {64, 64, 1}, step[3] = {1, 1, 1};
+    const CUresult r = encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
+                              strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(OXZ_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)r);
+    return OXZ_OK;
+}
+
+template <typename T, typename S, typename G, int PARTS>
+struct Products {
+    template <int P>
+    static void launch(const oxz_head* h, const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, uint64_t m, uint64_t n, cudaStream_t s) {
+        const uint64_t tiles = (m + MMA_M - 1) / MMA_M * ((n + MMA_N - 1) / MMA_N) * (P == D_HIDDEN ? a.splits : 1);
+        if (tiles) k_head_product<T, S, G, P, PARTS><<<2 * (unsigned)std::min<uint64_t>(tiles, h->clusters), MMA_THREADS, MMA_SMEM, s>>>(ma, mb, a);
     }
-    if (gr) {
+    template <int P>
+    static int32_t prepare(int* clusters) {
+        auto k = k_head_product<T, S, G, P, PARTS>;
+        OXZ_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MMA_SMEM));
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(2);
+        cfg.blockDim = dim3(MMA_THREADS);
+        cfg.dynamicSmemBytes = MMA_SMEM;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {2, 1, 1};
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int c = 0;
+        OXZ_CUDA(cudaOccupancyMaxActiveClusters(&c, k, &cfg));
+        if (c < 1) return fail(OXZ_ERR_UNSUPPORTED, "the device runs no pair of blocks with %u bytes of shared memory", MMA_SMEM);
+        *clusters = *clusters ? std::min(*clusters, c) : c;
+        return OXZ_OK;
+    }
+    static int32_t prepare_all(oxz_head* h) {
+        OXZ_TRY(prepare<LOGITS_STATS>(&h->clusters));
+        OXZ_TRY(prepare<LOGITS_GRAD>(&h->clusters));
+        OXZ_TRY(prepare<D_HIDDEN>(&h->clusters));
+        return prepare<D_WEIGHT>(&h->clusters);
+    }
+
+    static int32_t run(oxz_head* h, const oxz_head_batch& b, float* row_loss, float2* row_stats, bool want_loss, float* totals,
+                       const oxz_head_grads* gr, cudaStream_t s) {
+        const oxz_head_desc& d = h->d;
+        constexpr bool F32 = sizeof(T) == 4, BF16 = std::is_same<S, __nv_bfloat16>::value;
+        const size_t es = sizeof(T);
+        const unsigned many = (unsigned)h->clusters * 2 * 8;  // blocks of the elementwise kernels
+        k_head_rows<<<1, 1024, 0, s>>>(b.targets, b.loss_mask, (uint32_t)b.rows, d.vocab, h->row_of, h->slot_of, h->meta, !BF16);
+        const uint64_t x_part = h->cap * h->pitch, w_part = d.vocab * h->pitch;
+        const bool x_wide = !misaligned(b.hidden, 16) && b.hidden_stride * es % 16 == 0;
+        if (b.rows) {
+            const uint64_t work = (b.rows + MMA_M) * (h->pitch / 8);
+            k_head_pack<T, S><<<(unsigned)std::min<uint64_t>((work + 255) / 256, many), 256, 0, s>>>(
+                static_cast<const T*>(b.hidden), b.hidden_stride, (uint32_t)d.hidden, h->pitch, b.rows, h->row_of, h->meta,
+                static_cast<S*>(h->x), x_part, h->parts, x_wide);
+        }
+        if (h->w)
+            k_head_pack<T, S><<<many, 256, 0, s>>>(static_cast<const T*>(b.weight), d.hidden, (uint32_t)d.hidden, h->pitch, d.vocab, nullptr,
+                                                   h->meta, static_cast<S*>(h->w), w_part, h->parts, d.hidden * es % 16 == 0);
+        CUtensorMap mx, mw, mg;
+        OXZ_TRY(tensor_map(&mx, BF16, h->x, h->pitch, h->cap, h->parts, x_part));
+        OXZ_TRY(tensor_map(&mw, BF16, h->w ? h->w : b.weight, h->pitch, d.vocab, h->parts, w_part));
+
+        ProductArgs a{};
+        a.meta = h->meta;
+        a.row_of = h->row_of;
+        a.hidden = (uint32_t)d.hidden;
+        a.pitch = (uint32_t)d.max_rows;
+        a.dx_pitch = h->dx_pitch;
+        a.targets = b.targets;
+        a.mask = b.loss_mask;
+        a.part = h->part;
+        a.target_logit = h->target_logit;
+        a.g = h->g;
+        a.dx = h->dx;
+        a.bf16 = BF16;
+        a.expired = h->d_expired;
+        // an f32 operand is hi + mid + lo; of the nine products the six above 2^-24 are formed, the small ones first
+        static const uint8_t six[2][6] = {{2, 1, 0, 1, 0, 0}, {0, 1, 2, 0, 1, 0}};
+        auto pairs = [&](int g_only) {
+            a.n_pairs = F32 ? 6 : g_only;
+            for (int p = 0; p < a.n_pairs; p++) {
+                a.pair_a[p] = F32 ? six[0][p] : (uint8_t)(g_only - 1 - p);
+                a.pair_b[p] = F32 ? six[1][p] : 0;
+            }
+        };
+        float2* stats = row_stats ? row_stats : h->stats;
+        pairs(1);
+        if (want_loss) {
+            a.columns = (uint32_t)d.vocab;
+            launch<LOGITS_STATS>(h, mx, mw, a, b.rows, d.vocab, s);
+            const unsigned blocks = std::max<unsigned>(1, (unsigned)((b.rows + FINISH_ROWS - 1) / FINISH_ROWS));
+            k_head_finish<<<blocks, 32 * FINISH_ROWS, 0, s>>>((uint32_t)b.rows, a.pitch, 2 * (uint32_t)((d.vocab + MMA_N - 1) / MMA_N), h->slot_of,
+                                                              h->part, h->target_logit, b.loss_mask, stats, row_loss, h->loss_part, h->meta, totals);
+        }
+        if (!gr) return OXZ_OK;
         a.stats = stats;
         a.scale = (float)gr->grad_scale;
         a.accumulate = gr->accumulate;
         a.dw = gr->d_weight;
+        a.g_pitch = (uint32_t)h->piece;
+        a.g_part = h->cap * h->piece;
+        OXZ_TRY(tensor_map(&mg, BF16, h->g, h->piece, h->cap, h->g_parts, a.g_part));
+        // few output tiles of d_hidden: K, the vocabulary of a piece, is split so that every pair has work
+        const uint64_t mt = (b.rows + MMA_M - 1) / MMA_M, nt = (d.hidden + MMA_N - 1) / MMA_N;
+        a.splits = mt ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(h->clusters / (mt * nt), h->piece / MMA_K)) : 1;
+        a.dx_slab = mt * MMA_M * h->dx_pitch;
         for (uint64_t v = 0; v < d.vocab; v += h->piece) {
             a.first = (uint32_t)v;
             a.columns = (uint32_t)std::min(h->piece, d.vocab - v);
             a.add = v > 0;
-            product<T, G, LOGITS_GRAD>(a, b.rows, a.columns, s);
-            if (gr->d_hidden) product<T, G, D_HIDDEN>(a, b.rows, d.hidden, s);
-            if (gr->d_weight) product<T, G, D_WEIGHT>(a, a.columns, d.hidden, s);
+            pairs(1);
+            launch<LOGITS_GRAD>(h, mx, mw, a, b.rows, a.columns, s);
+            if (gr->d_hidden) launch<D_HIDDEN>(h, mg, mw, a, b.rows, d.hidden, s);
+            pairs(h->g_parts);
+            if (gr->d_weight) launch<D_WEIGHT>(h, mg, mx, a, a.columns, d.hidden, s);
         }
         if (gr->d_hidden && b.rows)
-            k_head_d_hidden<T><<<(unsigned)std::min<uint64_t>((b.rows * d.hidden + 255) / 256, 148 * 8), 256, 0, s>>>(
-                (uint32_t)b.rows, (uint32_t)d.hidden, h->slot_of, h->dx, (float)gr->grad_scale, static_cast<T*>(gr->d_hidden), gr->d_hidden_stride);
+            k_head_d_hidden<T><<<(unsigned)std::min<uint64_t>((b.rows * d.hidden + 255) / 256, many), 256, 0, s>>>(
+                (uint32_t)b.rows, (uint32_t)d.hidden, h->dx_pitch, a.splits, a.dx_slab, h->slot_of, h->dx, h->meta, a.scale,
+                static_cast<T*>(gr->d_hidden), gr->d_hidden_stride);
+        return OXZ_OK;
     }
-    return OXZ_OK;
+};
+using BF = __nv_bfloat16;
+using F32Products = Products<float, BF, float, 3>;
+using Bf16Products = Products<BF, BF, BF, 1>;
+using Bf16F32Products = Products<BF, BF, float, 3>;
+using F16Products = Products<__half, __half, __half, 1>;
+using F16F32Products = Products<__half, __half, float, 3>;
+// f(P): P the product family of the handle's types
+template <typename F>
+int32_t with_types(const oxz_head_desc& d, F&& f) {
+    if (d.dtype == OXZ_F32) return f(F32Products{});
+    if (d.dtype == OXZ_BF16) return d.grad_dtype == OXZ_F32 ? f(Bf16F32Products{}) : f(Bf16Products{});
+    return d.grad_dtype == OXZ_F32 ? f(F16F32Products{}) : f(F16Products{});
 }
 
 int32_t call(const char* who, oxz_head* h, const oxz_head_batch* batch, float* row_loss, float* row_stats, float* totals, bool want_loss,
@@ -361,18 +732,15 @@ int32_t call(const char* who, oxz_head* h, const oxz_head_batch* batch, float* r
     if (misaligned(b.weight, 16) || misaligned(g.d_weight, 16)) return fail(OXZ_ERR_INVALID, "%s: weight and d_weight are aligned to 16 bytes", who);
     if (want_grads && !std::isfinite((float)g.grad_scale)) return fail(OXZ_ERR_INVALID, "%s: grad_scale %g is not a finite f32", who, g.grad_scale);
     if (!h->allocated) return fail(OXZ_ERR_STATE, "%s: no workspace: call oxz_head_alloc first", who);
+    if (*reinterpret_cast<volatile int32_t*>(h->expired))
+        return fail(OXZ_ERR_TIMEOUT, "%s: a bounded wait inside a kernel of an earlier call ran out; its results are not valid", who);
     DeviceGuard dev;
     OXZ_TRY(dev.enter(d.device));
     cudaStream_t s = (cudaStream_t)stream;
     OXZ_TRY(h->order.begin(s));
     float2* st = reinterpret_cast<float2*>(row_stats);
     const oxz_head_grads* gp = want_grads ? &g : nullptr;
-    int32_t rc;
-    if (d.dtype == OXZ_F32) rc = run<float, float>(h, b, row_loss, st, want_loss, totals, gp, s);
-    else if (d.dtype == OXZ_BF16 && d.grad_dtype == OXZ_F32) rc = run<__nv_bfloat16, float>(h, b, row_loss, st, want_loss, totals, gp, s);
-    else if (d.dtype == OXZ_BF16) rc = run<__nv_bfloat16, __nv_bfloat16>(h, b, row_loss, st, want_loss, totals, gp, s);
-    else if (d.grad_dtype == OXZ_F32) rc = run<__half, float>(h, b, row_loss, st, want_loss, totals, gp, s);
-    else rc = run<__half, __half>(h, b, row_loss, st, want_loss, totals, gp, s);
+    const int32_t rc = with_types(d, [&](auto p) { return decltype(p)::run(h, b, row_loss, st, want_loss, totals, gp, s); });
     OXZ_TRY(rc);
     OXZ_CUDA(cudaGetLastError());
     return h->order.end(s);
@@ -415,8 +783,15 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             DeviceGuard dev;
             OXZ_TRY(dev.enter(h->d.device));
             const oxz_head_desc& d = h->d;
+            h->cap = (d.max_rows + MMA_M - 1) / MMA_M * MMA_M;
+            h->pitch = (uint32_t)((d.hidden + 7) / 8 * 8);
+            h->dx_pitch = (uint32_t)((d.hidden + 31) / 32 * 32);
+            h->parts = d.dtype == OXZ_F32 ? 3 : 1;
+            h->g_parts = d.grad_dtype == OXZ_F32 ? 3 : 1;
+            OXZ_TRY(with_types(d, [&](auto p) { return decltype(p)::prepare_all(h); }));
             const uint64_t limit = d.piece_bytes ? d.piece_bytes : 512ull << 20;
-            h->piece = std::min<uint64_t>(d.vocab, std::max<uint64_t>(64, limit / (d.max_rows * 4) / 64 * 64));
+            const uint64_t all = (d.vocab + MMA_N - 1) / MMA_N * MMA_N;
+            h->piece = std::min(all, std::max<uint64_t>(MMA_N, limit / (h->cap * 2 * h->g_parts) / MMA_N * MMA_N));
             uint64_t bytes = 0;
             auto get = [&](auto** p, uint64_t n) -> int32_t {  // what a failed attempt left behind is kept and used by the next one
                 if (!*p) OXZ_CUDA(cudaMalloc((void**)p, n));
@@ -425,13 +800,21 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             };
             OXZ_TRY(get(&h->row_of, d.max_rows * 4));
             OXZ_TRY(get(&h->slot_of, d.max_rows * 4));
-            OXZ_TRY(get(&h->part, (d.vocab + 63) / 64 * d.max_rows * 8));
+            OXZ_TRY(get(&h->part, 2 * (all / MMA_N) * d.max_rows * 8));
             OXZ_TRY(get(&h->target_logit, d.max_rows * 4));
             OXZ_TRY(get(&h->stats, d.max_rows * 8));
             OXZ_TRY(get(&h->loss_part, (d.max_rows + FINISH_ROWS - 1) / FINISH_ROWS * 8));
             OXZ_TRY(get(&h->meta, sizeof(HeadMeta)));
-            OXZ_TRY(get(&h->g, d.max_rows * h->piece * 4));
-            OXZ_TRY(get(&h->dx, d.max_rows * d.hidden * 4));
+            OXZ_TRY(get(&h->x, h->cap * h->pitch * h->parts * 2));
+            if (d.dtype == OXZ_F32 || d.hidden % 8) OXZ_TRY(get(&h->w, d.vocab * h->pitch * h->parts * 2));
+            OXZ_TRY(get(&h->g, h->cap * h->piece * h->g_parts * 2));
+            // splits x tiles of d_hidden is at most the pairs wherever there is more than one split
+            OXZ_TRY(get(&h->dx, std::max<uint64_t>((uint64_t)h->clusters * MMA_M * MMA_N, h->cap * h->dx_pitch) * 4));
+            if (!h->expired) {
+                OXZ_CUDA(cudaHostAlloc((void**)&h->expired, 4, cudaHostAllocMapped));
+                *h->expired = 0;
+                OXZ_CUDA(cudaHostGetDevicePointer((void**)&h->d_expired, h->expired, 0));
+            }
             OXZ_TRY(h->order.create());
             h->bytes = bytes;
             h->allocated = true;
@@ -448,8 +831,9 @@ int32_t oxz_head_destroy(oxz_head* h) {
         if (h->row_of) dev.enter(h->d.device);
         h->order.destroy();
         for (void* p : {(void*)h->row_of, (void*)h->slot_of, (void*)h->part, (void*)h->target_logit, (void*)h->stats, (void*)h->loss_part,
-                        (void*)h->meta, (void*)h->g, (void*)h->dx})
+                        (void*)h->meta, h->x, h->w, h->g, (void*)h->dx})
             if (p) cudaFree(p);
+        if (h->expired) cudaFreeHost(h->expired);
         delete h;
         return OXZ_OK;
     });

@@ -1,0 +1,122 @@
+// The tensor-core path of sm_100a as the loss head's products use it: mbarriers with bounded waits, TMA tile loads, and
+// tcgen05.mma on a pair of SMs (cta_group::2) with its accumulators in tensor memory. Thin wrappers over single instructions.
+#pragma once
+
+#include <stdint.h>
+
+namespace oxz {
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// The address of the same place in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {  // bar: a peer_smem address
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+
+// What a block that gives up leaves for its other warps (shared) and for the host (mapped memory).
+struct WaitState {
+    volatile uint32_t* dead;
+    int32_t* expired;
+};
+constexpr uint32_t WAIT_TRIES = 1u << 24;  // each try suspends the thread for a while: seconds in all
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const WaitState& w) {
+    for (uint32_t i = 0; i < WAIT_TRIES; i++) {
+        if (mbar_try(bar, parity)) return true;
+        if ((i & 255) == 255 && *w.dead) return false;
+    }
+    *w.dead = 1;
+    *reinterpret_cast<volatile int32_t*>(w.expired) = 1;
+    __threadfence_system();
+    return false;
+}
+
+// A box of a 3-d tensor map into this block's shared memory; the bytes are counted on `bar`, which may be the pair's first block's.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const void* map, int32_t x, int32_t y, int32_t z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_map(const void* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t to_smem, uint32_t columns) {  // one warp of each block of the pair
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to_smem), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t addr, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// D[256 x N] (+)= A[256 x 16] B[N x 16]^T over the two blocks of a pair: 128 rows of A and D and half of B's rows in each.
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+// Arrives at `bar` (same place in both blocks) once the pair's products issued so far have read and written what they use.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+// 32 columns of this warp's 32 lanes of tensor memory: x[c] is column c of the thread's row. Complete after tmem_wait(x).
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&x)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
+          "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
+          "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]),
+          "=r"(x[31])
+        : "r"(addr));
+}
+// The registers pass through, so that nothing that reads them is moved above the wait.
+__device__ __forceinline__ void tmem_wait(uint32_t (&x)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15]), "+r"(x[16]), "+r"(x[17]), "+r"(x[18]), "+r"(x[19]), "+r"(x[20]), "+r"(x[21]), "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]), "+r"(x[29]), "+r"(x[30]), "+r"(x[31])
+                 :
+                 : "memory");
+}
+
+// Shared-memory operand descriptors for tiles that TMA wrote with the 128-byte swizzle, in boxes of 64 elements (128 bytes) by
+// 64 lines, 8192 bytes each.
+//   K along the 128 bytes: lines are rows of the operand; 8 lines (1024 bytes) form a group, groups follow each other.
+//   K along the lines: the 128 bytes hold 64 rows of the operand, the next 64 are one box (8192 bytes) on; 8 lines form a group.
+constexpr uint32_t BOX_BYTES = 8192;
+__device__ __forceinline__ uint64_t operand(uint32_t addr, bool k_along_lines) {
+    const uint64_t leading = k_along_lines ? BOX_BYTES >> 4 : 1, stride = 1024 >> 4;
+    return (uint64_t)((addr >> 4) & 0x3fff) | leading << 16 | stride << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// f32 accumulators, both operands bf16 or both f16
+__host__ __device__ __forceinline__ uint32_t instruction(bool bf16, bool a_along_lines, bool b_along_lines, uint32_t m, uint32_t n) {
+    const uint32_t fmt = bf16 ? 1 : 0;
+    return 1u << 4 | fmt << 7 | fmt << 10 | (uint32_t)a_along_lines << 15 | (uint32_t)b_along_lines << 16 | (n >> 3) << 17 | (m >> 4) << 24;
+}
+
+}  // namespace oxz

@@ -7,7 +7,8 @@ adder rounds:
             additions in a chain (the cases have vocab below 60000) and a few roundings of exp
   loss      |d loss| <= 2E + r + 4u (|m| + |l_t| + |log s|)
   g         |dg| <= |w| p (E + r + 8u) + |w| 4u [v = t]  and one rounding to the type: half a step of |g|; f16 is scaled so that the
-            largest weight times one stays normal, and loses 2^-25 2^-13 max|w| at most below its normal range
+            largest weight times one stays normal, and loses 2^-25 2^-13 max|w| at most below its normal range. The exponential that
+        16-bit operands use flushes results below 2^-126, the smallest normal f32, to zero: 2^-126 |w| (s is one or more)
   d_hidden  scale (sum_v |dg||W| + (V + 64) 2u sum_v |g||W|) and half a step of the result
   d_weight  scale (sum_i |dg||X| + (N + 64) 2u sum_i |g||X|) and half a step of the result; g is not rounded to 16 bits when
             d_weight is f32 (three pieces of 8 bits or more: 2u)
@@ -139,7 +140,7 @@ class Problem:
         g = np.where(on[:, None], w * (p - y), 0.0)
         dg = np.where(on[:, None], np.abs(w) * (p * (E + r + 8 * U)[:, None] + 4 * U * y), 0.0)
         top = np.abs(self.w_row).max(initial=0.0)
-        low = 2.0 ** -38 * top if self.dtype == "f16" else 2.0 ** -133
+        low = {"f16": 2.0 ** -38 * top, "bf16": 2.0 ** -126 * top, "f32": 2.0 ** -133}[self.dtype]
         dg_t = dg + HALF_STEP[self.dtype] * np.abs(g) + low * on[:, None]
         dg_w = dg + 2 * U * np.abs(g) + low * on[:, None] if self.grad == "f32" else dg_t
         c = abs(scale)
