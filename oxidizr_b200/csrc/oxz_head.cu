@@ -25,6 +25,7 @@ struct HeadMeta {
     uint32_t done;       // blocks of k_head_finish that have added their part (put back to 0 by the last)
     double weight_sum;   // of the scored rows
     float up, down;      // power of two G is scaled by before it is rounded (f16 only), and its inverse
+    uint32_t kept;       // columns of a row of `l` where the losses leave the logits for the gradients; 0: they do not all fit
 };
 
 }  // namespace oxz
@@ -49,7 +50,10 @@ struct oxz_head {
     void* x = nullptr;               // [parts][cap][pitch] packed hidden states
     void* w = nullptr;               // [parts][vocab][pitch] packed weight, where TMA cannot read the caller's
     void* g = nullptr;               // [g_parts][cap][piece]
-    float* dx = nullptr;             // [splits][rows][dx_pitch] sums over the pieces
+    float* l = nullptr;              // [scored rows][kept] logits
+    uint64_t l_elems = 0, kept_pitch = 0;
+    float* dx = nullptr;             // [scored rows][dx_pitch] sums over the pieces
+    float* dx_shares = nullptr;      // tiles of 256 x 256: the shares after the first of the tiles that are cut
     int32_t* expired = nullptr;      // mapped host memory: a bounded wait inside a kernel ran out
     int32_t* d_expired = nullptr;
     oxz::StreamOrder order;
@@ -58,75 +62,73 @@ struct oxz_head {
 namespace oxz {
 namespace {
 
-constexpr int FINISH_ROWS = 8;  // rows a block of k_head_finish takes: one per warp
+constexpr uint32_t FINISH_ROWS = 32;  // rows a block of k_head_finish takes
 constexpr uint32_t MMA_M = 256, MMA_N = 256, MMA_K = 64;  // tile of a pair of SMs
 
-// ---- the scored rows, in order. One block: each thread counts a run of rows, a scan over the threads places them.
+// ---- the scored rows, in order, and what the other kernels need to know of them. One block: a warp takes a contiguous run of rows,
+// 32 at a time; a scan over the warps' counts places them.
 __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ targets, const float* __restrict__ mask, uint32_t rows,
-                                                    uint64_t vocab, int32_t* row_of, int32_t* slot_of, HeadMeta* meta, int f16) {
-    __shared__ uint32_t scan[32];
+                                                    uint64_t vocab, int32_t* row_of, int32_t* slot_of, HeadMeta* meta, int f16,
+                                                    uint64_t l_elems) {
+    __shared__ uint32_t counts[32];
     __shared__ double wsum[32];
     __shared__ float wtop[32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const uint32_t each = (rows + 1023) / 1024;
-    const uint32_t lo = min(rows, threadIdx.x * each), hi = min(rows, lo + each);
-    uint32_t count = 0;
-    double w = 0.0;
+    const uint32_t turns = (rows + 1023) / 1024;
+    const uint64_t begin = (uint64_t)warp * turns * 32;
+    auto weight = [&](uint64_t i) { return i < rows && (uint64_t)targets[i] < vocab ? (mask ? mask[i] : 1.f) : 0.f; };
+    uint32_t count = 0, kept_bits = 0;  // lane k keeps the flags of turn k: the second walk of up to 32 turns reads nothing again
+    double sum = 0.0;
     float top = 0.f;
-    auto scored = [&](uint32_t i) { return (mask == nullptr || mask[i] != 0.f) && (uint64_t)targets[i] < vocab; };
-    for (uint32_t i = lo; i < hi; i++)
-        if (scored(i)) {
-            count++;
-            w += mask ? (double)mask[i] : 1.0;
-            top = fmaxf(top, mask ? fabsf(mask[i]) : 1.f);
-        }
-    uint32_t inc = count;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= (uint32_t)o) inc += up;
+    for (uint32_t t = 0; t < turns; t++) {
+        const float w = weight(begin + (uint64_t)t * 32 + lane);
+        const uint32_t bits = __ballot_sync(0xffffffffu, w != 0.f);
+        if (t == lane) kept_bits = bits;
+        count += __popc(bits);
+        sum += (double)w;
+        top = fmaxf(top, fabsf(w));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        w += __shfl_xor_sync(0xffffffffu, w, o);
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
-    if (lane == 31) scan[warp] = inc;
     if (lane == 0) {
-        wsum[warp] = w;
+        counts[warp] = count;
+        wsum[warp] = sum;
         wtop[warp] = top;
     }
     __syncthreads();
-    if (warp == 0) {
-        uint32_t v = scan[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t up = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= (uint32_t)o) v += up;
-        }
-        scan[lane] = v;
-        if (lane == 31) {
-            double total = 0.0;
-            for (int k = 0; k < 32; k++) {
-                total += wsum[k];
-                top = fmaxf(top, wtop[k]);
-            }
-            meta->n = v;
-            meta->done = 0;
-            meta->weight_sum = total;
-            // f16 holds 2^-24 .. 65504: the largest weight times one goes to 2^13 .. 2^14, so that probabilities down to 2^-27 of it
-            // stay normal numbers
-            const int up = f16 && top > 0.f && isfinite(top) ? 13 - ilogbf(top) : 0;
-            meta->up = exp2f((float)min(max(up, -100), 100));
-            meta->down = exp2f((float)-min(max(up, -100), 100));
-        }
+    uint32_t at = 0, n = 0;
+    for (uint32_t w = 0; w < 32; w++) {
+        at += w < warp ? counts[w] : 0;
+        n += counts[w];
     }
-    __syncthreads();
-    uint32_t at = inc - count + (warp ? scan[warp - 1] : 0);
-    for (uint32_t i = lo; i < hi; i++) {
-        const bool yes = scored(i);
-        slot_of[i] = yes ? (int32_t)at : -1;
-        if (yes) row_of[at++] = (int32_t)i;
+    if (threadIdx.x == 0) {
+        double total = 0.0;
+        for (int k = 0; k < 32; k++) {
+            total += wsum[k];
+            top = fmaxf(top, wtop[k]);
+        }
+        meta->n = n;
+        meta->done = 0;
+        meta->weight_sum = total;
+        // f16 holds 2^-24 .. 65504: the largest weight times one goes to 2^13 .. 2^14, so that probabilities down to 2^-27 of it
+        // stay normal numbers
+        const int up = f16 && top > 0.f && isfinite(top) ? min(max(13 - ilogbf(top), -100), 100) : 0;
+        meta->up = exp2f((float)up);
+        meta->down = exp2f((float)-up);
+        const uint64_t all = (vocab + MMA_N - 1) / MMA_N * MMA_N;
+        meta->kept = n * all <= l_elems ? (uint32_t)all : 0;
+    }
+    for (uint32_t t = 0; t < turns; t++) {
+        const uint64_t i = begin + (uint64_t)t * 32 + lane;
+        const uint32_t bits = turns <= 32 ? __shfl_sync(0xffffffffu, kept_bits, t) : __ballot_sync(0xffffffffu, weight(i) != 0.f);
+        const bool yes = bits >> lane & 1;
+        const uint32_t slot = at + __popc(bits & ((1u << lane) - 1));
+        if (i < rows) slot_of[i] = yes ? (int32_t)slot : -1;
+        if (yes) row_of[slot] = (int32_t)i;
+        at += __popc(bits);
     }
 }
 
@@ -137,41 +139,47 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
     return make_float2(m, a.y * expf(a.x - m) + b.y * expf(b.x - m));
 }
 
-// ---- a row's statistics from its tiles', its loss, and the totals (by the block that ends last, in block order)
-__global__ void __launch_bounds__(32 * FINISH_ROWS) k_head_finish(uint32_t rows, uint32_t pitch, uint32_t tiles, const int32_t* __restrict__ slot_of,
-                                                                  const float2* __restrict__ part, const float* __restrict__ target_logit,
-                                                                  const float* __restrict__ mask, float2* stats, float* row_loss,
-                                                                  double* loss_part, HeadMeta* meta, float* totals) {
-    __shared__ double mine[FINISH_ROWS];
+// ---- the rows' statistics from their tiles', their losses, and the totals (by the block that ends last, in block order). A block
+// takes 32 rows, a lane each; its warps take every 32nd tile and are joined in order.
+__global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pitch, uint32_t tiles, const int32_t* __restrict__ slot_of,
+                                                      const float2* __restrict__ part, const float* __restrict__ target_logit,
+                                                      const float* __restrict__ mask, float2* stats, float* row_loss, double* loss_part,
+                                                      HeadMeta* meta, float* totals) {
+    __shared__ float2 share[32][33];
     __shared__ uint32_t last;
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, row = blockIdx.x * FINISH_ROWS + warp;
-    if (row < rows) {
-        const int32_t slot = slot_of[row];
-        float2 s = make_float2(-INFINITY, 0.f);
-        if (slot >= 0)
-            for (uint32_t t = lane; t < tiles; t += 32) s = join(s, part[(uint64_t)t * pitch + slot]);
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, row = blockIdx.x * FINISH_ROWS + lane;
+    const int32_t slot = row < rows ? slot_of[row] : -1;
+    float2 s = make_float2(-INFINITY, 0.f);
+    if (slot >= 0) {
+        for (uint32_t t = warp; t < tiles; t += 4 * 32) {
+            float2 p[4];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s = join(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
-        if (lane == 0) {
-            const float loss = slot >= 0 ? logf(s.y) - (target_logit[slot] - s.x) : 0.f;
-            stats[row] = slot >= 0 ? s : make_float2(0.f, 0.f);
-            if (row_loss) row_loss[row] = loss;
-            mine[warp] = slot >= 0 ? (mask ? (double)mask[row] : 1.0) * (double)loss : 0.0;
+            for (int k = 0; k < 4; k++) p[k] = t + 32 * k < tiles ? part[(uint64_t)(t + 32 * k) * pitch + slot] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; k++) s = join(s, p[k]);
         }
-    } else if (lane == 0) {
-        mine[warp] = 0.0;
+    }
+    share[warp][lane] = s;
+    __syncthreads();
+    if (warp) return;
+    for (int w = 1; w < 32; w++) s = join(s, share[w][lane]);
+    double mine = 0.0;
+    if (row < rows) {
+        const float loss = slot >= 0 ? logf(s.y) - (target_logit[slot] - s.x) : 0.f;
+        stats[row] = slot >= 0 ? s : make_float2(0.f, 0.f);
+        if (row_loss) row_loss[row] = loss;
+        mine = slot >= 0 ? (mask ? (double)mask[row] : 1.0) * (double)loss : 0.0;
     }
     if (!totals) return;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double sum = 0.0;
-        for (int w = 0; w < FINISH_ROWS; w++) sum += mine[w];
-        loss_part[blockIdx.x] = sum;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) {
+        loss_part[blockIdx.x] = mine;
         __threadfence();
         last = atomicAdd(&meta->done, 1u) == gridDim.x - 1;
     }
-    __syncthreads();
-    if (!last || warp) return;
+    __syncwarp();
+    if (!last) return;
     __threadfence();
     double sum = 0.0;
     for (uint32_t b = lane; b < gridDim.x; b += 32) sum += __ldcg(&loss_part[b]);
@@ -245,9 +253,12 @@ __global__ void __launch_bounds__(256) k_head_pack(const T* __restrict__ src, ui
 // rows, so that a step of 64 in K costs an SM 32 KiB from L2 for 2 x 256 x 128 x 64 operations. One thread per SM keeps STAGES
 // steps of both operands in flight by TMA, one thread of the pair issues the products, eight warps per SM take the finished tile
 // from tensor memory while the other of its two buffers fills.
+// The tensor cores cut, not round, what they add to an accumulator: over K = 2048 the logits lose 2e-6 of the loss, over the
+// vocabulary of an f32 gradient 1e-5. Where that shows (RUN > 0) an accumulator holds RUN steps of K only and the runs are added in
+// f32 registers, rounded; parts of a value are added the small ones first.
 //   LOGITS_STATS  l = X W^T: each row's {max, sum of exp} over half a tile's columns goes out, and the target's logit
 //   LOGITS_GRAD   the same tile, turned into G
-//   D_HIDDEN      G W, summed over the pieces in f32 (each split of K in a slab of its own)
+//   D_HIDDEN      G W, summed over the pieces in f32; its tiles are few and long (K is a piece of the vocabulary): see Split
 //   D_WEIGHT      G^T X
 // Operands come as K runs in memory: G and X are K-major in the first three, W in the first two; the others are read with K along
 // the lines of their tiles. Values of more than 16 bits come in parts; a product of such operands is the sum over `pairs` of parts.
@@ -258,20 +269,49 @@ constexpr uint32_t STAGE_BYTES = 4 * BOX_BYTES, MMA_SMEM = STAGES * STAGE_BYTES 
 struct ProductArgs {
     const HeadMeta* meta;
     const int32_t* row_of;
-    uint32_t hidden, first, columns, pitch, g_pitch, dx_pitch, splits;  // the piece [first, first + columns) of the vocabulary
-    uint64_t g_part, dx_slab;
+    uint32_t hidden, first, columns, piece, pitch, g_pitch, dx_pitch, keep;  // the piece [first, first + columns) of the vocabulary
+    uint64_t g_part;
     const int64_t* targets;
     const float* mask;
     const float2* stats;
     float2* part;
     float* target_logit;
     void* g;
-    float* dx;
+    float* l;
+    float *dx, *dx_shares;
     void* dw;
     float scale;
     int accumulate, add, bf16, n_pairs;
     uint8_t pair_a[6], pair_b[6];
     int32_t* expired;
+};
+
+__host__ __device__ inline uint32_t tiles_of(uint64_t n, uint32_t of) { return (uint32_t)((n + of - 1) / of); }
+
+// How D_HIDDEN's tiles are shared among the pairs of SMs: rounds of whole tiles while there are enough for every pair; the rest,
+// fewer than the pairs, are cut in K into `shares` each, as many as fill one to four more rounds best. The pairs of a round walk K in
+// step, so that what they read is read once from memory (tiles cut at any step balance as well and read G six times over: 835 -> 1035
+// us a piece of 16384 words, 8192 rows, hidden 2048).
+constexpr uint32_t MIN_SHARE = 8, MAX_ROUNDS = 4;  // steps of K in a share at least
+struct Split {
+    uint32_t tiles, whole, rest, shares;
+    __host__ __device__ Split(uint64_t rows, uint32_t hidden, uint64_t piece, uint32_t pairs) {
+        tiles = tiles_of(rows, MMA_M) * tiles_of(hidden, MMA_N);
+        rest = tiles % pairs;
+        whole = tiles - rest;
+        shares = 1;
+        const uint32_t top = tiles_of(piece, MMA_K) / MIN_SHARE;
+        uint32_t rounds = 1;
+        for (uint32_t r = 1; rest && r <= MAX_ROUNDS; r++) {
+            uint32_t k = r * pairs / rest;
+            if (k > top) k = top;
+            if (k * rounds > shares * r) {  // r / k of a tile's time instead of rounds / shares
+                shares = k;
+                rounds = r;
+            }
+        }
+    }
+    __host__ __device__ uint32_t items() const { return whole + rest * shares; }
 };
 
 // exp(x - m). f32 results take the library's exponential. For 16-bit operands the unit's 2^x of one fused product is ample: it is
@@ -288,17 +328,76 @@ template <bool EXACT> struct ExpFrom {
     }
 };
 
+// G from 32 logits of a row: weight * up / s * (exp(l - m) - [v = t] s). `target`, `valid`: column of the target, columns that exist,
+// both counted from the first of the 32.
+template <bool EXACT>
+__device__ __forceinline__ void logits_to_g(float (&x)[32], const ExpFrom<EXACT>& ex, float s, float factor, uint32_t target, uint32_t valid, bool in) {
+    float hit = 0.f;
+    if (target < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) hit = target == (uint32_t)j ? x[j] : hit;
+        hit = (ex(hit) - s) * factor;
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j++) x[j] = ex(x[j]) * factor;
+    if (target < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) x[j] = target == (uint32_t)j ? hit : x[j];
+    }
+    if (!in || valid < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (!in || j >= (int)valid) x[j] = 0.f;
+    }
+}
+template <typename S, int PARTS>
+__device__ __forceinline__ void store_g(float (&g)[32], S* out, uint64_t part_stride) {
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            w[j] = pack2<S>(g[2 * j], g[2 * j + 1]);
+            if (p + 1 < PARTS) {  // what the part leaves; nothing of an infinity or a NaN
+                const float2 got = unpack2<S>(w[j]);
+                g[2 * j] = isfinite(g[2 * j]) ? g[2 * j] - got.x : 0.f;
+                g[2 * j + 1] = isfinite(g[2 * j + 1]) ? g[2 * j + 1] - got.y : 0.f;
+            }
+        }
+        store32(out + p * part_stride, w);
+        store32(out + p * part_stride + 16, w + 8);
+    }
+}
+// What a scored row brings to its line of G.
+struct RowOfG {
+    uint32_t target;
+    float m, s, factor;
+    __device__ __forceinline__ RowOfG(const ProductArgs& a, uint32_t slot) {
+        const uint32_t row = (uint32_t)a.row_of[slot];
+        const float2 st = a.stats[row];
+        target = (uint32_t)a.targets[row];
+        m = st.x;
+        s = st.y;
+        factor = (a.mask ? a.mask[row] : 1.f) * a.meta->up / s;
+    }
+    __device__ __forceinline__ RowOfG() : target(0xffffffffu), m(0.f), s(1.f), factor(0.f) {}
+};
+
 // T: type of the operands, S: type of the parts they come in, G: type of d_weight; PARTS: parts of G
 template <typename T, typename S, typename G, int P, int PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     k_head_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a) {
-    constexpr bool A_LINES = P == D_WEIGHT, B_LINES = P == D_HIDDEN || P == D_WEIGHT;
+    constexpr bool A_LINES = P == D_WEIGHT, B_LINES = P == D_HIDDEN || P == D_WEIGHT, LOGITS = P == LOGITS_STATS || P == LOGITS_GRAD;
+    constexpr bool F32 = sizeof(T) == 4;
+    // steps of K that stay in an accumulator (0: all): see above. f32 operands add 6 products of 64 a step, the five small ones first;
+    // d_hidden and d_weight in 16 bits hide the cut
+    constexpr uint32_t RUN = F32 ? 2 : LOGITS ? 8 : P == D_WEIGHT && sizeof(G) == 4 ? 4 : 0;
     extern __shared__ __align__(16) unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
     const uint32_t bars = base + STAGES * STAGE_BYTES;
     auto full = [&](uint32_t i) { return bars + 8 * i; };
     auto empty = [&](uint32_t i) { return bars + 8 * (STAGES + i); };
-    auto done = [&](uint32_t i) { return bars + 8 * (2 * STAGES + i); };       // a tile is in accumulator buffer i
+    auto done = [&](uint32_t i) { return bars + 8 * (2 * STAGES + i); };       // a run is in accumulator buffer i
     auto taken = [&](uint32_t i) { return bars + 8 * (2 * STAGES + 2 + i); };  // ... and has been read out by both blocks
     __shared__ uint32_t tmem_at, dead;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, rank = cluster_rank();
@@ -326,33 +425,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_at);
 
     const uint32_t n = a.meta->n;
-    const uint32_t M = P == D_WEIGHT ? a.columns : n, N = P == LOGITS_STATS || P == LOGITS_GRAD ? a.columns : a.hidden;
+    const uint32_t M = P == D_WEIGHT ? a.columns : n, N = LOGITS ? a.columns : a.hidden;
     const uint32_t K = P == D_HIDDEN ? a.columns : P == D_WEIGHT ? n : a.hidden;
-    const uint32_t mt = (M + 255) / 256, nt = (N + 255) / 256, steps_all = (K + 63) / 64;
-    const uint32_t splits = P == D_HIDDEN ? a.splits : 1;
-    const uint32_t tiles = mt * nt * splits, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+    const uint32_t mt = tiles_of(M, MMA_M), nt = tiles_of(N, MMA_N), steps = tiles_of(K, MMA_K);
+    const bool skip = P == LOGITS_GRAD && a.keep && a.meta->kept;  // k_head_grad_kept has made G from the logits that are kept
+    const Split split(n, a.hidden, a.piece, gridDim.x / 2);
     struct Tile {
-        uint32_t m0, n0, width, half, k0, steps, split;
+        uint32_t m0, n0, width, half, k0, steps, share;
     };
+    const uint32_t items = P == D_HIDDEN ? split.items() : skip ? 0 : mt * nt, pairs = gridDim.x / 2;
     auto tile_at = [&](uint32_t t) {
         Tile r;
         uint32_t m, c;
-        if (P == LOGITS_STATS || P == LOGITS_GRAD) {  // the rows run fastest: one stretch of W serves them all
+        r.k0 = 0;
+        r.steps = steps;
+        r.share = 0;
+        if (P == D_HIDDEN && t >= split.whole) {
+            const uint32_t q = t - split.whole;
+            r.share = q / split.rest;
+            t = split.whole + (q - r.share * split.rest);
+            r.k0 = (uint32_t)((uint64_t)steps * r.share / split.shares);
+            r.steps = (uint32_t)((uint64_t)steps * (r.share + 1) / split.shares) - r.k0;
+        }
+        if (LOGITS) {  // the rows run fastest: one stretch of W serves them all
             m = t % mt;
             c = t / mt;
-            r.split = 0;
         } else {
             c = t % nt;
-            const uint32_t q = t / nt;
-            m = q % mt;
-            r.split = q / mt;
+            m = t / nt;
         }
-        r.m0 = m * 256;
-        r.n0 = c * 256;
-        r.width = min(256u, (N - r.n0 + 31) & ~31u);
+        r.m0 = m * MMA_M;
+        r.n0 = c * MMA_N;
+        r.width = min(MMA_N, (N - r.n0 + 31) & ~31u);
         r.half = r.width / 2;
-        r.k0 = (uint32_t)((uint64_t)steps_all * r.split / splits);
-        r.steps = (uint32_t)((uint64_t)steps_all * (r.split + 1) / splits) - r.k0;
         return r;
     };
 
@@ -360,26 +465,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         // ---- loads
         uint32_t it = 0;
         bool ok = true;
-        for (uint32_t t = pair; t < tiles && ok; t += pairs) {
+        for (uint32_t t = blockIdx.x / 2; t < items && ok; t += pairs) {
             const Tile c = tile_at(t);
-            const uint32_t b_boxes = c.half > 64 ? 2 : 1;
-            for (uint32_t p = 0; p < (uint32_t)a.n_pairs && ok; p++) {
-                const int32_t za = a.pair_a[p], zb = a.pair_b[p];
-                for (uint32_t k = 0; k < c.steps; k++, it++) {
-                    const uint32_t st = it % STAGES, use = it / STAGES;
-                    if (!(ok = mbar_wait(empty(st), (use & 1) ^ 1, ws))) break;
-                    const uint32_t to = base + st * STAGE_BYTES, bar = peer_smem(full(st), 0);
-                    if (rank == 0) mbar_expect(full(st), 2 * (2 + b_boxes) * BOX_BYTES);
-                    const int32_t kk = (int32_t)(c.k0 + k) * 64, m = (int32_t)(c.m0 + rank * 128);
-                    const int32_t bn = (int32_t)(c.n0 + rank * c.half + (P == LOGITS_STATS || P == LOGITS_GRAD ? a.first : 0));
-                    const int32_t bk = kk + (int32_t)(P == D_HIDDEN ? a.first : 0);
-                    for (int i = 0; i < 2; i++) {
-                        if (A_LINES) tma_load_pair(to + i * BOX_BYTES, &map_a, m + 64 * i, kk, za, bar);
-                        else tma_load_pair(to + i * BOX_BYTES, &map_a, kk, m + 64 * i, za, bar);
-                    }
-                    for (int i = 0; i < (int)b_boxes; i++) {
-                        if (B_LINES) tma_load_pair(to + (2 + i) * BOX_BYTES, &map_b, bn + 64 * i, bk, zb, bar);
-                        else tma_load_pair(to + (2 + i) * BOX_BYTES, &map_b, bk, bn + 64 * i, zb, bar);
+            const uint32_t b_boxes = c.half > 64 ? 2 : 1, run = RUN ? RUN : c.steps;
+            for (uint32_t k1 = 0; k1 < c.steps && ok; k1 += run) {
+                for (uint32_t p = 0; p < (uint32_t)a.n_pairs && ok; p++) {
+                    const int32_t za = a.pair_a[p], zb = a.pair_b[p];
+                    for (uint32_t k = k1; k < min(k1 + run, c.steps); k++, it++) {
+                        const uint32_t st = it % STAGES, use = it / STAGES;
+                        if (!(ok = mbar_wait(empty(st), (use & 1) ^ 1, ws))) break;
+                        const uint32_t to = base + st * STAGE_BYTES, bar = peer_smem(full(st), 0);
+                        if (rank == 0) mbar_expect(full(st), 2 * (2 + b_boxes) * BOX_BYTES);
+                        const int32_t kk = (int32_t)(c.k0 + k) * 64, m = (int32_t)(c.m0 + rank * 128);
+                        const int32_t bn = (int32_t)(c.n0 + rank * c.half + (LOGITS ? a.first : 0));
+                        const int32_t bk = kk + (int32_t)(P == D_HIDDEN ? a.first : 0);
+                        for (int i = 0; i < 2; i++) {
+                            if (A_LINES) tma_load_pair(to + i * BOX_BYTES, &map_a, m + 64 * i, kk, za, bar);
+                            else tma_load_pair(to + i * BOX_BYTES, &map_a, kk, m + 64 * i, za, bar);
+                        }
+                        for (int i = 0; i < (int)b_boxes; i++) {
+                            if (B_LINES) tma_load_pair(to + (2 + i) * BOX_BYTES, &map_b, bn + 64 * i, bk, zb, bar);
+                            else tma_load_pair(to + (2 + i) * BOX_BYTES, &map_b, bk, bn + 64 * i, zb, bar);
+                        }
                     }
                 }
             }
@@ -392,63 +499,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         // ---- products
         uint32_t it = 0, round = 0;
         bool ok = true;
-        for (uint32_t t = pair; t < tiles && ok; t += pairs, round++) {
+        for (uint32_t t = blockIdx.x / 2; t < items && ok; t += pairs) {
             const Tile c = tile_at(t);
-            const uint32_t total = c.steps * a.n_pairs, buf = round & 1, d = tmem + buf * 256;
-            if (!(ok = mbar_wait(taken(buf), ((round >> 1) & 1) ^ 1, ws))) break;
-            fence_after_sync();
-            const uint32_t idesc = instruction(a.bf16, A_LINES, B_LINES, 256, c.width);
-            for (uint32_t k = 0; k < total; k++, it++) {
-                const uint32_t st = it % STAGES;
-                if (!(ok = mbar_wait(full(st), (it / STAGES) & 1, ws))) break;
+            const uint32_t idesc = instruction(a.bf16, A_LINES, B_LINES, MMA_M, c.width), run = RUN ? RUN : c.steps;
+            for (uint32_t k1 = 0; k1 < c.steps && ok; k1 += run, round++) {
+                const uint32_t total = min(run, c.steps - k1) * a.n_pairs, buf = round & 1, d = tmem + buf * 256;
+                if (!(ok = mbar_wait(taken(buf), ((round >> 1) & 1) ^ 1, ws))) break;
                 fence_after_sync();
-                const uint32_t sa = base + st * STAGE_BYTES, sb = sa + 2 * BOX_BYTES;
+                for (uint32_t k = 0; k < total; k++, it++) {
+                    const uint32_t st = it % STAGES;
+                    if (!(ok = mbar_wait(full(st), (it / STAGES) & 1, ws))) break;
+                    fence_after_sync();
+                    const uint32_t sa = base + st * STAGE_BYTES, sb = sa + 2 * BOX_BYTES;
 #pragma unroll
-                for (int q = 0; q < 4; q++)  // 16 of K: 32 bytes along a line, or 16 lines
-                    mma_pair(d, operand(sa + q * (A_LINES ? 2048 : 32), A_LINES), operand(sb + q * (B_LINES ? 2048 : 32), B_LINES), idesc,
-                             k > 0 || q > 0);
-                commit_pair(empty(st));
+                    for (int q = 0; q < 4; q++)  // 16 of K: 32 bytes along a line, or 16 lines
+                        mma_pair(d, operand(sa + q * (A_LINES ? 2048 : 32), A_LINES), operand(sb + q * (B_LINES ? 2048 : 32), B_LINES), idesc,
+                                 k > 0 || q > 0);
+                    commit_pair(empty(st));
+                }
+                commit_pair(done(buf));
             }
-            commit_pair(done(buf));
         }
     } else if (warp >= 2) {
         // ---- the finished tiles: a warp reads the 32 lanes of its quarter, half of the columns each
         const uint32_t quarter = warp & 3, side = (warp - 2) / 4, row_in = quarter * 32 + lane;
+        const float scale = P == D_WEIGHT ? a.scale * a.meta->down : 1.f;
+        const uint32_t kept = P == LOGITS_STATS && a.keep ? a.meta->kept : 0;
         uint32_t round = 0;
-        for (uint32_t t = pair; t < tiles; t += pairs, round++) {
+        bool ok = true;
+        for (uint32_t t = blockIdx.x / 2; t < items && ok; t += pairs) {
             const Tile c = tile_at(t);
-            const uint32_t buf = round & 1, i = c.m0 + rank * 128 + row_in;
+            const uint32_t i = c.m0 + rank * 128 + row_in;
             const bool in = i < M;
             // what the row needs is fetched while the tile is still being made
-            uint32_t target = 0xffffffffu;
-            float2 s = make_float2(0.f, 1.f);
-            float factor = 0.f;
-            if ((P == LOGITS_STATS || P == LOGITS_GRAD) && in) {
-                const uint32_t row = (uint32_t)a.row_of[i];
-                target = (uint32_t)a.targets[row] - a.first - c.n0;  // column of the tile; far outside it: another tile's
-                if (P == LOGITS_GRAD) {
-                    s = a.stats[row];
-                    factor = (a.mask ? a.mask[row] : 1.f) * a.meta->up / s.y;
-                }
-            }
-            const float scale = P == D_WEIGHT ? a.scale * a.meta->down : 1.f;
-            const bool ok = __all_sync(0xffffffffu, mbar_wait(done(buf), (round >> 1) & 1, ws));
-            if (!ok) break;
-            fence_after_sync();
-            const uint32_t valid = min(256u, N - c.n0);  // columns of the tile that exist
+            RowOfG row;
+            if (P == LOGITS_GRAD && in) row = RowOfG(a, i);
+            if (P == LOGITS_STATS && in) row.target = (uint32_t)a.targets[a.row_of[i]];
+            // column of the tile that the target has; far outside it where another tile has it
+            const uint32_t target = LOGITS && in ? row.target - a.first - c.n0 : 0xffffffffu;
+            const ExpFrom<F32> ex(row.m);
+            const uint32_t valid = min(MMA_N, N - c.n0);  // columns of the tile that exist
             const uint32_t from = side * 128, to = min(from + 128, P == LOGITS_GRAD ? (valid + 63) & ~63u : valid);
-            float2 run = make_float2(-INFINITY, 0.f);
-            for (uint32_t c0 = from; c0 < to; c0 += 32) {
-                uint32_t x[32];
-                const bool made = c.steps > 0 && c0 < c.width;
-                if (made) {
-                    tmem_load32(tmem + buf * 256 + c0 + (quarter << 21), x);
-                    tmem_wait(x);
-                } else {
+            float2 run_stats = make_float2(-INFINITY, 0.f);
+            // one span of 32 columns from c0
+            auto span = [&](uint32_t c0, uint32_t (&x)[32]) {
+                if constexpr (P == LOGITS_STATS) {
+                    if (kept && in) {
+                        float* out = a.l + (uint64_t)i * kept + c.n0 + c0;
 #pragma unroll
-                    for (int j = 0; j < 32; j++) x[j] = 0;
-                }
-                if (P == LOGITS_STATS) {
+                        for (int q = 0; q < 4; q++) store32(out + 8 * q, x + 8 * q);
+                    }
                     if (c0 + 32 > valid) {
 #pragma unroll
                         for (int j = 0; j < 32; j++)
@@ -460,68 +560,104 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                         for (int j = 0; j < 32; j++) tl = target - c0 == (uint32_t)j ? __uint_as_float(x[j]) : tl;
                         a.target_logit[i] = tl;
                     }
-                    float m = run.x;
+                    float m = run_stats.x;
 #pragma unroll
                     for (int j = 0; j < 32; j++) m = fmaxf(m, __uint_as_float(x[j]));
                     const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf yet: exp(-inf - 0) is the zero it should be
-                    const ExpFrom<sizeof(T) == 4> ex(ref);
-                    float part[4] = {run.x == -INFINITY ? run.y : run.y * ex(run.x), 0.f, 0.f, 0.f};
+                    const ExpFrom<F32> e(ref);
+                    float part[4] = {run_stats.x == -INFINITY ? run_stats.y : run_stats.y * e(run_stats.x), 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 32; j++) part[j & 3] += ex(__uint_as_float(x[j]));
-                    run = make_float2(m, (part[0] + part[1]) + (part[2] + part[3]));
-                } else if (P == LOGITS_GRAD) {
-                    const ExpFrom<sizeof(T) == 4> ex(s.x);
+                    for (int j = 0; j < 32; j++) part[j & 3] += e(__uint_as_float(x[j]));
+                    run_stats = make_float2(m, (part[0] + part[1]) + (part[2] + part[3]));
+                } else if constexpr (P == LOGITS_GRAD) {
                     float g[32];
 #pragma unroll
-                    for (int j = 0; j < 32; j++) g[j] = ex(__uint_as_float(x[j])) * factor;
-                    if (target - c0 < 32) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (target - c0 == (uint32_t)j) g[j] = (ex(__uint_as_float(x[j])) - s.y) * factor;
-                    }
-                    if (!in || c0 + 32 > valid) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (!in || c0 + j >= valid) g[j] = 0.f;
-                    }
-                    S* out = static_cast<S*>(a.g) + (uint64_t)i * a.g_pitch + c.n0 + c0;
-#pragma unroll
-                    for (int p = 0; p < PARTS; p++) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            w[j] = pack2<S>(g[2 * j], g[2 * j + 1]);
-                            if (p + 1 < PARTS) {  // what the part leaves; nothing of an infinity or a NaN
-                                const float2 got = unpack2<S>(w[j]);
-                                g[2 * j] = isfinite(g[2 * j]) ? g[2 * j] - got.x : 0.f;
-                                g[2 * j + 1] = isfinite(g[2 * j + 1]) ? g[2 * j + 1] - got.y : 0.f;
-                            }
-                        }
-                        store32(out + p * a.g_part, w);
-                        store32(out + p * a.g_part + 16, w + 8);
-                    }
-                } else if (P == D_HIDDEN) {
+                    for (int j = 0; j < 32; j++) g[j] = __uint_as_float(x[j]);
+                    logits_to_g(g, ex, row.s, row.factor, target - c0, valid - min(valid, c0), in);
+                    store_g<S, PARTS>(g, static_cast<S*>(a.g) + (uint64_t)i * a.g_pitch + c.n0 + c0, a.g_part);
+                } else if constexpr (P == D_HIDDEN) {
                     if (in) {
-                        float* to_dx = a.dx + c.split * a.dx_slab + (uint64_t)i * a.dx_pitch + c.n0 + c0;
+                        // shares after the first are tiles of their own
+                        float* out = c.share == 0 ? a.dx + (uint64_t)i * a.dx_pitch + c.n0 + c0
+                                                  : a.dx_shares + ((uint64_t)(c.share - 1) * split.rest + (c.m0 / MMA_M * nt + c.n0 / MMA_N) - split.whole) * (MMA_M * MMA_N) +
+                                                        (i - c.m0) * MMA_N + c0;
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
                             uint32_t w[8];
-                            if (a.add) load32(to_dx + 8 * q, w);
+                            if (a.add) load32(out + 8 * q, w);
 #pragma unroll
                             for (int j = 0; j < 8; j++)
                                 w[j] = a.add ? __float_as_uint(__uint_as_float(w[j]) + __uint_as_float(x[8 * q + j])) : x[8 * q + j];
-                            store32(to_dx + 8 * q, w);
+                            store32(out + 8 * q, w);
                         }
                     }
                 } else if (in) {
                     G* out = static_cast<G*>(a.dw) + (uint64_t)(a.first + i) * a.hidden + c.n0 + c0;
                     write_span<G>(out, x, min(32u, valid - c0), scale, a.accumulate != 0);
                 }
+            };
+            if constexpr (RUN > 0) {
+                float acc[4][32];
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int j = 0; j < 32; j++) acc[q][j] = 0.f;
+                for (uint32_t k1 = 0; k1 < c.steps; k1 += RUN, round++) {
+                    const uint32_t buf = round & 1;
+                    ok = __all_sync(0xffffffffu, mbar_wait(done(buf), (round >> 1) & 1, ws));
+                    if (!ok) break;
+                    fence_after_sync();
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        if (from + 32 * q >= c.width) break;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 16) {
+                            uint32_t x[16];
+                            tmem_load16(tmem + buf * 256 + from + 32 * q + e + (quarter << 21), x);
+                            tmem_wait(x);
+#pragma unroll
+                            for (int j = 0; j < 16; j++) acc[q][e + j] += __uint_as_float(x[j]);
+                        }
+                    }
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(peer_smem(taken(buf), 0));
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    if (from + 32 * q >= to) break;
+                    uint32_t x[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) x[j] = __float_as_uint(acc[q][j]);
+                    span(from + 32 * q, x);
+                }
+            } else {
+                const uint32_t buf = round & 1;
+                if (c.steps) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(done(buf), (round >> 1) & 1, ws));
+                    if (!ok) break;
+                    fence_after_sync();
+                }
+                for (uint32_t c0 = from; c0 < to; c0 += 32) {
+                    uint32_t x[32];
+                    if (c.steps) {
+                        tmem_load32(tmem + buf * 256 + c0 + (quarter << 21), x);
+                        tmem_wait(x);
+                    } else {  // no scored row: a sum of nothing
+#pragma unroll
+                        for (int j = 0; j < 32; j++) x[j] = 0;
+                    }
+                    span(c0, x);
+                }
+                if (c.steps) {
+                    round++;
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(peer_smem(taken(buf), 0));
+                }
             }
-            if (P == LOGITS_STATS && in) a.part[(uint64_t)(2 * (c.n0 / 256) + side) * a.pitch + i] = run;
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(peer_smem(taken(buf), 0));
+            if (P == LOGITS_STATS && in) a.part[(uint64_t)(2 * (c.n0 / MMA_N) + side) * a.pitch + i] = run_stats;
         }
     }
     __syncwarp();
@@ -532,20 +668,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     if (warp == 1) tmem_free_pair(tmem, 512);
 }
 
-// ---- d_hidden: the scored rows' sums over the splits, in their order, times the scale, rounded; zeros for the others
-template <typename T>
-__global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t hidden, uint32_t dx_pitch, uint32_t splits, uint64_t dx_slab,
-                                                       const int32_t* __restrict__ slot_of, const float* __restrict__ dx,
-                                                       const HeadMeta* __restrict__ meta, float scale, T* out, uint64_t stride) {
-    scale *= meta->down;
-    const uint64_t total = (uint64_t)rows * hidden;
+// ---- a piece of G from logits that the losses have kept, the same bits as the product would give. A thread takes 32 columns of a
+// scored row; the rows up to the next multiple of a tile are zeros, as every line of G that a product reads.
+template <typename T, typename S, int PARTS>
+__global__ void __launch_bounds__(256) k_head_grad_kept(const ProductArgs a) {
+    const uint32_t n = a.meta->n, kept = a.meta->kept;
+    if (kept == 0 || n == 0) return;
+    const uint32_t per = ((a.columns + 63) & ~63u) / 32;
+    const uint64_t total = (uint64_t)tiles_of(n, MMA_M) * MMA_M * per;
     for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
-        const uint32_t row = (uint32_t)(e / hidden), col = (uint32_t)(e - (uint64_t)row * hidden);
+        const uint32_t slot = (uint32_t)(e / per), c0 = (uint32_t)(e - (uint64_t)slot * per) * 32;
+        const bool in = slot < n;
+        RowOfG row;
+        float g[32];
+        if (in) {
+            row = RowOfG(a, slot);
+            const float* from = a.l + (uint64_t)slot * kept + a.first + c0;
+#pragma unroll
+            for (int q = 0; q < 4; q++) load32(from + 8 * q, reinterpret_cast<uint32_t*>(g) + 8 * q);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) g[j] = 0.f;
+        }
+        const ExpFrom<sizeof(T) == 4> ex(row.m);
+        logits_to_g(g, ex, row.s, row.factor, in ? row.target - a.first - c0 : 0xffffffffu, a.columns - min(a.columns, c0), in);
+        store_g<S, PARTS>(g, static_cast<S*>(a.g) + (uint64_t)slot * a.g_pitch + c0, a.g_part);
+    }
+}
+
+// ---- d_hidden: the scored rows' sums, their shares in order, times the scale, rounded; zeros for the others
+template <typename T, int N>
+__global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t hidden, uint32_t dx_pitch, uint64_t piece, uint32_t pairs,
+                                                       const int32_t* __restrict__ slot_of, const float* __restrict__ dx,
+                                                       const float* __restrict__ dx_shares, const HeadMeta* __restrict__ meta, float scale, T* out,
+                                                       uint64_t stride) {
+    scale *= meta->down;
+    const Split split(meta->n, hidden, piece, pairs);
+    const uint32_t per = (hidden + N - 1) / N, nt = tiles_of(hidden, MMA_N);
+    const uint64_t total = (uint64_t)rows * per;
+    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
+        const uint32_t row = (uint32_t)(e / per), col = (uint32_t)(e - (uint64_t)row * per) * N;
         const int32_t slot = slot_of[row];
-        float sum = 0.f;
-        if (slot >= 0)
-            for (uint32_t k = 0; k < splits; k++) sum += dx[k * dx_slab + (uint64_t)slot * dx_pitch + col];
-        out[(uint64_t)row * stride + col] = from_f32<T>(slot < 0 ? 0.f : sum * scale);
+        Vec<float, N> sum;
+#pragma unroll
+        for (int j = 0; j < N; j++) sum.e[j] = 0.f;
+        if (slot >= 0) {
+            sum.load(dx + (uint64_t)slot * dx_pitch + col);
+            const uint32_t tile = slot / MMA_M * nt + col / MMA_N;
+            const float* from = dx_shares + ((uint64_t)tile - split.whole) * (MMA_M * MMA_N) + slot % MMA_M * MMA_N + col % MMA_N;
+            if (tile >= split.whole)
+                for (uint32_t k = 1; k < split.shares; k++, from += (uint64_t)split.rest * (MMA_M * MMA_N)) {
+                    Vec<float, N> v;
+                    v.load(from);
+#pragma unroll
+                    for (int j = 0; j < N; j++) sum.e[j] += v.e[j];
+                }
+        }
+        Vec<T, N> o;
+#pragma unroll
+        for (int j = 0; j < N; j++) o.e[j] = from_f32<T>(slot < 0 ? 0.f : sum.e[j] * scale);
+        o.store(out + (uint64_t)row * stride + col);
     }
 }
 
@@ -582,8 +764,10 @@ template <typename T, typename S, typename G, int PARTS>
 struct Products {
     template <int P>
     static void launch(const oxz_head* h, const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, uint64_t m, uint64_t n, cudaStream_t s) {
-        const uint64_t tiles = (m + MMA_M - 1) / MMA_M * ((n + MMA_N - 1) / MMA_N) * (P == D_HIDDEN ? a.splits : 1);
-        if (tiles) k_head_product<T, S, G, P, PARTS><<<2 * (unsigned)std::min<uint64_t>(tiles, h->clusters), MMA_THREADS, MMA_SMEM, s>>>(ma, mb, a);
+        const uint64_t tiles = (uint64_t)tiles_of(m, MMA_M) * tiles_of(n, MMA_N);
+        // the cut of D_HIDDEN goes by the number of pairs: always all of them
+        const unsigned pairs = P == D_HIDDEN ? (unsigned)h->clusters : (unsigned)std::min<uint64_t>(tiles, h->clusters);
+        if (tiles) k_head_product<T, S, G, P, PARTS><<<2 * pairs, MMA_THREADS, MMA_SMEM, s>>>(ma, mb, a);
     }
     template <int P>
     static int32_t prepare(int* clusters) {
@@ -617,7 +801,8 @@ struct Products {
         constexpr bool F32 = sizeof(T) == 4, BF16 = std::is_same<S, __nv_bfloat16>::value;
         const size_t es = sizeof(T);
         const unsigned many = (unsigned)h->clusters * 2 * 8;  // blocks of the elementwise kernels
-        k_head_rows<<<1, 1024, 0, s>>>(b.targets, b.loss_mask, (uint32_t)b.rows, d.vocab, h->row_of, h->slot_of, h->meta, !BF16);
+        k_head_rows<<<1, 1024, 0, s>>>(b.targets, b.loss_mask, (uint32_t)b.rows, d.vocab, h->row_of, h->slot_of, h->meta, !BF16,
+                                    want_loss && gr ? h->l_elems : 0);
         const uint64_t x_part = h->cap * h->pitch, w_part = d.vocab * h->pitch;
         const bool x_wide = !misaligned(b.hidden, 16) && b.hidden_stride * es % 16 == 0;
         if (b.rows) {
@@ -645,7 +830,11 @@ struct Products {
         a.target_logit = h->target_logit;
         a.g = h->g;
         a.dx = h->dx;
+        a.l = h->l;
         a.bf16 = BF16;
+        a.dx_shares = h->dx_shares;
+        a.piece = (uint32_t)h->piece;
+        a.keep = want_loss && gr;
         a.expired = h->d_expired;
         // an f32 operand is hi + mid + lo; of the nine products the six above 2^-24 are formed, the small ones first
         static const uint8_t six[2][6] = {{2, 1, 0, 1, 0, 0}, {0, 1, 2, 0, 1, 0}};
@@ -662,7 +851,7 @@ struct Products {
             a.columns = (uint32_t)d.vocab;
             launch<LOGITS_STATS>(h, mx, mw, a, b.rows, d.vocab, s);
             const unsigned blocks = std::max<unsigned>(1, (unsigned)((b.rows + FINISH_ROWS - 1) / FINISH_ROWS));
-            k_head_finish<<<blocks, 32 * FINISH_ROWS, 0, s>>>((uint32_t)b.rows, a.pitch, 2 * (uint32_t)((d.vocab + MMA_N - 1) / MMA_N), h->slot_of,
+            k_head_finish<<<blocks, 1024, 0, s>>>((uint32_t)b.rows, a.pitch, 2 * (uint32_t)((d.vocab + MMA_N - 1) / MMA_N), h->slot_of,
                                                               h->part, h->target_logit, b.loss_mask, stats, row_loss, h->loss_part, h->meta, totals);
         }
         if (!gr) return OXZ_OK;
@@ -673,24 +862,27 @@ struct Products {
         a.g_pitch = (uint32_t)h->piece;
         a.g_part = h->cap * h->piece;
         OXZ_TRY(tensor_map(&mg, BF16, h->g, h->piece, h->cap, h->g_parts, a.g_part));
-        // few output tiles of d_hidden: K, the vocabulary of a piece, is split so that every pair has work
-        const uint64_t mt = (b.rows + MMA_M - 1) / MMA_M, nt = (d.hidden + MMA_N - 1) / MMA_N;
-        a.splits = mt ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(h->clusters / (mt * nt), h->piece / MMA_K)) : 1;
-        a.dx_slab = mt * MMA_M * h->dx_pitch;
+        const bool sure = b.rows * h->kept_pitch <= h->l_elems;  // kept whatever the mask
         for (uint64_t v = 0; v < d.vocab; v += h->piece) {
             a.first = (uint32_t)v;
             a.columns = (uint32_t)std::min(h->piece, d.vocab - v);
             a.add = v > 0;
             pairs(1);
-            launch<LOGITS_GRAD>(h, mx, mw, a, b.rows, a.columns, s);
+            // the scored rows' count decides on the device which of the two has work
+            if (a.keep && b.rows && h->l_elems) k_head_grad_kept<T, S, PARTS><<<many, 256, 0, s>>>(a);
+            if (!a.keep || !sure) launch<LOGITS_GRAD>(h, mx, mw, a, b.rows, a.columns, s);
             if (gr->d_hidden) launch<D_HIDDEN>(h, mg, mw, a, b.rows, d.hidden, s);
             pairs(h->g_parts);
             if (gr->d_weight) launch<D_WEIGHT>(h, mg, mx, a, a.columns, d.hidden, s);
         }
-        if (gr->d_hidden && b.rows)
-            k_head_d_hidden<T><<<(unsigned)std::min<uint64_t>((b.rows * d.hidden + 255) / 256, many), 256, 0, s>>>(
-                (uint32_t)b.rows, (uint32_t)d.hidden, h->dx_pitch, a.splits, a.dx_slab, h->slot_of, h->dx, h->meta, a.scale,
+        if (gr->d_hidden && b.rows) {
+            constexpr int N = 16 / (int)sizeof(T);
+            const bool wide = !misaligned(gr->d_hidden, 16) && gr->d_hidden_stride * es % 16 == 0 && d.hidden % N == 0;
+            auto k = wide ? k_head_d_hidden<T, N> : k_head_d_hidden<T, 1>;
+            k<<<(unsigned)std::min<uint64_t>((b.rows * d.hidden / (wide ? N : 1) + 255) / 256, many), 256, 0, s>>>(
+                (uint32_t)b.rows, (uint32_t)d.hidden, h->dx_pitch, h->piece, (uint32_t)h->clusters, h->slot_of, h->dx, h->dx_shares, h->meta, a.scale,
                 static_cast<T*>(gr->d_hidden), gr->d_hidden_stride);
+        }
         return OXZ_OK;
     }
 };
@@ -789,7 +981,8 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             h->parts = d.dtype == OXZ_F32 ? 3 : 1;
             h->g_parts = d.grad_dtype == OXZ_F32 ? 3 : 1;
             OXZ_TRY(with_types(d, [&](auto p) { return decltype(p)::prepare_all(h); }));
-            const uint64_t limit = d.piece_bytes ? d.piece_bytes : 512ull << 20;
+            // a third of the limit for a piece's G, the rest for logits that are kept, where there are so many
+            const uint64_t budget = d.piece_bytes ? d.piece_bytes : 1536ull << 20, limit = budget / 3;
             const uint64_t all = (d.vocab + MMA_N - 1) / MMA_N * MMA_N;
             h->piece = std::min(all, std::max<uint64_t>(MMA_N, limit / (h->cap * 2 * h->g_parts) / MMA_N * MMA_N));
             uint64_t bytes = 0;
@@ -808,8 +1001,14 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             OXZ_TRY(get(&h->x, h->cap * h->pitch * h->parts * 2));
             if (d.dtype == OXZ_F32 || d.hidden % 8) OXZ_TRY(get(&h->w, d.vocab * h->pitch * h->parts * 2));
             OXZ_TRY(get(&h->g, h->cap * h->piece * h->g_parts * 2));
-            // splits x tiles of d_hidden is at most the pairs wherever there is more than one split
-            OXZ_TRY(get(&h->dx, std::max<uint64_t>((uint64_t)h->clusters * MMA_M * MMA_N, h->cap * h->dx_pitch) * 4));
+            h->kept_pitch = all;
+            // kept logits are written and read once (10 bytes of traffic an element with G's 2: 1.6 ps measured); forming them again
+            // takes 2 x hidden operations on the tensor cores, six times that for f32 (0.85 ps at hidden 384, 2.9 at 2048, 16 bits)
+            h->l_elems = d.hidden * (d.dtype == OXZ_F32 ? 6 : 1) >= 1024 ? std::min(budget / 3 * 2 / 4, h->cap * all) : 0;
+            if (h->l_elems) OXZ_TRY(get(&h->l, h->l_elems * 4));
+            OXZ_TRY(get(&h->dx, h->cap * h->dx_pitch * 4));
+            // rest x shares is at most MAX_ROUNDS x pairs
+            OXZ_TRY(get(&h->dx_shares, (uint64_t)MAX_ROUNDS * h->clusters * MMA_M * MMA_N * 4));
             if (!h->expired) {
                 OXZ_CUDA(cudaHostAlloc((void**)&h->expired, 4, cudaHostAllocMapped));
                 *h->expired = 0;
@@ -831,7 +1030,7 @@ int32_t oxz_head_destroy(oxz_head* h) {
         if (h->row_of) dev.enter(h->d.device);
         h->order.destroy();
         for (void* p : {(void*)h->row_of, (void*)h->slot_of, (void*)h->part, (void*)h->target_logit, (void*)h->stats, (void*)h->loss_part,
-                        (void*)h->meta, h->x, h->w, h->g, (void*)h->dx})
+                        (void*)h->meta, h->x, h->w, h->g, (void*)h->l, (void*)h->dx, (void*)h->dx_shares})
             if (p) cudaFree(p);
         if (h->expired) cudaFreeHost(h->expired);
         delete h;
