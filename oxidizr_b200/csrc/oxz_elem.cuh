@@ -8,6 +8,12 @@
 
 namespace oxz {
 
+// Launches overlap (launch_after, programmatic dependent launch): a kernel may start while the one before it in the stream still runs.
+// after_previous() waits until that one has ended and what it wrote is visible; every thread of every kernel calls it before it ends,
+// so that the end of a kernel is also the end of all before it. let_next() allows the next kernel to start.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }

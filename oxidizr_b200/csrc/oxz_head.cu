@@ -70,6 +70,7 @@ constexpr uint32_t MMA_M = 256, MMA_N = 256, MMA_K = 64;  // tile of a pair of S
 __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ targets, const float* __restrict__ mask, uint32_t rows,
                                                     uint64_t vocab, int32_t* row_of, int32_t* slot_of, HeadMeta* meta, int f16,
                                                     uint64_t l_elems) {
+    let_next();
     __shared__ uint32_t counts[32];
     __shared__ double wsum[32];
     __shared__ float wtop[32];
@@ -146,7 +147,10 @@ __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pi
                                                       const float* __restrict__ mask, float2* stats, float* row_loss, double* loss_part,
                                                       HeadMeta* meta, float* totals) {
     __shared__ float2 share[32][33];
+    __shared__ double mine[32];
     __shared__ uint32_t last;
+    let_next();
+    after_previous();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, row = blockIdx.x * FINISH_ROWS + lane;
     const int32_t slot = row < rows ? slot_of[row] : -1;
     float2 s = make_float2(-INFINITY, 0.f);
@@ -161,27 +165,36 @@ __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pi
     }
     share[warp][lane] = s;
     __syncthreads();
-    if (warp) return;
-    for (int w = 1; w < 32; w++) s = join(s, share[w][lane]);
-    double mine = 0.0;
-    if (row < rows) {
-        const float loss = slot >= 0 ? logf(s.y) - (target_logit[slot] - s.x) : 0.f;
-        stats[row] = slot >= 0 ? s : make_float2(0.f, 0.f);
-        if (row_loss) row_loss[row] = loss;
-        mine = slot >= 0 ? (mask ? (double)mask[row] : 1.0) * (double)loss : 0.0;
+    // now a warp has one row, a lane one of its parts
+    s = share[lane][warp];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) s = join(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
+    const uint32_t own = blockIdx.x * FINISH_ROWS + warp;
+    if (lane == 0) {
+        mine[warp] = 0.0;
+        if (own < rows) {
+            const int32_t at = slot_of[own];
+            const float loss = at >= 0 ? logf(s.y) - (target_logit[at] - s.x) : 0.f;
+            stats[own] = at >= 0 ? s : make_float2(0.f, 0.f);
+            if (row_loss) row_loss[own] = loss;
+            if (at >= 0) mine[warp] = (mask ? (double)mask[own] : 1.0) * (double)loss;
+        }
     }
     if (!totals) return;
+    __syncthreads();
+    if (warp) return;
+    double sum = mine[lane];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
-        loss_part[blockIdx.x] = mine;
+        loss_part[blockIdx.x] = sum;
         __threadfence();
         last = atomicAdd(&meta->done, 1u) == gridDim.x - 1;
     }
     __syncwarp();
     if (!last) return;
     __threadfence();
-    double sum = 0.0;
+    sum = 0.0;
     for (uint32_t b = lane; b < gridDim.x; b += 32) sum += __ldcg(&loss_part[b]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -222,6 +235,8 @@ template <typename T, typename S>
 __global__ void __launch_bounds__(256) k_head_pack(const T* __restrict__ src, uint64_t stride, uint32_t hidden, uint32_t pitch, uint64_t rows,
                                                    const int32_t* __restrict__ row_of, const HeadMeta* __restrict__ meta, S* out,
                                                    uint64_t part_stride, int parts, int wide) {
+    let_next();
+    after_previous();
     const uint32_t n = row_of ? meta->n : (uint32_t)rows, per = pitch / 8;
     const uint64_t total = (row_of ? (uint64_t)(n + MMA_M - 1) / MMA_M * MMA_M : rows) * per;
     for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
@@ -264,7 +279,8 @@ __global__ void __launch_bounds__(256) k_head_pack(const T* __restrict__ src, ui
 // the lines of their tiles. Values of more than 16 bits come in parts; a product of such operands is the sum over `pairs` of parts.
 enum Product { LOGITS_STATS, LOGITS_GRAD, D_HIDDEN, D_WEIGHT };
 constexpr int STAGES = 6, MMA_THREADS = 320, EPILOGUE_WARPS = 8;
-constexpr uint32_t STAGE_BYTES = 4 * BOX_BYTES, MMA_SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr uint32_t STAGE_BYTES = 4 * BOX_BYTES, OUT_BYTES = 32 * 128;
+constexpr uint32_t MMA_SMEM = STAGES * STAGE_BYTES + EPILOGUE_WARPS * OUT_BYTES + 1024 + 256;
 
 struct ProductArgs {
     const HeadMeta* meta;
@@ -282,6 +298,8 @@ struct ProductArgs {
     void* dw;
     float scale;
     int accumulate, add, bf16, n_pairs;
+    int boxes;   // d_weight leaves by TMA
+    int beside;  // d_weight starts beside d_hidden, on which it does not depend
     uint8_t pair_a[6], pair_b[6];
     int32_t* expired;
 };
@@ -350,23 +368,16 @@ __device__ __forceinline__ void logits_to_g(float (&x)[32], const ExpFrom<EXACT>
             if (!in || j >= (int)valid) x[j] = 0.f;
     }
 }
-template <typename S, int PARTS>
-__device__ __forceinline__ void store_g(float (&g)[32], S* out, uint64_t part_stride) {
-#pragma unroll
-    for (int p = 0; p < PARTS; p++) {
-        uint32_t w[16];
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            w[j] = pack2<S>(g[2 * j], g[2 * j + 1]);
-            if (p + 1 < PARTS) {  // what the part leaves; nothing of an infinity or a NaN
-                const float2 got = unpack2<S>(w[j]);
-                g[2 * j] = isfinite(g[2 * j]) ? g[2 * j] - got.x : 0.f;
-                g[2 * j + 1] = isfinite(g[2 * j + 1]) ? g[2 * j + 1] - got.y : 0.f;
-            }
-        }
-        store32(out + p * part_stride, w);
-        store32(out + p * part_stride + 16, w + 8);
+// Two values as 16-bit ones, rounded; with `more`, they are left as what the rounding leaves (nothing of an infinity or a NaN).
+template <typename S>
+__device__ __forceinline__ uint32_t next_part(float& lo, float& hi, bool more) {
+    const uint32_t w = pack2<S>(lo, hi);
+    if (more) {
+        const float2 got = unpack2<S>(w);
+        lo = isfinite(lo) ? lo - got.x : 0.f;
+        hi = isfinite(hi) ? hi - got.y : 0.f;
     }
+    return w;
 }
 // What a scored row brings to its line of G.
 struct RowOfG {
@@ -386,7 +397,8 @@ struct RowOfG {
 // T: type of the operands, S: type of the parts they come in, G: type of d_weight; PARTS: parts of G
 template <typename T, typename S, typename G, int P, int PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
-    k_head_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a) {
+    k_head_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_shares, const ProductArgs a) {
     constexpr bool A_LINES = P == D_WEIGHT, B_LINES = P == D_HIDDEN || P == D_WEIGHT, LOGITS = P == LOGITS_STATS || P == LOGITS_GRAD;
     constexpr bool F32 = sizeof(T) == 4;
     // steps of K that stay in an accumulator (0: all): see above. f32 operands add 6 products of 64 a step, the five small ones first;
@@ -394,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     constexpr uint32_t RUN = F32 ? 2 : LOGITS ? 8 : P == D_WEIGHT && sizeof(G) == 4 ? 4 : 0;
     extern __shared__ __align__(16) unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t bars = base + STAGES * STAGE_BYTES;
+    const uint32_t bars = base + STAGES * STAGE_BYTES + EPILOGUE_WARPS * OUT_BYTES;
     auto full = [&](uint32_t i) { return bars + 8 * i; };
     auto empty = [&](uint32_t i) { return bars + 8 * (STAGES + i); };
     auto done = [&](uint32_t i) { return bars + 8 * (2 * STAGES + i); };       // a run is in accumulator buffer i
@@ -416,6 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tma_prefetch_map(&map_a);
         tma_prefetch_map(&map_b);
+        tma_prefetch_map(&map_out);
     }
     if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_at), 512);
     fence_before_sync();
@@ -423,6 +436,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     cluster_sync();
     fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_at);
+    if (!a.beside) after_previous();
+    let_next();
 
     const uint32_t n = a.meta->n;
     const uint32_t M = P == D_WEIGHT ? a.columns : n, N = LOGITS ? a.columns : a.hidden;
@@ -523,6 +538,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     } else if (warp >= 2) {
         // ---- the finished tiles: a warp reads the 32 lanes of its quarter, half of the columns each
         const uint32_t quarter = warp & 3, side = (warp - 2) / 4, row_in = quarter * 32 + lane;
+        const uint32_t out_at = base + STAGES * STAGE_BYTES + (warp - 2) * OUT_BYTES;
         const float scale = P == D_WEIGHT ? a.scale * a.meta->down : 1.f;
         const uint32_t kept = P == LOGITS_STATS && a.keep ? a.meta->kept : 0;
         uint32_t round = 0;
@@ -540,125 +556,140 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             const ExpFrom<F32> ex(row.m);
             const uint32_t valid = min(MMA_N, N - c.n0);  // columns of the tile that exist
             const uint32_t from = side * 128, to = min(from + 128, P == LOGITS_GRAD ? (valid + 63) & ~63u : valid);
-            float2 run_stats = make_float2(-INFINITY, 0.f);
-            // one span of 32 columns from c0
-            auto span = [&](uint32_t c0, uint32_t (&x)[32]) {
-                if constexpr (P == LOGITS_STATS) {
-                    if (kept && in) {
-                        float* out = a.l + (uint64_t)i * kept + c.n0 + c0;
+            // the tile's 128 columns of this warp leave tensor memory at once, which frees the accumulator for the next tile
+            float acc[4][32];
 #pragma unroll
-                        for (int q = 0; q < 4; q++) store32(out + 8 * q, x + 8 * q);
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int j = 0; j < 32; j++) acc[q][j] = 0.f;
+            for (uint32_t k1 = 0; k1 < c.steps; k1 += RUN ? RUN : c.steps, round++) {
+                const uint32_t buf = round & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(done(buf), (round >> 1) & 1, ws));
+                if (!ok) break;
+                fence_after_sync();
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    if (from + 32 * q >= c.width) break;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 16) {
+                        uint32_t x[16];
+                        tmem_load16(tmem + buf * 256 + from + 32 * q + e + (quarter << 21), x);
+                        tmem_wait(x);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) acc[q][e + j] = RUN ? acc[q][e + j] + __uint_as_float(x[j]) : __uint_as_float(x[j]);
+                    }
+                }
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(peer_smem(taken(buf), 0));
+            }
+            if (!ok) break;
+            const int32_t line = (int32_t)(c.m0 + rank * 128 + quarter * 32);  // the warp's first row
+            // 128 bytes of each of the warp's rows go out as one box: 16-byte pieces in the order of the 128-byte swizzle, no two lanes of
+            // a quarter warp in one bank
+            auto box = [&](const CUtensorMap& map, int32_t x, int32_t y, int32_t z, const uint32_t (&w)[32], bool add) {
+                if (lane == 0) store_read();
+                __syncwarp();
+#pragma unroll
+                for (int p = 0; p < 8; p++) st_shared16(out_at + lane * 128 + ((p ^ (lane & 7)) << 4), w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+                store_fence();
+                __syncwarp();
+                if (lane == 0) {
+                    if (add) tma_add(&map, x, y, z, out_at);
+                    else tma_store(&map, x, y, z, out_at);
+                }
+            };
+            auto words = [&](int q, uint32_t (&w)[32]) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) w[j] = __float_as_uint(acc[q][j]);
+            };
+            if constexpr (P == LOGITS_STATS) {
+                float2 run_stats = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t c0 = from + 32 * q;
+                    if (c0 >= to) break;
+                    if (kept) {
+                        uint32_t w[32];
+                        words(q, w);
+                        box(map_out, (int32_t)(c.n0 + c0), line, 0, w, false);
                     }
                     if (c0 + 32 > valid) {
 #pragma unroll
                         for (int j = 0; j < 32; j++)
-                            if (c0 + j >= valid) x[j] = 0xff800000u;  // -inf: no word of the vocabulary
+                            if (c0 + j >= valid) acc[q][j] = -INFINITY;  // no word of the vocabulary
                     }
                     if (target - c0 < 32) {
                         float tl = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 32; j++) tl = target - c0 == (uint32_t)j ? __uint_as_float(x[j]) : tl;
+                        for (int j = 0; j < 32; j++) tl = target - c0 == (uint32_t)j ? acc[q][j] : tl;
                         a.target_logit[i] = tl;
                     }
                     float m = run_stats.x;
 #pragma unroll
-                    for (int j = 0; j < 32; j++) m = fmaxf(m, __uint_as_float(x[j]));
+                    for (int j = 0; j < 32; j++) m = fmaxf(m, acc[q][j]);
                     const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf yet: exp(-inf - 0) is the zero it should be
                     const ExpFrom<F32> e(ref);
                     float part[4] = {run_stats.x == -INFINITY ? run_stats.y : run_stats.y * e(run_stats.x), 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 32; j++) part[j & 3] += e(__uint_as_float(x[j]));
+                    for (int j = 0; j < 32; j++) part[j & 3] += e(acc[q][j]);
                     run_stats = make_float2(m, (part[0] + part[1]) + (part[2] + part[3]));
-                } else if constexpr (P == LOGITS_GRAD) {
-                    float g[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) g[j] = __uint_as_float(x[j]);
-                    logits_to_g(g, ex, row.s, row.factor, target - c0, valid - min(valid, c0), in);
-                    store_g<S, PARTS>(g, static_cast<S*>(a.g) + (uint64_t)i * a.g_pitch + c.n0 + c0, a.g_part);
-                } else if constexpr (P == D_HIDDEN) {
-                    if (in) {
-                        // shares after the first are tiles of their own
-                        float* out = c.share == 0 ? a.dx + (uint64_t)i * a.dx_pitch + c.n0 + c0
-                                                  : a.dx_shares + ((uint64_t)(c.share - 1) * split.rest + (c.m0 / MMA_M * nt + c.n0 / MMA_N) - split.whole) * (MMA_M * MMA_N) +
-                                                        (i - c.m0) * MMA_N + c0;
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            uint32_t w[8];
-                            if (a.add) load32(out + 8 * q, w);
-#pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                w[j] = a.add ? __float_as_uint(__uint_as_float(w[j]) + __uint_as_float(x[8 * q + j])) : x[8 * q + j];
-                            store32(out + 8 * q, w);
-                        }
-                    }
-                } else if (in) {
-                    G* out = static_cast<G*>(a.dw) + (uint64_t)(a.first + i) * a.hidden + c.n0 + c0;
-                    write_span<G>(out, x, min(32u, valid - c0), scale, a.accumulate != 0);
                 }
-            };
-            if constexpr (RUN > 0) {
-                float acc[4][32];
+                if (in) a.part[(uint64_t)(2 * (c.n0 / MMA_N) + side) * a.pitch + i] = run_stats;
+            } else if constexpr (P == LOGITS_GRAD) {
 #pragma unroll
-                for (int q = 0; q < 4; q++)
+                for (int q = 0; q < 4; q += 2) {
+                    const uint32_t c0 = from + 32 * q;
+                    if (c0 >= to) break;
 #pragma unroll
-                    for (int j = 0; j < 32; j++) acc[q][j] = 0.f;
-                for (uint32_t k1 = 0; k1 < c.steps; k1 += RUN, round++) {
-                    const uint32_t buf = round & 1;
-                    ok = __all_sync(0xffffffffu, mbar_wait(done(buf), (round >> 1) & 1, ws));
-                    if (!ok) break;
-                    fence_after_sync();
+                    for (int e = 0; e < 2; e++)
+                        logits_to_g(acc[q + e], ex, row.s, row.factor, target - c0 - 32 * e, valid - min(valid, c0 + 32 * e), in);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        if (from + 32 * q >= c.width) break;
+                    for (int p = 0; p < PARTS; p++) {
+                        uint32_t w[32];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 16) {
-                            uint32_t x[16];
-                            tmem_load16(tmem + buf * 256 + from + 32 * q + e + (quarter << 21), x);
-                            tmem_wait(x);
-#pragma unroll
-                            for (int j = 0; j < 16; j++) acc[q][e + j] += __uint_as_float(x[j]);
-                        }
+                        for (int j = 0; j < 32; j++) w[j] = next_part<S>(acc[q + j / 16][2 * (j & 15)], acc[q + j / 16][2 * (j & 15) + 1], p + 1 < PARTS);
+                        box(map_out, (int32_t)(c.n0 + c0), line, p, w, false);
                     }
-                    fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(peer_smem(taken(buf), 0));
                 }
-                if (!ok) break;
+            } else if constexpr (P == D_HIDDEN) {
+                // shares after the first are tiles of their own
+                const uint32_t tile = (c.share - 1) * split.rest + (c.m0 / MMA_M * nt + c.n0 / MMA_N) - split.whole;
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    if (from + 32 * q >= to) break;
-                    uint32_t x[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) x[j] = __float_as_uint(acc[q][j]);
-                    span(from + 32 * q, x);
+                    const uint32_t c0 = from + 32 * q;
+                    if (c0 >= to) break;
+                    uint32_t w[32];
+                    words(q, w);
+                    if (c.share == 0) box(map_out, (int32_t)(c.n0 + c0), line, 0, w, a.add);
+                    else box(map_shares, (int32_t)c0, (int32_t)(tile * MMA_M + (line - c.m0)), 0, w, a.add);
                 }
-            } else {
-                const uint32_t buf = round & 1;
-                if (c.steps) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(done(buf), (round >> 1) & 1, ws));
-                    if (!ok) break;
-                    fence_after_sync();
-                }
-                for (uint32_t c0 = from; c0 < to; c0 += 32) {
-                    uint32_t x[32];
-                    if (c.steps) {
-                        tmem_load32(tmem + buf * 256 + c0 + (quarter << 21), x);
-                        tmem_wait(x);
-                    } else {  // no scored row: a sum of nothing
+            } else if (a.boxes) {
+                constexpr int PER = 4 / (int)sizeof(G);  // spans of 32 columns in a box
 #pragma unroll
-                        for (int j = 0; j < 32; j++) x[j] = 0;
+                for (int q = 0; q < 4; q += PER) {
+                    const uint32_t c0 = from + 32 * q;
+                    if (c0 >= to) break;
+                    uint32_t w[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        if constexpr (sizeof(G) == 4) w[j] = __float_as_uint(acc[q][j] * scale);
+                        else w[j] = pack2<G>(acc[q + j / 16][2 * (j & 15)] * scale, acc[q + j / 16][2 * (j & 15) + 1] * scale);
                     }
-                    span(c0, x);
+                    box(map_out, (int32_t)(c.n0 + c0), (int32_t)a.first + line, 0, w, sizeof(G) == 4 && a.accumulate);
                 }
-                if (c.steps) {
-                    round++;
-                    fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(peer_smem(taken(buf), 0));
+            } else if (in) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t c0 = from + 32 * q;
+                    if (c0 >= to) break;
+                    uint32_t w[32];
+                    words(q, w);
+                    write_span<G>(static_cast<G*>(a.dw) + (uint64_t)(a.first + i) * a.hidden + c.n0 + c0, w, min(32u, valid - c0), scale, a.accumulate != 0);
                 }
             }
-            if (P == LOGITS_STATS && in) a.part[(uint64_t)(2 * (c.n0 / MMA_N) + side) * a.pitch + i] = run_stats;
         }
+        if (lane == 0) store_done();
     }
     __syncwarp();
     fence_before_sync();
@@ -666,12 +697,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     cluster_sync();  // nobody arrives at a barrier of a block that has ended
     fence_after_sync();
     if (warp == 1) tmem_free_pair(tmem, 512);
+    if (a.beside) after_previous();
 }
 
 // ---- a piece of G from logits that the losses have kept, the same bits as the product would give. A thread takes 32 columns of a
 // scored row; the rows up to the next multiple of a tile are zeros, as every line of G that a product reads.
 template <typename T, typename S, int PARTS>
 __global__ void __launch_bounds__(256) k_head_grad_kept(const ProductArgs a) {
+    let_next();
+    after_previous();
     const uint32_t n = a.meta->n, kept = a.meta->kept;
     if (kept == 0 || n == 0) return;
     const uint32_t per = ((a.columns + 63) & ~63u) / 32;
@@ -692,7 +726,15 @@ __global__ void __launch_bounds__(256) k_head_grad_kept(const ProductArgs a) {
         }
         const ExpFrom<sizeof(T) == 4> ex(row.m);
         logits_to_g(g, ex, row.s, row.factor, in ? row.target - a.first - c0 : 0xffffffffu, a.columns - min(a.columns, c0), in);
-        store_g<S, PARTS>(g, static_cast<S*>(a.g) + (uint64_t)slot * a.g_pitch + c0, a.g_part);
+        S* out = static_cast<S*>(a.g) + (uint64_t)slot * a.g_pitch + c0;
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) w[j] = next_part<S>(g[2 * j], g[2 * j + 1], p + 1 < PARTS);
+            store32(out + p * a.g_part, w);
+            store32(out + p * a.g_part + 16, w + 8);
+        }
     }
 }
 
@@ -702,6 +744,8 @@ __global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t h
                                                        const int32_t* __restrict__ slot_of, const float* __restrict__ dx,
                                                        const float* __restrict__ dx_shares, const HeadMeta* __restrict__ meta, float scale, T* out,
                                                        uint64_t stride) {
+    let_next();
+    after_previous();
     scale *= meta->down;
     const Split split(meta->n, hidden, piece, pairs);
     const uint32_t per = (hidden + N - 1) / N, nt = tiles_of(hidden, MMA_N);
@@ -717,9 +761,10 @@ __global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t h
             const uint32_t tile = slot / MMA_M * nt + col / MMA_N;
             const float* from = dx_shares + ((uint64_t)tile - split.whole) * (MMA_M * MMA_N) + slot % MMA_M * MMA_N + col % MMA_N;
             if (tile >= split.whole)
-                for (uint32_t k = 1; k < split.shares; k++, from += (uint64_t)split.rest * (MMA_M * MMA_N)) {
+#pragma unroll 4
+                for (uint32_t k = 1; k < split.shares; k++) {
                     Vec<float, N> v;
-                    v.load(from);
+                    v.load(from + (uint64_t)(k - 1) * split.rest * (MMA_M * MMA_N));
 #pragma unroll
                     for (int j = 0; j < N; j++) sum.e[j] += v.e[j];
                 }
@@ -747,15 +792,17 @@ int32_t encoder(Encode* out) {
     return OXZ_OK;
 }
 
-// [parts][lines][pitch] 16-bit values as boxes of 64 x 64, 128-byte swizzle; what lies outside reads as zeros
-int32_t tensor_map(CUtensorMap* m, bool bf16, const void* base, uint64_t pitch, uint64_t lines, uint64_t parts, uint64_t part_stride) {
+// [parts][lines][pitch] values as boxes of 128 bytes by `box_lines`, 128-byte swizzle; what lies outside reads as zeros and is not written
+int32_t tensor_map(CUtensorMap* m, int32_t dtype, const void* base, uint64_t pitch, uint64_t lines, uint64_t parts, uint64_t part_stride,
+                   uint32_t box_lines = 64) {
     Encode encode = nullptr;
     OXZ_TRY(encoder(&encode));
-    const cuuint64_t dims[3] = {pitch, lines, parts}, strides[2] = {pitch * 2, part_stride * 2};
-    const cuuint32_t box[3] = {64, 64, 1}, step[3] = {1, 1, 1};
-    const CUresult r = encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
-                              strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const uint32_t es = (uint32_t)dtype_size(dtype);
+    const cuuint64_t dims[3] = {pitch, lines, parts}, strides[2] = {pitch * es, part_stride * es};
+    const cuuint32_t box[3] = {128 / es, box_lines, 1}, step[3] = {1, 1, 1};
+    const CUtensorMapDataType t = dtype == OXZ_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == OXZ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult r = encode(m, t, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(OXZ_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)r);
     return OXZ_OK;
 }
@@ -763,11 +810,13 @@ int32_t tensor_map(CUtensorMap* m, bool bf16, const void* base, uint64_t pitch, 
 template <typename T, typename S, typename G, int PARTS>
 struct Products {
     template <int P>
-    static void launch(const oxz_head* h, const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, uint64_t m, uint64_t n, cudaStream_t s) {
+    static int32_t launch(const oxz_head* h, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& out, const CUtensorMap& shares,
+                          const ProductArgs& a, uint64_t m, uint64_t n, cudaStream_t s) {
         const uint64_t tiles = (uint64_t)tiles_of(m, MMA_M) * tiles_of(n, MMA_N);
         // the cut of D_HIDDEN goes by the number of pairs: always all of them
         const unsigned pairs = P == D_HIDDEN ? (unsigned)h->clusters : (unsigned)std::min<uint64_t>(tiles, h->clusters);
-        if (tiles) k_head_product<T, S, G, P, PARTS><<<2 * pairs, MMA_THREADS, MMA_SMEM, s>>>(ma, mb, a);
+        if (tiles) OXZ_CUDA(launch_after(true, k_head_product<T, S, G, P, PARTS>, 2 * pairs, MMA_THREADS, MMA_SMEM, s, ma, mb, out, shares, a));
+        return OXZ_OK;
     }
     template <int P>
     static int32_t prepare(int* clusters) {
@@ -807,16 +856,17 @@ struct Products {
         const bool x_wide = !misaligned(b.hidden, 16) && b.hidden_stride * es % 16 == 0;
         if (b.rows) {
             const uint64_t work = (b.rows + MMA_M) * (h->pitch / 8);
-            k_head_pack<T, S><<<(unsigned)std::min<uint64_t>((work + 255) / 256, many), 256, 0, s>>>(
-                static_cast<const T*>(b.hidden), b.hidden_stride, (uint32_t)d.hidden, h->pitch, b.rows, h->row_of, h->meta,
-                static_cast<S*>(h->x), x_part, h->parts, x_wide);
+            OXZ_CUDA(launch_after(true, k_head_pack<T, S>, (unsigned)std::min<uint64_t>((work + 255) / 256, many), 256, 0, s,
+                                  static_cast<const T*>(b.hidden), b.hidden_stride, (uint32_t)d.hidden, h->pitch, b.rows, h->row_of, h->meta,
+                                  static_cast<S*>(h->x), x_part, h->parts, x_wide));
         }
         if (h->w)
-            k_head_pack<T, S><<<many, 256, 0, s>>>(static_cast<const T*>(b.weight), d.hidden, (uint32_t)d.hidden, h->pitch, d.vocab, nullptr,
-                                                   h->meta, static_cast<S*>(h->w), w_part, h->parts, d.hidden * es % 16 == 0);
+            OXZ_CUDA(launch_after(true, k_head_pack<T, S>, many, 256, 0, s, static_cast<const T*>(b.weight), d.hidden, (uint32_t)d.hidden, h->pitch, d.vocab,
+                                  nullptr, h->meta, static_cast<S*>(h->w), w_part, h->parts, d.hidden * es % 16 == 0));
+        constexpr int32_t ST = BF16 ? OXZ_BF16 : OXZ_F16;
         CUtensorMap mx, mw, mg;
-        OXZ_TRY(tensor_map(&mx, BF16, h->x, h->pitch, h->cap, h->parts, x_part));
-        OXZ_TRY(tensor_map(&mw, BF16, h->w ? h->w : b.weight, h->pitch, d.vocab, h->parts, w_part));
+        OXZ_TRY(tensor_map(&mx, ST, h->x, h->pitch, h->cap, h->parts, x_part));
+        OXZ_TRY(tensor_map(&mw, ST, h->w ? h->w : b.weight, h->pitch, d.vocab, h->parts, w_part));
 
         ProductArgs a{};
         a.meta = h->meta;
@@ -849,10 +899,12 @@ struct Products {
         pairs(1);
         if (want_loss) {
             a.columns = (uint32_t)d.vocab;
-            launch<LOGITS_STATS>(h, mx, mw, a, b.rows, d.vocab, s);
+            CUtensorMap ml = mx;  // not used where nothing is kept
+            if (a.keep && h->l_elems) OXZ_TRY(tensor_map(&ml, OXZ_F32, h->l, h->kept_pitch, h->l_elems / h->kept_pitch, 1, h->l_elems / h->kept_pitch * h->kept_pitch, 32));
+            OXZ_TRY(launch<LOGITS_STATS>(h, mx, mw, ml, ml, a, b.rows, d.vocab, s));
             const unsigned blocks = std::max<unsigned>(1, (unsigned)((b.rows + FINISH_ROWS - 1) / FINISH_ROWS));
-            k_head_finish<<<blocks, 1024, 0, s>>>((uint32_t)b.rows, a.pitch, 2 * (uint32_t)((d.vocab + MMA_N - 1) / MMA_N), h->slot_of,
-                                                              h->part, h->target_logit, b.loss_mask, stats, row_loss, h->loss_part, h->meta, totals);
+            OXZ_CUDA(launch_after(true, k_head_finish, blocks, 1024, 0, s, (uint32_t)b.rows, a.pitch, 2 * tiles_of(d.vocab, MMA_N), h->slot_of, h->part,
+                                  h->target_logit, b.loss_mask, stats, row_loss, h->loss_part, h->meta, totals));
         }
         if (!gr) return OXZ_OK;
         a.stats = stats;
@@ -861,7 +913,15 @@ struct Products {
         a.dw = gr->d_weight;
         a.g_pitch = (uint32_t)h->piece;
         a.g_part = h->cap * h->piece;
-        OXZ_TRY(tensor_map(&mg, BF16, h->g, h->piece, h->cap, h->g_parts, a.g_part));
+        OXZ_TRY(tensor_map(&mg, ST, h->g, h->piece, h->cap, h->g_parts, a.g_part));
+        CUtensorMap mgo, mdx, mds, mdw = mg;
+        OXZ_TRY(tensor_map(&mgo, ST, h->g, h->piece, h->cap, h->g_parts, a.g_part, 32));
+        OXZ_TRY(tensor_map(&mdx, OXZ_F32, h->dx, h->dx_pitch, h->cap, 1, h->cap * h->dx_pitch, 32));
+        const uint64_t share_lines = (uint64_t)MAX_ROUNDS * h->clusters * MMA_M;
+        OXZ_TRY(tensor_map(&mds, OXZ_F32, h->dx_shares, MMA_N, share_lines, 1, share_lines * MMA_N, 32));
+        // d_weight leaves by TMA where its rows are whole 16-byte pieces; 16-bit sums with what was there are made by the threads
+        a.boxes = gr->d_weight && d.hidden * sizeof(G) % 16 == 0 && (sizeof(G) == 4 || !gr->accumulate);
+        if (a.boxes) OXZ_TRY(tensor_map(&mdw, d.grad_dtype, gr->d_weight, d.hidden, d.vocab, 1, d.vocab * d.hidden, 32));
         const bool sure = b.rows * h->kept_pitch <= h->l_elems;  // kept whatever the mask
         for (uint64_t v = 0; v < d.vocab; v += h->piece) {
             a.first = (uint32_t)v;
@@ -869,19 +929,21 @@ struct Products {
             a.add = v > 0;
             pairs(1);
             // the scored rows' count decides on the device which of the two has work
-            if (a.keep && b.rows && h->l_elems) k_head_grad_kept<T, S, PARTS><<<many, 256, 0, s>>>(a);
-            if (!a.keep || !sure) launch<LOGITS_GRAD>(h, mx, mw, a, b.rows, a.columns, s);
-            if (gr->d_hidden) launch<D_HIDDEN>(h, mg, mw, a, b.rows, d.hidden, s);
+            if (a.keep && b.rows && h->l_elems) OXZ_CUDA(launch_after(true, k_head_grad_kept<T, S, PARTS>, many, 256, 0, s, a));
+            if (!a.keep || !sure) OXZ_TRY(launch<LOGITS_GRAD>(h, mx, mw, mgo, mgo, a, b.rows, a.columns, s));
+            if (gr->d_hidden) OXZ_TRY(launch<D_HIDDEN>(h, mg, mw, mdx, mds, a, b.rows, d.hidden, s));
             pairs(h->g_parts);
-            if (gr->d_weight) launch<D_WEIGHT>(h, mg, mx, a, a.columns, d.hidden, s);
+            a.beside = gr->d_hidden && b.rows;
+            if (gr->d_weight) OXZ_TRY(launch<D_WEIGHT>(h, mg, mx, mdw, mdw, a, a.columns, d.hidden, s));
+            a.beside = 0;
         }
         if (gr->d_hidden && b.rows) {
             constexpr int N = 16 / (int)sizeof(T);
             const bool wide = !misaligned(gr->d_hidden, 16) && gr->d_hidden_stride * es % 16 == 0 && d.hidden % N == 0;
             auto k = wide ? k_head_d_hidden<T, N> : k_head_d_hidden<T, 1>;
-            k<<<(unsigned)std::min<uint64_t>((b.rows * d.hidden / (wide ? N : 1) + 255) / 256, many), 256, 0, s>>>(
-                (uint32_t)b.rows, (uint32_t)d.hidden, h->dx_pitch, h->piece, (uint32_t)h->clusters, h->slot_of, h->dx, h->dx_shares, h->meta, a.scale,
-                static_cast<T*>(gr->d_hidden), gr->d_hidden_stride);
+            OXZ_CUDA(launch_after(true, k, (unsigned)std::min<uint64_t>((b.rows * d.hidden / (wide ? N : 1) + 255) / 256, many), 256, 0, s, (uint32_t)b.rows,
+                                  (uint32_t)d.hidden, h->dx_pitch, h->piece, (uint32_t)h->clusters, h->slot_of, h->dx, h->dx_shares, h->meta, a.scale,
+                                  static_cast<T*>(gr->d_hidden), gr->d_hidden_stride));
         }
         return OXZ_OK;
     }
@@ -982,7 +1044,7 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             h->g_parts = d.grad_dtype == OXZ_F32 ? 3 : 1;
             OXZ_TRY(with_types(d, [&](auto p) { return decltype(p)::prepare_all(h); }));
             // a third of the limit for a piece's G, the rest for logits that are kept, where there are so many
-            const uint64_t budget = d.piece_bytes ? d.piece_bytes : 1536ull << 20, limit = budget / 3;
+            const uint64_t budget = d.piece_bytes ? d.piece_bytes : 2048ull << 20, limit = budget / 3;
             const uint64_t all = (d.vocab + MMA_N - 1) / MMA_N * MMA_N;
             h->piece = std::min(all, std::max<uint64_t>(MMA_N, limit / (h->cap * 2 * h->g_parts) / MMA_N * MMA_N));
             uint64_t bytes = 0;
@@ -1005,6 +1067,7 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             // kept logits are written and read once (10 bytes of traffic an element with G's 2: 1.6 ps measured); forming them again
             // takes 2 x hidden operations on the tensor cores, six times that for f32 (0.85 ps at hidden 384, 2.9 at 2048, 16 bits)
             h->l_elems = d.hidden * (d.dtype == OXZ_F32 ? 6 : 1) >= 1024 ? std::min(budget / 3 * 2 / 4, h->cap * all) : 0;
+            if (h->l_elems < all) h->l_elems = 0;  // not a single row
             if (h->l_elems) OXZ_TRY(get(&h->l, h->l_elems * 4));
             OXZ_TRY(get(&h->dx, h->cap * h->dx_pitch * 4));
             // rest x shares is at most MAX_ROUNDS x pairs

@@ -68,6 +68,23 @@ struct DeviceGuard {
     }
 };
 
+// Launches `kernel` so that it may start before the kernel in front of it in the stream has ended (it waits for that one itself,
+// after_previous()). The first kernel of a call is launched with `overlap` false: what the caller ran before knows nothing of it.
+template <typename... P, typename... A>
+cudaError_t launch_after(bool overlap, void (*kernel)(P...), dim3 grid, dim3 block, size_t shared, cudaStream_t s, A&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = overlap ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Orders the calls of a handle whose workspace they share: a call waits for the one before it, whatever stream that used. A
 // call that is being captured into a graph is left out: an event of the running stream cannot be waited for in a capture, and a
 // replay's place is the replaying program's business.

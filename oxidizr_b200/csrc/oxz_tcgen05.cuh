@@ -60,6 +60,24 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const void* map, int
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
+// A box from this block's shared memory into a tensor map's memory, or added to it in f32; what lies outside is left out. `from` has been
+// written by this thread's warp (store_fence, then a warp barrier). One thread of the warp; store_read waits until the shared memory of
+// the stores before may be written again, store_done until they are in memory.
+__device__ __forceinline__ void tma_store(const void* map, int32_t x, int32_t y, int32_t z, uint32_t from) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n\tcp.async.bulk.commit_group;"
+                 ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(from) : "memory");
+}
+__device__ __forceinline__ void tma_add(const void* map, int32_t x, int32_t y, int32_t z, uint32_t from) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n\tcp.async.bulk.commit_group;"
+                 ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(from) : "memory");
+}
+__device__ __forceinline__ void store_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void st_shared16(uint32_t to, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 __device__ __forceinline__ void tma_prefetch_map(const void* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
