@@ -14,6 +14,7 @@
 #include <cuda.h>
 
 #include "oxz_elem.cuh"
+#include "oxz_head_few.cuh"
 #include "oxz_internal.h"
 #include "oxz_tcgen05.cuh"
 
@@ -54,6 +55,11 @@ struct oxz_head {
     uint64_t l_elems = 0, kept_pitch = 0;
     float* dx = nullptr;             // [scored rows][dx_pitch] sums over the pieces
     float* dx_shares = nullptr;      // tiles of 256 x 256: the shares after the first of the tiles that are cut
+    int sms = 0;
+    float* few_logits = nullptr;     // [vocab][FEW_ROWS] and less: the path for a handful of rows
+    float2* few_part = nullptr;
+    float* few_dx = nullptr;
+    uint32_t* few_done = nullptr;
     int32_t* expired = nullptr;      // mapped host memory: a bounded wait inside a kernel ran out
     int32_t* d_expired = nullptr;
     oxz::StreamOrder order;
@@ -133,13 +139,6 @@ __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ 
     }
 }
 
-// {max, sum of exp(x - max)} of two sets together. An empty set is {-inf, 0}.
-__device__ __forceinline__ float2 join(float2 a, float2 b) {
-    const float m = fmaxf(a.x, b.x);
-    if (m == -INFINITY) return make_float2(m, a.y + b.y);
-    return make_float2(m, a.y * expf(a.x - m) + b.y * expf(b.x - m));
-}
-
 // ---- the rows' statistics from their tiles', their losses, and the totals (by the block that ends last, in block order). A block
 // takes 32 rows, a lane each; its warps take every 32nd tile and are joined in order.
 __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pitch, uint32_t tiles, const int32_t* __restrict__ slot_of,
@@ -160,7 +159,7 @@ __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pi
 #pragma unroll
             for (int k = 0; k < 4; k++) p[k] = t + 32 * k < tiles ? part[(uint64_t)(t + 32 * k) * pitch + slot] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-            for (int k = 0; k < 4; k++) s = join(s, p[k]);
+            for (int k = 0; k < 4; k++) s = join_stats(s, p[k]);
         }
     }
     share[warp][lane] = s;
@@ -168,7 +167,7 @@ __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pi
     // now a warp has one row, a lane one of its parts
     s = share[lane][warp];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) s = join(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
+    for (int o = 1; o < 32; o <<= 1) s = join_stats(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
     const uint32_t own = blockIdx.x * FINISH_ROWS + warp;
     if (lane == 0) {
         mine[warp] = 0.0;
@@ -841,12 +840,50 @@ struct Products {
         OXZ_TRY(prepare<LOGITS_STATS>(&h->clusters));
         OXZ_TRY(prepare<LOGITS_GRAD>(&h->clusters));
         OXZ_TRY(prepare<D_HIDDEN>(&h->clusters));
-        return prepare<D_WEIGHT>(&h->clusters);
+        OXZ_TRY(prepare<D_WEIGHT>(&h->clusters));
+        return few_prepare<T, G>();
+    }
+
+    // A handful of rows: see oxz_head_few.cuh
+    static int32_t run_few(oxz_head* h, const oxz_head_batch& b, bool wide, float* row_loss, float2* row_stats, bool want_loss, float* totals,
+                           const oxz_head_grads* gr, cudaStream_t s) {
+        const oxz_head_desc& d = h->d;
+        FewArgs a{};
+        a.x = b.hidden;
+        a.x_stride = b.hidden_stride;
+        a.w = b.weight;
+        a.targets = b.targets;
+        a.mask = b.loss_mask;
+        a.rows = (uint32_t)b.rows;
+        a.hidden = (uint32_t)d.hidden;
+        a.vocab = (uint32_t)d.vocab;
+        a.logits = h->few_logits;
+        a.part = h->few_part;
+        a.done = h->few_done;
+        a.stats = row_stats ? row_stats : h->stats;
+        a.row_loss = row_loss;
+        a.totals = totals;
+        a.finish = want_loss;
+        bool out_wide = true;
+        if (gr) {
+            a.dw = gr->d_weight;
+            a.dx = gr->d_hidden;
+            a.dx_stride = gr->d_hidden_stride;
+            a.dx_part = h->few_dx;
+            a.scale = (float)gr->grad_scale;
+            a.accumulate = gr->accumulate && gr->d_weight;
+            a.want_dx = gr->d_hidden != nullptr;
+            out_wide = d.hidden % 4 == 0;  // weight and d_weight begin on 16 bytes; x is read by elements
+        }
+        return few_run<T, G>(a, wide, out_wide, gr != nullptr, h->sms, s);
     }
 
     static int32_t run(oxz_head* h, const oxz_head_batch& b, float* row_loss, float2* row_stats, bool want_loss, float* totals,
                        const oxz_head_grads* gr, cudaStream_t s) {
         const oxz_head_desc& d = h->d;
+        const bool on16 = !misaligned(b.hidden, 16) && b.hidden_stride * sizeof(T) % 16 == 0 && d.hidden * sizeof(T) % 16 == 0;
+        if (b.rows <= (uint64_t)FEW_ROWS && ((sizeof(T) == 2 && on16) || (uint64_t)FEW_ROWS * (d.hidden + 255) * 4 <= FEW_X_BYTES))
+            return run_few(h, b, on16, row_loss, row_stats, want_loss, totals, gr, s);
         constexpr bool F32 = sizeof(T) == 4, BF16 = std::is_same<S, __nv_bfloat16>::value;
         const size_t es = sizeof(T);
         const unsigned many = (unsigned)h->clusters * 2 * 8;  // blocks of the elementwise kernels
@@ -1043,6 +1080,7 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             h->parts = d.dtype == OXZ_F32 ? 3 : 1;
             h->g_parts = d.grad_dtype == OXZ_F32 ? 3 : 1;
             OXZ_TRY(with_types(d, [&](auto p) { return decltype(p)::prepare_all(h); }));
+            OXZ_CUDA(cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, d.device));
             // a third of the limit for a piece's G, the rest for logits that are kept, where there are so many
             const uint64_t budget = d.piece_bytes ? d.piece_bytes : 2048ull << 20, limit = budget / 3;
             const uint64_t all = (d.vocab + MMA_N - 1) / MMA_N * MMA_N;
@@ -1072,6 +1110,12 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             OXZ_TRY(get(&h->dx, h->cap * h->dx_pitch * 4));
             // rest x shares is at most MAX_ROUNDS x pairs
             OXZ_TRY(get(&h->dx_shares, (uint64_t)MAX_ROUNDS * h->clusters * MMA_M * MMA_N * 4));
+            OXZ_TRY(get(&h->few_logits, d.vocab * FEW_ROWS * 4));
+            OXZ_TRY(get(&h->few_part, (uint64_t)h->sms * FEW_LOGIT_BLOCKS * FEW_ROWS * 8));
+            OXZ_TRY(get(&h->few_dx, (uint64_t)std::max(few_parts(d.hidden, d.vocab, h->sms, 1), few_parts_16(d.hidden, d.vocab, h->sms)) * FEW_ROWS * d.hidden * 4));
+            OXZ_TRY(get(&h->few_done, 4));
+            OXZ_CUDA(cudaMemset(h->few_done, 0, 4));
+            OXZ_CUDA(cudaDeviceSynchronize());
             if (!h->expired) {
                 OXZ_CUDA(cudaHostAlloc((void**)&h->expired, 4, cudaHostAllocMapped));
                 *h->expired = 0;
@@ -1093,7 +1137,8 @@ int32_t oxz_head_destroy(oxz_head* h) {
         if (h->row_of) dev.enter(h->d.device);
         h->order.destroy();
         for (void* p : {(void*)h->row_of, (void*)h->slot_of, (void*)h->part, (void*)h->target_logit, (void*)h->stats, (void*)h->loss_part,
-                        (void*)h->meta, h->x, h->w, h->g, (void*)h->l, (void*)h->dx, (void*)h->dx_shares})
+                        (void*)h->meta, h->x, h->w, h->g, (void*)h->l, (void*)h->dx, (void*)h->dx_shares, (void*)h->few_logits,
+                        (void*)h->few_part, (void*)h->few_dx, (void*)h->few_done})
             if (p) cudaFree(p);
         if (h->expired) cudaFreeHost(h->expired);
         delete h;
