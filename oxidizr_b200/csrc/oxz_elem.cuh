@@ -88,40 +88,4 @@ template <typename S> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// `count` of 32 consecutive f32 times `scale`, rounded to G at `out`, or added to what is there. Whole spans on 32 bytes go by sectors.
-template <typename G>
-__device__ __forceinline__ void write_span(G* out, const uint32_t (&x)[32], uint32_t count, float scale, bool accumulate) {
-    if (count == 32 && (reinterpret_cast<uintptr_t>(out) & 31) == 0) {
-        constexpr int PER = 32 / (int)sizeof(G);  // elements of a sector
-#pragma unroll
-        for (int q = 0; q < 32 / PER; q++) {
-            uint32_t old[8], w[8];
-            if (accumulate) load32(out + q * PER, old);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if constexpr (sizeof(G) == 4) {
-                    const float v = __uint_as_float(x[q * 8 + j]) * scale;
-                    w[j] = __float_as_uint(accumulate ? __uint_as_float(old[j]) + v : v);
-                } else {
-                    float lo = __uint_as_float(x[q * 16 + 2 * j]) * scale, hi = __uint_as_float(x[q * 16 + 2 * j + 1]) * scale;
-                    if (accumulate) {
-                        const float2 o = unpack2<G>(old[j]);
-                        lo += o.x;
-                        hi += o.y;
-                    }
-                    w[j] = pack2<G>(lo, hi);
-                }
-            }
-            store32(out + q * PER, w);
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 32; j++)
-        if ((uint32_t)j < count) {
-            const float v = __uint_as_float(x[j]) * scale;
-            out[j] = from_f32<G>(accumulate ? to_f32<G>(out[j]) + v : v);
-        }
-}
-
 }  // namespace oxz

@@ -677,14 +677,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                     }
                     box(map_out, (int32_t)(c.n0 + c0), (int32_t)a.first + line, 0, w, sizeof(G) == 4 && a.accumulate);
                 }
-            } else if (in) {
+            } else {
+                // 16-bit sums with what was there, or rows that are not whole 16-byte pieces: 32 x 32 results are turned in shared memory, so
+                // that a warp writes 32 neighbours
+                const uint32_t rows = min(32u, M - min(M, (uint32_t)line));
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const uint32_t c0 = from + 32 * q;
                     if (c0 >= to) break;
-                    uint32_t w[32];
-                    words(q, w);
-                    write_span<G>(static_cast<G*>(a.dw) + (uint64_t)(a.first + i) * a.hidden + c.n0 + c0, w, min(32u, valid - c0), scale, a.accumulate != 0);
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const uint32_t at = out_at + lane * 128 + ((j ^ lane) << 2);
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(acc[q][j] * scale) : "memory");
+                    }
+                    __syncwarp();
+                    G* out = static_cast<G*>(a.dw) + (uint64_t)(a.first + line) * a.hidden + c.n0 + c0 + lane;
+                    const bool here = c0 + lane < valid;
+#pragma unroll 8
+                    for (uint32_t k = 0; k < rows; k++, out += a.hidden) {
+                        float v;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(out_at + k * 128 + ((lane ^ k) << 2)) : "memory");
+                        if (here) *out = from_f32<G>(a.accumulate ? to_f32<G>(*out) + v : v);
+                    }
                 }
             }
         }
@@ -882,7 +897,7 @@ struct Products {
                        const oxz_head_grads* gr, cudaStream_t s) {
         const oxz_head_desc& d = h->d;
         const bool on16 = !misaligned(b.hidden, 16) && b.hidden_stride * sizeof(T) % 16 == 0 && d.hidden * sizeof(T) % 16 == 0;
-        if (b.rows <= (uint64_t)FEW_ROWS && ((sizeof(T) == 2 && on16) || (uint64_t)FEW_ROWS * (d.hidden + 255) * 4 <= FEW_X_BYTES))
+        if (few_fits(b.rows, d.hidden, sizeof(T), on16))
             return run_few(h, b, on16, row_loss, row_stats, want_loss, totals, gr, s);
         constexpr bool F32 = sizeof(T) == 4, BF16 = std::is_same<S, __nv_bfloat16>::value;
         const size_t es = sizeof(T);

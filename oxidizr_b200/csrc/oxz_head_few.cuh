@@ -128,6 +128,15 @@ __device__ void few_finish(const FewArgs& a, float2 (&by_warp)[FEW_THREADS / 32]
     }
 }
 
+__device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 template <typename T>
 __device__ __forceinline__ void warp_product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (sizeof(T) == 2) {
@@ -140,53 +149,84 @@ __device__ __forceinline__ void warp_product(float (&c)[4], const uint32_t (&a)[
     }
 }
 
-// 16-bit logits, rows on 16 bytes. A warp takes 16 words. Lane (r, q) = (lane / 4, lane % 4) loads 16 bytes, elements 8q .. 8q + 7 of a
+// 16-bit logits, rows on 16 bytes. A warp takes 16 words. Lane (r, q) = (lane / 4, lane % 4) has 16 bytes, elements 8q .. 8q + 7 of a
 // stretch of 32, of words r and r + 8 and of rows r, r + 8 of x; as the order of a dot product's terms is free, elements 0..3 of every
-// lane make one warp product and 4..7 the next, which is how their fragments lie, with no exchange. Two products of a stretch stay in
-// an accumulator with the six of the next three, then they are added in f32 (the units cut what they add).
+// lane make one warp product and 4..7 the next, which is how their fragments lie, with no exchange. The weight's pieces come by
+// asynchronous copies into a ring of the thread's own, LOGIT_DEPTH steps of 128 elements ahead across the words' bounds; x lies in
+// shared memory. The products of a step are added in f32 (the units cut what they add).
+constexpr int LOGIT_DEPTH = 3, LOGIT_STEP = 128;
+inline uint32_t few_x_pitch(uint64_t hidden) { return (uint32_t)((hidden + 127) / 128 * 128 + 32); }  // 64 bytes off a multiple of 128: no bank twice
 template <typename T, int R>
-__global__ void __launch_bounds__(FEW_THREADS) k_few_logits_16(const FewArgs a) {
+__global__ void __launch_bounds__(FEW_THREADS) k_few_logits_16(const FewArgs a, uint32_t x_pitch) {
     static_assert(R == 8 || R == 16, "8 rows a product");
+    extern __shared__ __align__(16) unsigned char ring[];  // [LOGIT_DEPTH][8][threads] 16 bytes, then x [R][x_pitch]
     __shared__ float2 by_warp[FEW_THREADS / 32][R];
     let_next();
     after_previous();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
     const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.w);
-    bool on[R / 8];
+    T* xs = reinterpret_cast<T*>(ring + LOGIT_DEPTH * 8 * FEW_THREADS * 16);
+    const uint32_t tiles = (a.vocab + 15) / 16, steps = (a.hidden + LOGIT_STEP - 1) / LOGIT_STEP, stride = gridDim.x * (FEW_THREADS / 32);
+    const uint32_t first = blockIdx.x * (FEW_THREADS / 32) + warp;
+    uint32_t ft = first, fk = 0;  // what is fetched next: tile, step
+    auto fetch = [&](uint32_t slot) {
+        if (ft < tiles) {
+            const T *w0 = w + (uint64_t)min(ft * 16 + r, a.vocab - 1) * a.hidden, *w1 = w + (uint64_t)min(ft * 16 + r + 8, a.vocab - 1) * a.hidden;
+            const uint32_t to = smem_address(ring + (slot * 8 * FEW_THREADS + threadIdx.x) * 16), k = fk * LOGIT_STEP + 8 * q;
 #pragma unroll
-    for (int j = 0; j < R / 8; j++) on[j] = few_scored(a, r + 8 * j);
+            for (int e = 0; e < 4; e++)
+                if (k + 32 * e < a.hidden) {
+                    copy_async<16>(to + 2 * e * FEW_THREADS * 16, w0 + k + 32 * e);
+                    copy_async<16>(to + (2 * e + 1) * FEW_THREADS * 16, w1 + k + 32 * e);
+                }
+        }
+        copies_end();
+        if (++fk == steps) {
+            fk = 0;
+            ft += stride;
+        }
+    };
+#pragma unroll
+    for (int e = 0; e < LOGIT_DEPTH; e++) fetch(e);
+    for (uint32_t e = threadIdx.x; e < R * (x_pitch / 8); e += FEW_THREADS) {
+        const uint32_t i = e / (x_pitch / 8), k = (e - i * (x_pitch / 8)) * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (k < a.hidden && few_scored(a, i)) v = __ldg(reinterpret_cast<const uint4*>(x + (uint64_t)i * a.x_stride + k));
+        *reinterpret_cast<uint4*>(xs + i * x_pitch + k) = v;
+    }
+    __syncthreads();
     float2 s[R / 8][2];
 #pragma unroll
     for (int j = 0; j < R / 8; j++) s[j][0] = s[j][1] = make_float2(-INFINITY, 0.f);
-    const uint32_t tiles = (a.vocab + 15) / 16;
-    for (uint32_t t = blockIdx.x * (FEW_THREADS / 32) + warp; t < tiles; t += gridDim.x * (FEW_THREADS / 32)) {
+    uint32_t slot = 0;
+    for (uint32_t t = first; t < tiles; t += stride) {
         const uint32_t v0 = t * 16 + r, v1 = v0 + 8;
-        const T *w0 = w + (uint64_t)min(v0, a.vocab - 1) * a.hidden, *w1 = w + (uint64_t)min(v1, a.vocab - 1) * a.hidden;
         float acc[R / 8][4] = {};
-        for (uint32_t k0 = 0; k0 < a.hidden; k0 += 128) {
-            uint4 p[4], u[4], y[4][R / 8];
+        for (uint32_t k0 = 0; k0 < a.hidden; k0 += LOGIT_STEP) {
+            copies_but<LOGIT_DEPTH - 1>();
+            const unsigned char* from = ring + (slot * 8 * FEW_THREADS + threadIdx.x) * 16;
+            float c[R / 8][4] = {};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t k = k0 + 32 * e + 8 * q;
-                const bool in = k < a.hidden;
-                p[e] = in ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : make_uint4(0, 0, 0, 0);
-                u[e] = in ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < R / 8; j++)
-                    y[e][j] = in && on[j] ? __ldg(reinterpret_cast<const uint4*>(x + (uint64_t)(r + 8 * j) * a.x_stride + k)) : make_uint4(0, 0, 0, 0);
-            }
-            float c[R / 8][4] = {};
-#pragma unroll
-            for (int e = 0; e < 4; e++)
+                uint4 p = make_uint4(0, 0, 0, 0), u = p;
+                if (k < a.hidden) {
+                    p = *reinterpret_cast<const uint4*>(from + 2 * e * FEW_THREADS * 16);
+                    u = *reinterpret_cast<const uint4*>(from + (2 * e + 1) * FEW_THREADS * 16);
+                }
 #pragma unroll
                 for (int j = 0; j < R / 8; j++) {
-                    warp_product<T>(c[j], {p[e].x, u[e].x, p[e].y, u[e].y}, y[e][j].x, y[e][j].y);
-                    warp_product<T>(c[j], {p[e].z, u[e].z, p[e].w, u[e].w}, y[e][j].z, y[e][j].w);
+                    const uint4 y = *reinterpret_cast<const uint4*>(xs + (r + 8 * j) * x_pitch + k);
+                    warp_product<T>(c[j], {p.x, u.x, p.y, u.y}, y.x, y.y);
+                    warp_product<T>(c[j], {p.z, u.z, p.w, u.w}, y.z, y.w);
                 }
+            }
 #pragma unroll
             for (int j = 0; j < R / 8; j++)
 #pragma unroll
                 for (int m = 0; m < 4; m++) acc[j][m] += c[j][m];
+            fetch(slot);
+            slot = slot + 1 == LOGIT_DEPTH ? 0 : slot + 1;
         }
         // this lane: words v0, v1 of rows 8 j + 2 q, + 1
 #pragma unroll
@@ -195,11 +235,14 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits_16(const FewArgs a) 
             for (int h = 0; h < 2; h++) {
                 const uint32_t v = h ? v1 : v0;
                 if (v >= a.vocab) continue;
-                add_logit(s[j][0], acc[j][2 * h]);
-                add_logit(s[j][1], acc[j][2 * h + 1]);
+                if (a.finish) {
+                    add_logit(s[j][0], acc[j][2 * h]);
+                    add_logit(s[j][1], acc[j][2 * h + 1]);
+                }
                 *reinterpret_cast<float2*>(a.logits + (uint64_t)v * R + 8 * j + 2 * q) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
             }
     }
+    copies_but<0>();
     if (!a.finish) return;
 #pragma unroll
     for (int j = 0; j < R / 8; j++)
@@ -213,17 +256,38 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits_16(const FewArgs a) 
     few_finish<R>(a, by_warp);
 }
 
-// Any type and alignment: a warp takes WORDS words, lanes along hidden; the rows of x are in shared memory as f32. N elements a lane:
-// 16 bytes of the weight (WIDE) or one.
+// Any type and alignment: a warp takes WORDS words, lanes along hidden; the rows of x are in shared memory as f32. A lane has 16 bytes of
+// a word at a time, by asynchronous copies as above (WIDE), or one element.
 template <typename T, int R, bool WIDE>
 __global__ void __launch_bounds__(FEW_THREADS) k_few_logits(const FewArgs a) {
     constexpr int N = WIDE ? 16 / (int)sizeof(T) : 1, WORDS = 64 / R;
-    extern __shared__ __align__(16) float xs[];  // [R][pitch]
+    constexpr int DEPTH = R == 4 ? 2 : R == 8 ? 3 : 4;
+    extern __shared__ __align__(16) float xs[];  // [R][pitch], then (WIDE) the ring [DEPTH][WORDS][threads] 16 bytes
     __shared__ float2 by_warp[FEW_THREADS / 32][R];
     let_next();
     after_previous();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, pitch = (a.hidden + 32 * N - 1) / (32 * N) * (32 * N);
     const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.w);
+    const uint32_t tiles = (a.vocab + WORDS - 1) / WORDS, stride = gridDim.x * (FEW_THREADS / 32), first = blockIdx.x * (FEW_THREADS / 32) + warp;
+    unsigned char* ring = reinterpret_cast<unsigned char*>(xs + R * pitch) + threadIdx.x * 16;
+    uint32_t ft = first, fk = lane * N;  // what is fetched next: tile, element
+    auto fetch = [&](uint32_t slot) {
+        if (ft < tiles && fk < a.hidden) {
+#pragma unroll
+            for (int d = 0; d < WORDS; d++)
+                copy_async<16>(smem_address(ring + (slot * WORDS + d) * FEW_THREADS * 16), w + (uint64_t)min(ft * WORDS + d, a.vocab - 1) * a.hidden + fk);
+        }
+        copies_end();
+        fk += 32 * N;
+        if (fk >= pitch) {
+            fk = lane * N;
+            ft += stride;
+        }
+    };
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int e = 0; e < DEPTH; e++) fetch(e);
+    }
     for (uint32_t i = 0; i < R; i++) {
         const bool on = few_scored(a, i);
         for (uint32_t k = threadIdx.x; k < pitch; k += FEW_THREADS) xs[i * pitch + k] = on && k < a.hidden ? to_f32<T>(x[(uint64_t)i * a.x_stride + k]) : 0.f;
@@ -231,20 +295,24 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits(const FewArgs a) {
     __syncthreads();
     // after the exchange below a lane has the logits of 64 / 32 = 2 (word, row) pairs
     float2 s[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
-    const uint32_t tiles = (a.vocab + WORDS - 1) / WORDS;
-    for (uint32_t t = blockIdx.x * (FEW_THREADS / 32) + warp; t < tiles; t += gridDim.x * (FEW_THREADS / 32)) {
+    uint32_t slot = 0;
+    for (uint32_t t = first; t < tiles; t += stride) {
         float acc[64];  // [WORDS][R]
 #pragma unroll
         for (int e = 0; e < 64; e++) acc[e] = 0.f;
         for (uint32_t k = lane * N; k < pitch; k += 32 * N) {
             Vec<T, N> v[WORDS];
             const bool in = k < a.hidden;
+            if constexpr (WIDE) copies_but<DEPTH - 1>();
 #pragma unroll
-            for (int d = 0; d < WORDS; d++)
-                if (in) v[d].load(w + (uint64_t)min(t * WORDS + d, a.vocab - 1) * a.hidden + k);
-            if (!in) continue;
+            for (int d = 0; d < WORDS; d++) {
+                if (!in) continue;
+                if constexpr (WIDE) v[d].q[0] = *reinterpret_cast<const uint4*>(ring + (slot * WORDS + d) * FEW_THREADS * 16);
+                else v[d].load(w + (uint64_t)min(t * WORDS + d, a.vocab - 1) * a.hidden + k);
+            }
 #pragma unroll
             for (int i = 0; i < R; i++) {
+                if (!in) continue;
                 float y[N];
                 if constexpr (N >= 4) {
 #pragma unroll
@@ -256,6 +324,10 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits(const FewArgs a) {
                 for (int d = 0; d < WORDS; d++)
 #pragma unroll
                     for (int n = 0; n < N; n++) acc[d * R + i] = fmaf(to_f32<T>(v[d].e[n]), y[n], acc[d * R + i]);
+            }
+            if constexpr (WIDE) {
+                fetch(slot);
+                slot = slot + 1 == DEPTH ? 0 : slot + 1;
             }
         }
         // 64 sums over 32 lanes: halves are exchanged, so that every lane ends with two of them
@@ -272,11 +344,14 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits(const FewArgs a) {
         // lane bits 16, 8, 4, 2, 1 chose the halves: its pair begins at 2 * lane (bit order kept)
         const uint32_t e0 = 2 * lane, word = t * WORDS + e0 / R, row = e0 % R;
         if (word < a.vocab) {
-            add_logit(s[0], acc[0]);
-            add_logit(s[1], acc[1]);
+            if (a.finish) {
+                add_logit(s[0], acc[0]);
+                add_logit(s[1], acc[1]);
+            }
             *reinterpret_cast<float2*>(a.logits + (uint64_t)word * R + row) = make_float2(acc[0], acc[1]);
         }
     }
+    if constexpr (WIDE) copies_but<0>();
     if (!a.finish) return;
     // lanes with the same rows: those R / 2 apart
 #pragma unroll
@@ -315,15 +390,6 @@ __device__ __forceinline__ void store4(T* row, uint32_t col0, uint32_t at, uint3
             if (col0 + at + c * across < hidden) row[col0 + at + c * across] = from_f32<T>(v[c]);
     }
 }
-
-__device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
-}
-__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Gradients. A thread has four columns of every row: x_i in registers, dX_i summed in registers; `along` threads share the words of a
 // block where a row is shorter than the block (their sums are joined in order at the end).
@@ -482,10 +548,12 @@ __device__ __forceinline__ void load_matrices_turned(uint32_t (&r)[4], uint32_t 
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 template <typename T, typename G, int R>
-__global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, uint32_t across) {
+__global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, uint32_t across_log) {
     extern __shared__ __align__(128) unsigned char raw16[];
-    const uint32_t along = 4 / across, words = 16 * along;  // of a stretch
+    const uint32_t across = 1u << across_log, along = 4 >> across_log, words = 16 * along;  // of a stretch
     constexpr uint32_t PIECE = 8192;
+    constexpr int PARTS = R == 8 ? 1 : 2;  // 8 rows: both parts of G fill one product, the second as rows 8 .. 15
+    constexpr bool SCALED = __is_same(T, __nv_bfloat16);  // bf16 has f32's range: the scale goes into G
     const uint32_t l_bytes = words * R * 4;
     unsigned char* wp = raw16;                                                 // [GRAD_DEPTH][words][64 * across], 16-byte chunks turned by the word
     float* lp = reinterpret_cast<float*>(raw16 + GRAD_DEPTH * PIECE);          // [GRAD_DEPTH][words][R]
@@ -494,7 +562,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
     __shared__ uint32_t row_t[16];
     let_next();
     after_previous();
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3, mine = warp / across, group = warp % across;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3, mine = warp >> across_log, group = warp & (across - 1);
     const uint32_t col0 = blockIdx.y * 64 * across, col = col0 + group * 64;
     const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.w);
     if (threadIdx.x < 16) {
@@ -503,7 +571,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
         const float2 s = on ? a.stats[i] : make_float2(0.f, 1.f);
         row_m[i] = s.x;
         row_s[i] = s.y;
-        row_f[i] = on ? (a.mask ? a.mask[i] : 1.f) / s.y : 0.f;
+        row_f[i] = on ? (a.mask ? a.mask[i] : 1.f) / s.y * (SCALED ? a.scale : 1.f) : 0.f;
         row_t[i] = on ? (uint32_t)a.targets[i] : 0xffffffffu;
     }
     const uint32_t begin = blockIdx.x * a.words, end = min(a.vocab, begin + a.words), turns = (end - begin + words - 1) / words;
@@ -511,7 +579,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
         if (turn < turns) {
             const uint32_t st = turn % GRAD_DEPTH, v0 = begin + turn * words;
             for (uint32_t e = threadIdx.x; e < PIECE / 16; e += GRAD_THREADS) {  // 16-byte chunk of a word
-                const uint32_t d = e / (8 * across), c = e - d * 8 * across, at = col0 + 8 * c;
+                const uint32_t d = e >> (3 + across_log), c = e & (8 * across - 1), at = col0 + 8 * c;
                 const uint32_t to = smem_address(wp + st * PIECE + d * 128 * across + (c & ~7u) * 16 + (((c ^ d) & 7) << 4));
                 if (v0 + d < end && at < a.hidden) copy_async<16>(to, w + (uint64_t)(v0 + d) * a.hidden + at);
                 else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
@@ -542,7 +610,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
             T v[2];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const uint32_t i = 8 * k + 2 * q + e;
+                const uint32_t i = (R == 8 ? 0 : 8 * k) + 2 * q + e;
                 v[e] = h < a.hidden && row_t[i] != 0xffffffffu ? x[(uint64_t)i * a.x_stride + h] : from_f32<T>(0.f);
             }
             xb[j][k] = (uint32_t)*reinterpret_cast<uint16_t*>(&v[0]) | (uint32_t)*reinterpret_cast<uint16_t*>(&v[1]) << 16;
@@ -554,28 +622,29 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
 #pragma unroll
         for (int m = 0; m < 4; m++) dx[j][m] = 0.f;
     G* dw = static_cast<G*>(a.dw);
-    const float out_scale = a.scale * down;
+    const float out_scale = SCALED ? 1.f : a.scale * down, dx_scale = SCALED ? 1.f : a.scale * down;
     for (uint32_t turn = 0; turn < turns; turn++) {
         const uint32_t st = turn % GRAD_DEPTH, v0 = begin + turn * words;
         copies_but<GRAD_DEPTH - 2>();
         __syncthreads();  // this stretch is here for everyone, and everyone is done with the one before
         fetch(turn + GRAD_DEPTH - 1);
-        for (uint32_t e = threadIdx.x; e < words * 16; e += GRAD_THREADS) {
-            const uint32_t d = e / 16, i = e % 16, v = v0 + d;
+        for (uint32_t e = threadIdx.x; e < words * R; e += GRAD_THREADS) {
+            const uint32_t d = e / R, i = e % R, v = v0 + d;
             float y = 0.f;
             if (v < end && row_t[i] != 0xffffffffu) {
-                const float p = expf(lp[st * words * R + d * R + (i & (R - 1))] - row_m[i]);
+                const float p = expf(lp[st * words * R + e] - row_m[i]);
                 y = (v == row_t[i] ? p - row_s[i] : p) * row_f[i] * up;
             }
-            const T hi = from_f32<T>(y);
+            const T hi = from_f32<T>(y), lo = from_f32<T>(isfinite(y) ? y - to_f32<T>(hi) : 0.f);
             gp[d * 16 + i] = hi;
-            gp[(words + d) * 16 + i] = from_f32<T>(isfinite(y) ? y - to_f32<T>(hi) : 0.f);
+            if (R == 8) gp[d * 16 + 8 + i] = lo;
+            else gp[(words + d) * 16 + i] = lo;
         }
         __syncthreads();
         if (col >= a.hidden) continue;
-        uint32_t gt[2][4], gn[2][4];  // G^T and G of the warp's 16 words, both parts
+        uint32_t gt[PARTS][4], gn[PARTS][4];  // G^T and G of the warp's 16 words, both parts
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
+        for (int p = 0; p < PARTS; p++) {
             const T* from = gp + (p * words + mine * 16) * 16;
             load_matrices_turned(gt[p], smem_address(from + ((lane >> 4) * 8 + (lane & 7)) * 16 + ((lane >> 3) & 1) * 8));
             load_matrices(gn[p], smem_address(from + (((lane >> 3) & 1) * 8 + (lane & 7)) * 16 + (lane >> 4) * 8));
@@ -589,7 +658,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
                 const uint32_t c = j + (lane >> 4);
                 load_matrices_turned(b, smem_address(piece + d * 128 * across + group * 128 + (((c ^ d) & 7) << 4)));
 #pragma unroll
-                for (int p = 1; p >= 0; p--) {
+                for (int p = PARTS - 1; p >= 0; p--) {
                     warp_product<T>(dx[j], gt[p], b[0], b[1]);
                     warp_product<T>(dx[j + 1], gt[p], b[2], b[3]);
                 }
@@ -601,7 +670,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
             for (int j = 0; j < 8; j++) {
                 out[j][0] = out[j][1] = out[j][2] = out[j][3] = 0.f;
 #pragma unroll
-                for (int p = 1; p >= 0; p--) warp_product<T>(out[j], gn[p], xb[j][0], xb[j][1]);
+                for (int p = PARTS - 1; p >= 0; p--) warp_product<T>(out[j], gn[p], xb[j][0], xb[j][1]);
             }
             const uint32_t h = col + 16 * q;
 #pragma unroll
@@ -614,7 +683,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
                     if (h + 8 * e >= a.hidden) break;
                     float y[8];
 #pragma unroll
-                    for (int c = 0; c < 8; c++) y[c] = out[4 * e + c / 2][2 * k + (c & 1)] * out_scale;
+                    for (int c = 0; c < 8; c++) y[c] = SCALED ? out[4 * e + c / 2][2 * k + (c & 1)] : out[4 * e + c / 2][2 * k + (c & 1)] * out_scale;
                     Vec<G, 8> o;
                     if (a.accumulate) o.load_coherent(to + 8 * e);
 #pragma unroll
@@ -632,19 +701,22 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
 #pragma unroll
     for (int j = 0; j < 8; j++)
 #pragma unroll
-        for (int m = 0; m < 4; m++) sums[((mine * 16) + r + 8 * (m >> 1)) * 64 * across + group * 64 + 8 * j + 2 * q + (m & 1)] = dx[j][m] * down;
+        for (int m = 0; m < 4; m++) sums[((mine * 16) + r + 8 * (m >> 1)) * 64 * across + group * 64 + 8 * j + 2 * q + (m & 1)] = dx[j][m] * dx_scale;
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < R * 64 * across; e += GRAD_THREADS) {
         const uint32_t i = e / (64 * across), c = e - i * 64 * across;
         float t = 0.f;
-        for (uint32_t p = 0; p < along; p++) t += sums[(p * 16 + i) * 64 * across + c];
+        for (uint32_t p = 0; p < along; p++) {
+            t += sums[(p * 16 + i) * 64 * across + c];
+            if (R == 8) t += sums[(p * 16 + 8 + i) * 64 * across + c];
+        }
         if (col0 + c < a.hidden) to[(uint64_t)i * a.hidden + col0 + c] = t;
     }
 }
 
 // d_hidden: the blocks' sums in order, eight warps a part each, joined in order. A block has one row and 32 columns.
 template <typename T, int R>
-__global__ void __launch_bounds__(256) k_few_d_hidden(const FewArgs a, uint32_t parts) {
+__global__ void __launch_bounds__(256) k_few_d_hidden(const FewArgs a, uint32_t parts, float scale) {
     __shared__ float share[8][32];
     let_next();
     after_previous();
@@ -661,7 +733,7 @@ __global__ void __launch_bounds__(256) k_few_d_hidden(const FewArgs a, uint32_t 
     if (warp || col >= a.hidden) return;
 #pragma unroll
     for (int w = 1; w < 8; w++) t += share[w][lane];
-    static_cast<T*>(a.dx)[(uint64_t)i * a.dx_stride + col] = from_f32<T>(on ? t * a.scale : 0.f);
+    static_cast<T*>(a.dx)[(uint64_t)i * a.dx_stride + col] = from_f32<T>(on ? t * scale : 0.f);
 }
 
 // ---- the launches of one call
@@ -685,23 +757,31 @@ inline uint32_t few_parts_16(uint64_t hidden, uint64_t vocab, int sms) {
 }
 constexpr int FEW_LOGIT_BLOCKS = 4;  // blocks of k_few_logits* an SM
 constexpr int FEW_GRAD_BYTES = FEW_THREADS * 4 * FEW_ROWS * 4;  // k_few_grads: the ring of copies, or the joined sums
-constexpr size_t FEW_X_BYTES = 160 << 10;  // rows of x that k_few_logits keeps in shared memory at most
-
+constexpr size_t FEW_SHARED = 227 << 10;   // what a block can have
+// The rows a kernel is made for that serves `rows`.
+inline int few_kernel_rows(uint64_t rows, size_t size, bool wide) { return rows <= 4 && !(size == 2 && wide) ? 4 : rows <= 8 ? 8 : 16; }
+// Shared memory of the logits' kernel: the rows of x and the ring of copies.
+inline size_t few_logit_bytes(int r, uint64_t hidden, size_t size, bool wide) {
+    if (size == 2 && wide) return LOGIT_DEPTH * 8 * FEW_THREADS * 16 + (size_t)r * few_x_pitch(hidden) * 2;
+    const uint64_t n = wide ? 16 / size : 1, pitch = (hidden + 32 * n - 1) / (32 * n) * (32 * n);
+    return (size_t)r * pitch * 4 + (wide ? (size_t)(r == 4 ? 2 : r == 8 ? 3 : 4) * (64 / r) * FEW_THREADS * 16 : 0);
+}
+inline bool few_fits(uint64_t rows, uint64_t hidden, size_t size, bool wide) {
+    return rows <= (uint64_t)FEW_ROWS && few_logit_bytes(few_kernel_rows(rows, size, wide), hidden, size, wide) + 8192 <= FEW_SHARED;
+}
 template <typename T, int R>
 int32_t few_logits(const FewArgs& a, bool wide, int sms, cudaStream_t s) {
+    const size_t shared = few_logit_bytes(R, a.hidden, sizeof(T), wide);
+    const uint32_t fit = std::max<uint32_t>(1, std::min<uint32_t>(FEW_LOGIT_BLOCKS, (uint32_t)((220 << 10) / shared)));
+    auto blocks = [&](uint32_t words) { return std::min<uint32_t>(((a.vocab + words - 1) / words + 7) / 8, sms * fit); };
     if constexpr (sizeof(T) == 2 && R >= 8) {
         if (wide) {
-            const uint32_t tiles = (a.vocab + 15) / 16, blocks = std::min<uint32_t>((tiles + 7) / 8, sms * FEW_LOGIT_BLOCKS);
-            OXZ_CUDA(launch_after(false, k_few_logits_16<T, R>, blocks, FEW_THREADS, 0, s, a));
+            OXZ_CUDA(launch_after(false, k_few_logits_16<T, R>, blocks(16), FEW_THREADS, shared, s, a, few_x_pitch(a.hidden)));
             return OXZ_OK;
         }
     }
-    const uint32_t n = wide ? 16 / (uint32_t)sizeof(T) : 1, pitch = (a.hidden + 32 * n - 1) / (32 * n) * (32 * n), words = 64 / R;
-    const size_t shared = (size_t)R * pitch * 4;
-    const uint32_t tiles = (a.vocab + words - 1) / words, fit = std::max<uint32_t>(1, std::min<uint32_t>(FEW_LOGIT_BLOCKS, (uint32_t)((200 << 10) / shared)));
-    const uint32_t blocks = std::min<uint32_t>((tiles + 7) / 8, sms * fit);
     auto k = wide ? k_few_logits<T, R, true> : k_few_logits<T, R, false>;
-    OXZ_CUDA(launch_after(false, k, blocks, FEW_THREADS, shared, s, a));
+    OXZ_CUDA(launch_after(false, k, blocks(64 / R), FEW_THREADS, shared, s, a));
     return OXZ_OK;
 }
 
@@ -711,7 +791,7 @@ int32_t few_run_rows(FewArgs a, bool wide, bool out_wide, bool grads, int sms, c
     OXZ_TRY((few_logits<T, R>(a, wide, sms, s)));
     if (!grads) return OXZ_OK;
     uint32_t parts = 0;
-    bool done = false;
+    bool scaled = false;  // the partial sums carry the scale already
     if constexpr (sizeof(T) == 2 && R >= 8) {
         if (wide) {
             const uint32_t across = few_across_16(a.hidden), columns = (a.hidden + 64 * across - 1) / (64 * across), words = 64 / across;
@@ -719,11 +799,11 @@ int32_t few_run_rows(FewArgs a, bool wide, bool out_wide, bool grads, int sms, c
             a.words = ((a.vocab + parts - 1) / parts + words - 1) / words * words;
             parts = (a.vocab + a.words - 1) / a.words;
             const size_t shared = (size_t)GRAD_DEPTH * (8192 + words * R * 4) + 2 * words * 16 * 2;
-            OXZ_CUDA(launch_after(true, k_few_grads_16<T, G, R>, dim3(parts, columns), GRAD_THREADS, shared, s, a, across));
-            done = true;
+            OXZ_CUDA(launch_after(true, k_few_grads_16<T, G, R>, dim3(parts, columns), GRAD_THREADS, shared, s, a, across == 4 ? 2u : across == 2 ? 1u : 0u));
+            scaled = true;
         }
     }
-    if (!done) {
+    if (!scaled) {
         const uint32_t across = few_across(a.hidden), columns = (a.hidden + 4 * across - 1) / (4 * across);
         parts = few_parts(a.hidden, a.vocab, sms, R);
         a.words = (a.vocab + parts - 1) / parts;
@@ -732,22 +812,24 @@ int32_t few_run_rows(FewArgs a, bool wide, bool out_wide, bool grads, int sms, c
         OXZ_CUDA(launch_after(true, k, dim3(parts, columns), FEW_THREADS, FEW_GRAD_BYTES, s, a, across));
     }
     if (a.want_dx && a.rows)
-        OXZ_CUDA(launch_after(true, k_few_d_hidden<T, R>, dim3((a.hidden + 31) / 32, a.rows), 256, 0, s, a, parts));
+        OXZ_CUDA(launch_after(true, k_few_d_hidden<T, R>, dim3((a.hidden + 31) / 32, a.rows), 256, 0, s, a, parts, scaled ? 1.f : a.scale));
     return OXZ_OK;
 }
 template <typename T, typename G>
 int32_t few_run(const FewArgs& a, bool wide, bool out_wide, bool grads, int sms, cudaStream_t s) {
-    if (a.rows <= 4 && !(sizeof(T) == 2 && wide)) return few_run_rows<T, G, 4>(a, wide, out_wide, grads, sms, s);
-    if (a.rows <= 8) return few_run_rows<T, G, 8>(a, wide, out_wide, grads, sms, s);
+    const int r = few_kernel_rows(a.rows, sizeof(T), wide);
+    if (r == 4) return few_run_rows<T, G, 4>(a, wide, out_wide, grads, sms, s);
+    if (r == 8) return few_run_rows<T, G, 8>(a, wide, out_wide, grads, sms, s);
     return few_run_rows<T, G, 16>(a, wide, out_wide, grads, sms, s);
 }
 // The shared memory that the kernels may need, granted once.
 template <typename T, typename G, int R>
 int32_t few_prepare_rows() {
-    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_X_BYTES));
-    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_X_BYTES));
+    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 2048));
+    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 2048));
     OXZ_CUDA(cudaFuncSetAttribute(k_few_grads<T, G, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_GRAD_BYTES));
     OXZ_CUDA(cudaFuncSetAttribute(k_few_grads<T, G, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_GRAD_BYTES));
+    if constexpr (sizeof(T) == 2 && R >= 8) OXZ_CUDA(cudaFuncSetAttribute(k_few_logits_16<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 2048));
     if constexpr (sizeof(T) == 2 && R >= 8) OXZ_CUDA(cudaFuncSetAttribute(k_few_grads_16<T, G, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 << 10));
     return OXZ_OK;
 }
