@@ -30,6 +30,8 @@ namespace {
 constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_CLUSTER = 8;
 constexpr int DIGIT_BITS = 9, BINS = 1 << DIGIT_BITS;
 constexpr uint32_t CHUNK = 16;  // sorted tokens a warp sums on its own
+constexpr uint32_t DIRECT = 1024;  // tokens that are summed without being sorted: see k_embed_direct
+constexpr uint32_t RANKED = 8192;  // tokens that are sorted by counting: see rank_tokens
 
 // ---- lookup: a warp takes a piece of 32 x 4 vectors of one row
 template <typename T, int N>
@@ -162,29 +164,70 @@ __device__ void sort_tokens(cg::cluster_group& cl, SortShared& sh, const int64_t
     }
 }
 
+// Zeros over `bytes` at `fill`, by blocks first, first + step, ..
+__device__ __forceinline__ void fill_zeros(unsigned char* fill, uint64_t bytes, uint64_t first, uint64_t step) {
+    // up to 31 bytes either side of the 32-byte pieces (a table whose rows are not whole pieces)
+    unsigned char* lo = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fill) + 31) & ~(uintptr_t)31);
+    const uint64_t head = min((uint64_t)(lo - fill), bytes), pieces = (bytes - head) / 32, tail = bytes - head - pieces * 32;
+    if (first == 0) {
+        if (threadIdx.x < head) fill[threadIdx.x] = 0;
+        if (threadIdx.x < tail) lo[pieces * 32 + threadIdx.x] = 0;
+    }
+    const uint32_t zero[8] = {};
+    for (uint64_t i = first * blockDim.x + threadIdx.x; i < pieces; i += step * blockDim.x) store32(lo + 32 * i, zero);
+}
+
 __global__ void __launch_bounds__(SORT_THREADS) k_embed_sort(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, int passes,
                                                              int bits, unsigned long long* a, unsigned long long* b,
                                                              unsigned char* fill, uint64_t fill_bytes) {
     extern __shared__ __align__(16) unsigned char raw[];
+    let_next();
     cg::cluster_group cl = cg::this_cluster();
     const uint32_t blocks = cl.num_blocks();
     if (blockIdx.x < blocks) {
-        if (n) sort_tokens(cl, *reinterpret_cast<SortShared*>(raw), ids, n, vocab, passes, bits, a, b);
+        sort_tokens(cl, *reinterpret_cast<SortShared*>(raw), ids, n, vocab, passes, bits, a, b);
         if (gridDim.x > blocks) return;  // others fill
     }
     const bool alone = gridDim.x <= blocks;
-    const uint64_t first = alone ? blockIdx.x : blockIdx.x - blocks, step = alone ? gridDim.x : gridDim.x - blocks;
-    // up to 15 bytes either side of the 16-byte pieces (a table whose rows are not whole pieces)
-    unsigned char* lo = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fill) + 15) & ~(uintptr_t)15);
-    const uint64_t head = min((uint64_t)(lo - fill), fill_bytes), pieces = (fill_bytes - head) / 16;
-    const uint64_t tail = fill_bytes - head - pieces * 16;
-    if (first == 0) {
-        if (threadIdx.x < head) fill[threadIdx.x] = 0;
-        if (threadIdx.x < tail) lo[pieces * 16 + threadIdx.x] = 0;
+    fill_zeros(fill, fill_bytes, alone ? blockIdx.x : blockIdx.x - blocks, alone ? gridDim.x : gridDim.x - blocks);
+}
+
+// ---- gradient, first launch, up to RANKED tokens: a token's place is the count of tokens with a smaller id, and of equal ones before it.
+// A block takes 64 tokens, 16 threads each, every one of which counts over a sixteenth of all tokens in shared memory: n^2 / 2 comparisons
+// a pair of instructions each, over all SMs in about 3 us for 8192 tokens, where the radix sort's barriers take 16. The other blocks fill.
+constexpr uint32_t RANK_TOKENS = 64;
+__global__ void __launch_bounds__(SORT_THREADS) k_embed_rank(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, unsigned long long* sorted,
+                                                             unsigned char* fill, uint64_t fill_bytes) {
+    __shared__ __align__(16) uint32_t key[RANKED];
+    let_next();
+    const uint32_t blocks = (n + RANK_TOKENS - 1) / RANK_TOKENS;
+    if (blockIdx.x < blocks) {
+        const uint32_t padded = (n + 63) & ~63u;
+        for (uint32_t i = threadIdx.x; i < padded; i += SORT_THREADS) {
+            const int64_t id = i < n ? ids[i] : -1;
+            key[i] = i < n ? ((uint64_t)id < vocab ? (uint32_t)id : vocab) : 0xffffffffu;
+        }
+        __syncthreads();
+        const uint32_t i = blockIdx.x * RANK_TOKENS + threadIdx.x / 16, part = threadIdx.x & 15;
+        const uint32_t mine = i < n ? key[i] : 0;
+        uint32_t count = 0;
+        for (uint32_t j = part * 4; j < padded; j += 64) {
+            const uint4 k = *reinterpret_cast<const uint4*>(key + j);
+            const uint32_t below = j + 4 <= i ? mine + 1 : mine;  // in front of the token equal ids count too
+            count += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
+            if (j < i && i < j + 4) count += (k.x == mine) + (j + 1 < i && k.y == mine) + (j + 2 < i && k.z == mine);
+        }
+#pragma unroll
+        for (int o = 8; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
+        if (part == 0 && i < n) sorted[count] = (unsigned long long)mine << 32 | i;
+        if (gridDim.x > blocks) return;  // others fill
     }
-    uint4* q = reinterpret_cast<uint4*>(lo);
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (uint64_t i = first * SORT_THREADS + threadIdx.x; i < pieces; i += step * SORT_THREADS) q[i] = zero;
+    const bool alone = gridDim.x <= blocks;
+    fill_zeros(fill, fill_bytes, alone ? blockIdx.x : blockIdx.x - blocks, alone ? gridDim.x : gridDim.x - blocks);
+}
+__global__ void __launch_bounds__(SORT_THREADS) k_embed_fill(unsigned char* fill, uint64_t fill_bytes) {
+    let_next();
+    fill_zeros(fill, fill_bytes, blockIdx.x, gridDim.x);
 }
 
 __device__ __forceinline__ uint32_t key_of(unsigned long long it) { return (uint32_t)(it >> 32); }
@@ -205,6 +248,8 @@ template <typename T, typename G, int N>
 __global__ void __launch_bounds__(256) k_embed_sums(const unsigned long long* __restrict__ sorted, uint32_t n, uint32_t vocab,
                                                     const T* __restrict__ d_out, uint64_t stride, uint32_t hidden, G* d_table,
                                                     float* __restrict__ carry, float scale, int accumulate, uint32_t slices) {
+    let_next();
+    after_previous();
     const uint64_t chunks = (n + CHUNK - 1) / CHUNK;
     const uint32_t lane = threadIdx.x & 31;
     for (uint64_t unit = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; unit < chunks * slices; unit += (uint64_t)gridDim.x * 8) {
@@ -266,6 +311,8 @@ __global__ void __launch_bounds__(256) k_embed_join(const unsigned long long* __
                                                     uint32_t hidden, G* d_table, const float* __restrict__ carry, float scale,
                                                     int accumulate) {
     __shared__ float part[8][32 * N];
+    let_next();
+    after_previous();
     const uint32_t chunk = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const uint64_t c0 = (uint64_t)chunk * CHUNK, c1 = c0 + CHUNK;
     if (c1 >= n) return;  // nothing leaves the last chunk
@@ -308,6 +355,79 @@ __global__ void __launch_bounds__(256) k_embed_join(const unsigned long long* __
     write_row<G, N>(d_table + (uint64_t)key * hidden + col, sum, scale, accumulate != 0);
 }
 
+// ---- gradient of up to DIRECT tokens in one launch (after the fill, when the table is overwritten). A block has one token and up to
+// 8 x 32 N columns: it leaves where an equal id stands before the token; else it lists the equal ones behind, in order, and sums their
+// rows, `splits` groups of warps a contiguous part of the list each, joined in order.
+template <typename T, typename G, int N>
+__global__ void __launch_bounds__(256) k_embed_direct(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, const T* __restrict__ d_out,
+                                                      uint64_t stride, uint32_t hidden, G* d_table, float scale, int accumulate, uint32_t wide) {
+    __shared__ uint16_t list[DIRECT];
+    __shared__ uint32_t counts[8];
+    __shared__ float share[256 * N];
+    let_next();
+    after_previous();
+    const uint32_t i = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const int64_t id = ids[i];
+    if ((uint64_t)id >= vocab) return;
+    bool before = false;
+    for (uint32_t j = threadIdx.x; j < i; j += 256) before |= ids[j] == id;
+    if (__syncthreads_or(before)) return;
+    // the equal ones from i on: each warp a run of 32 x turns tokens
+    const uint32_t turns = (n - i + 255) / 256, begin = i + warp * turns * 32;
+    uint32_t count = 0;
+    for (uint32_t t = 0; t < turns; t++) {
+        const uint32_t j = begin + t * 32 + lane;
+        count += __popc(__ballot_sync(0xffffffffu, j < n && ids[j] == id));
+    }
+    if (lane == 0) counts[warp] = count;
+    __syncthreads();
+    uint32_t at = 0, total = 0;
+    for (uint32_t w = 0; w < 8; w++) {
+        at += w < warp ? counts[w] : 0;
+        total += counts[w];
+    }
+    for (uint32_t t = 0; t < turns; t++) {
+        const uint32_t j = begin + t * 32 + lane;
+        const bool yes = j < n && ids[j] == id;
+        const uint32_t bits = __ballot_sync(0xffffffffu, yes);
+        if (yes) list[at + __popc(bits & ((1u << lane) - 1))] = (uint16_t)j;
+        at += __popc(bits);
+    }
+    __syncthreads();
+    // `wide` warps along a row, 8 / wide along the list
+    const uint32_t splits = 8 / wide, part = warp / wide, col = (blockIdx.y * wide + warp % wide) * 32 * N + lane * N;
+    const bool live = part < splits && col < hidden;
+    float sum[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) sum[j] = 0.f;
+    if (live) {
+        const uint32_t each = (total + splits - 1) / splits, k0 = min(total, part * each), k1 = min(total, k0 + each);
+        constexpr int AHEAD = 8;
+        for (uint32_t k = k0; k < k1; k += AHEAD) {
+            Vec<T, N> v[AHEAD];
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+                if (k + a < k1) v[a].load(d_out + (uint64_t)list[k + a] * stride + col);
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+                if (k + a < k1) {
+#pragma unroll
+                    for (int j = 0; j < N; j++) sum[j] += to_f32<T>(v[a].e[j]);
+                }
+        }
+    }
+    if (splits > 1) {
+#pragma unroll
+        for (int j = 0; j < N; j++) share[threadIdx.x * N + j] = sum[j];
+        __syncthreads();
+        if (part) return;
+        for (uint32_t p = 1; p < splits; p++)
+#pragma unroll
+            for (int j = 0; j < N; j++) sum[j] += share[(p * wide * 32 + threadIdx.x) * N + j];
+    }
+    if (live) write_row<G, N>(d_table + (uint64_t)id * hidden + col, sum, scale, accumulate != 0);
+}
+
 bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) % to) != 0; }
 
 template <typename T, int N>
@@ -319,17 +439,23 @@ void lookup(const oxz_embed_desc& d, const int64_t* ids, uint64_t n, const void*
 }
 
 template <typename T, typename G, int N>
-void sums(oxz_embed* e, uint32_t n, const unsigned long long* sorted, const void* d_out, uint64_t stride, void* d_table,
+int32_t sums(oxz_embed* e, uint32_t n, const int64_t* ids, const unsigned long long* sorted, const void* d_out, uint64_t stride, void* d_table,
              int32_t accumulate, cudaStream_t s) {
     const oxz_embed_desc& d = e->d;
-    const uint32_t chunks = (n + CHUNK - 1) / CHUNK, slices = (uint32_t)((d.hidden + 32 * N - 1) / (32 * N));
+    const uint32_t slices = (uint32_t)((d.hidden + 32 * N - 1) / (32 * N)), vocab = (uint32_t)d.vocab, hidden = (uint32_t)d.hidden;
+    if (n <= DIRECT) {
+        const uint32_t wide = std::min<uint32_t>(8, slices);
+        OXZ_CUDA(launch_after(!accumulate, k_embed_direct<T, G, N>, dim3(n, (slices + wide - 1) / wide), 256, 0, s, ids, n, vocab, static_cast<const T*>(d_out),
+                              stride, hidden, static_cast<G*>(d_table), (float)d.scale, accumulate, wide));
+        return OXZ_OK;
+    }
+    const uint32_t chunks = (n + CHUNK - 1) / CHUNK;
     const uint64_t blocks = std::min<uint64_t>(((uint64_t)chunks * slices + 7) / 8, 1u << 30);
-    k_embed_sums<T, G, N><<<(unsigned)blocks, 256, 0, s>>>(sorted, n, (uint32_t)d.vocab, static_cast<const T*>(d_out), stride,
-                                                           (uint32_t)d.hidden, static_cast<G*>(d_table), e->carry, (float)d.scale,
-                                                           accumulate, slices);
-    if (chunks > 1)
-        k_embed_join<G, N><<<dim3(chunks - 1, slices), 256, 0, s>>>(sorted, n, (uint32_t)d.vocab, (uint32_t)d.hidden,
-                                                                   static_cast<G*>(d_table), e->carry, (float)d.scale, accumulate);
+    OXZ_CUDA(launch_after(true, k_embed_sums<T, G, N>, (unsigned)blocks, 256, 0, s, sorted, n, vocab, static_cast<const T*>(d_out), stride, hidden,
+                          static_cast<G*>(d_table), e->carry, (float)d.scale, accumulate, slices));
+    OXZ_CUDA(launch_after(true, k_embed_join<G, N>, dim3(chunks - 1, slices), 256, 0, s, sorted, n, vocab, hidden, static_cast<G*>(d_table), e->carry,
+                          (float)d.scale, accumulate));
+    return OXZ_OK;
 }
 
 }  // namespace
@@ -446,41 +572,45 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
         OXZ_TRY(dev.enter(d.device));
         cudaStream_t s = (cudaStream_t)stream;
         OXZ_TRY(e->order.begin(s));
-        // keys run to vocab itself (ids outside the table): as few passes of at most DIGIT_BITS bits as hold them, of equal width
-        int key_bits = 1;
-        while ((d.vocab >> key_bits) != 0) key_bits++;
-        const int passes = (key_bits + DIGIT_BITS - 1) / DIGIT_BITS, bits = (key_bits + passes - 1) / passes;
         int sms = 0;
         OXZ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d.device));
-        // a cluster no larger than the tokens need: a warp walks 32 at a time
-        unsigned cluster = 1;
-        while (cluster < (unsigned)SORT_CLUSTER && (uint64_t)cluster * SORT_THREADS < n) cluster *= 2;
         const uint64_t fill_bytes = accumulate ? 0 : d.vocab * d.hidden * gs;
-        unsigned grid = cluster;
-        if (fill_bytes > (1u << 20)) grid = (unsigned)(sms * 2) / cluster * cluster;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(grid);
-        cfg.blockDim = dim3(SORT_THREADS);
-        cfg.dynamicSmemBytes = sizeof(SortShared);
-        cfg.stream = s;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim = {cluster, 1, 1};
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        OXZ_CUDA(cudaLaunchKernelEx(&cfg, k_embed_sort, ids, (uint32_t)n, (uint32_t)d.vocab, passes, bits, e->sorted[0], e->sorted[1],
-                                    static_cast<unsigned char*>(d_table), fill_bytes));
+        unsigned char* fill = static_cast<unsigned char*>(d_table);
+        const unsigned fillers = (unsigned)std::min<uint64_t>(sms * 2, (fill_bytes + (32 << 10) - 1) / (32 << 10));  // blocks of 32 KiB at least
+        const unsigned long long* sorted = e->sorted[0];
+        if (n <= DIRECT) {
+            if (fill_bytes) OXZ_CUDA(launch_after(false, k_embed_fill, fillers, SORT_THREADS, 0, s, fill, fill_bytes));
+        } else if (n <= RANKED) {
+            const unsigned blocks = ((unsigned)n + RANK_TOKENS - 1) / RANK_TOKENS;
+            OXZ_CUDA(launch_after(false, k_embed_rank, blocks + fillers, SORT_THREADS, 0, s, ids, (uint32_t)n, (uint32_t)d.vocab, e->sorted[0], fill, fill_bytes));
+        } else {
+            // keys run to vocab itself (ids outside the table): as few passes of at most DIGIT_BITS bits as hold them, of equal width
+            int key_bits = 1;
+            while ((d.vocab >> key_bits) != 0) key_bits++;
+            const int passes = (key_bits + DIGIT_BITS - 1) / DIGIT_BITS, bits = (key_bits + passes - 1) / passes;
+            sorted = e->sorted[passes & 1];
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3((SORT_CLUSTER + fillers + SORT_CLUSTER - 1) / SORT_CLUSTER * SORT_CLUSTER);
+            cfg.blockDim = dim3(SORT_THREADS);
+            cfg.dynamicSmemBytes = sizeof(SortShared);
+            cfg.stream = s;
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim = {SORT_CLUSTER, 1, 1};
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            OXZ_CUDA(cudaLaunchKernelEx(&cfg, k_embed_sort, ids, (uint32_t)n, (uint32_t)d.vocab, passes, bits, e->sorted[0], e->sorted[1], fill, fill_bytes));
+        }
         if (n) {
-            const unsigned long long* sorted = e->sorted[passes & 1];
             const bool wide = !misaligned(d_out, 16) && !misaligned(d_table, 16) && d.hidden * es % 16 == 0 && d_out_stride * es % 16 == 0;
             const uint32_t m = (uint32_t)n;
             const uint64_t st = d_out_stride;
             const bool f32g = d.grad_dtype == OXZ_F32;
-            if (d.dtype == OXZ_F32) wide ? (sums<float, float, 4>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<float, float, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
-            else if (d.dtype == OXZ_BF16 && !f32g) wide ? (sums<__nv_bfloat16, __nv_bfloat16, 8>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<__nv_bfloat16, __nv_bfloat16, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
-            else if (d.dtype == OXZ_BF16) wide ? (sums<__nv_bfloat16, float, 8>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<__nv_bfloat16, float, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
-            else if (!f32g) wide ? (sums<__half, __half, 8>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<__half, __half, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
-            else wide ? (sums<__half, float, 8>(e, m, sorted, d_out, st, d_table, accumulate, s)) : (sums<__half, float, 1>(e, m, sorted, d_out, st, d_table, accumulate, s));
+            if (d.dtype == OXZ_F32) OXZ_TRY((wide ? sums<float, float, 4>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<float, float, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
+            else if (d.dtype == OXZ_BF16 && !f32g) OXZ_TRY((wide ? sums<__nv_bfloat16, __nv_bfloat16, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__nv_bfloat16, __nv_bfloat16, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
+            else if (d.dtype == OXZ_BF16) OXZ_TRY((wide ? sums<__nv_bfloat16, float, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__nv_bfloat16, float, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
+            else if (!f32g) OXZ_TRY((wide ? sums<__half, __half, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__half, __half, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
+            else OXZ_TRY((wide ? sums<__half, float, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__half, float, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
         }
         OXZ_CUDA(cudaGetLastError());
         return e->order.end(s);
