@@ -375,6 +375,49 @@ class LitDataLoader {
     uint64_t batch_;
 };
 
+// ---- the token operators: the embedding and the loss head, on device pointers
+class TokenEmbedding {
+  public:
+    TokenEmbedding(uint64_t vocab, uint64_t hidden, uint64_t max_tokens, oxz_dtype dtype, oxz_dtype grad_dtype, double scale = 1.0, int32_t device = 0) {
+        const oxz_embed_desc d{max_tokens, hidden, vocab, scale, dtype, grad_dtype, device, 0};
+        check(oxz_embed_create(&d, &h_));
+    }
+    TokenEmbedding(TokenEmbedding&& o) noexcept : h_(o.h_) { o.h_ = nullptr; }
+    TokenEmbedding(const TokenEmbedding&) = delete;
+    ~TokenEmbedding() { if (h_) oxz_embed_destroy(h_); }
+    uint64_t alloc() { uint64_t bytes = 0; check(oxz_embed_alloc(h_, &bytes)); return bytes; }
+    void lookup(const int64_t* ids, uint64_t n, const void* table, void* out, uint64_t out_stride = 0, void* stream = nullptr) const {
+        check(oxz_embed_lookup_async(h_, ids, n, table, out, out_stride, stream));
+    }
+    void grads(const int64_t* ids, uint64_t n, const void* d_out, void* d_table, bool accumulate, uint64_t d_out_stride = 0, void* stream = nullptr) {
+        check(oxz_embed_grads_async(h_, ids, n, d_out, d_out_stride, d_table, accumulate, stream));
+    }
+  private:
+    oxz_embed* h_ = nullptr;
+};
+class LossHead {
+  public:
+    LossHead(uint64_t vocab, uint64_t hidden, uint64_t max_rows, oxz_dtype dtype, oxz_dtype grad_dtype, uint64_t piece_bytes = 0, int32_t device = 0) {
+        const oxz_head_desc d{max_rows, hidden, vocab, piece_bytes, dtype, grad_dtype, device, 0};
+        check(oxz_head_create(&d, &h_));
+    }
+    LossHead(LossHead&& o) noexcept : h_(o.h_) { o.h_ = nullptr; }
+    LossHead(const LossHead&) = delete;
+    ~LossHead() { if (h_) oxz_head_destroy(h_); }
+    uint64_t alloc() { uint64_t bytes = 0; check(oxz_head_alloc(h_, &bytes)); return bytes; }
+    void loss(const oxz_head_batch& b, float* row_loss, float* row_stats, float* totals, void* stream = nullptr) {
+        check(oxz_head_loss_async(h_, &b, row_loss, row_stats, totals, stream));
+    }
+    void grads(const oxz_head_batch& b, const float* row_stats, const oxz_head_grads& g, void* stream = nullptr) {
+        check(oxz_head_grads_async(h_, &b, row_stats, &g, stream));
+    }
+    void loss_and_grads(const oxz_head_batch& b, float* row_loss, float* row_stats, float* totals, const oxz_head_grads& g, void* stream = nullptr) {
+        check(oxz_head_loss_grads_async(h_, &b, row_loss, row_stats, totals, &g, stream));
+    }
+  private:
+    oxz_head* h_ = nullptr;
+};
+
 // ---- the optimizer state and step
 struct StepConfig {  // trainer keys with the reference's defaults (src/config.rs:40-62)
     double lr = 3e-4, beta1 = 0.9, beta2 = 0.95, eps = 1e-6, weight_decay = 0.1, max_grad_norm = 1.0;

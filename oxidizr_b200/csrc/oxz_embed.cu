@@ -21,6 +21,9 @@ struct oxz_embed {
     uint64_t bytes = 0;
     unsigned long long* sorted[2] = {nullptr, nullptr};  // token << 32 | position, max_tokens each
     float* carry = nullptr;                              // [chunks][2][hidden]: partial sums of the tokens that cross chunks
+    uint32_t* touched = nullptr;                         // a bit for every row of the table: it has a token. All 0 between calls
+    bool clean = false;                                  // ... unless a call broke off
+    int sms = 0;
     oxz::StreamOrder order;
 };
 
@@ -59,8 +62,7 @@ __global__ void __launch_bounds__(256) k_embed_lookup(const int64_t* __restrict_
     }
 }
 
-// ---- gradient, first launch. Cluster 0 sorts the tokens; when the table is overwritten the other clusters fill it with zeros
-// meanwhile, which hides the sort behind the fill (the longer of the two wherever the table is worth filling).
+// ---- gradient, first launch: the tokens sorted, by one cluster of blocks.
 //
 // The sort is a least-significant-digit radix sort by digits of at most 9 bits. A block owns a contiguous run of the items, a
 // warp a contiguous run of the block's, and walks it 32 at a time: __match_any_sync ranks equal digits within the 32, a
@@ -177,53 +179,62 @@ __device__ __forceinline__ void fill_zeros(unsigned char* fill, uint64_t bytes, 
     for (uint64_t i = first * blockDim.x + threadIdx.x; i < pieces; i += step * blockDim.x) store32(lo + 32 * i, zero);
 }
 
+// A table that is overwritten is filled with zeros where no token is: the first launch marks the rows that have one.
+__device__ __forceinline__ void mark(uint32_t* touched, uint32_t key, uint32_t vocab) {
+    if (touched && key < vocab) atomicOr(&touched[key >> 5], 1u << (key & 31));
+}
+
 __global__ void __launch_bounds__(SORT_THREADS) k_embed_sort(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, int passes,
-                                                             int bits, unsigned long long* a, unsigned long long* b,
-                                                             unsigned char* fill, uint64_t fill_bytes) {
+                                                             int bits, unsigned long long* a, unsigned long long* b, uint32_t* touched) {
     extern __shared__ __align__(16) unsigned char raw[];
     let_next();
     cg::cluster_group cl = cg::this_cluster();
-    const uint32_t blocks = cl.num_blocks();
-    if (blockIdx.x < blocks) {
-        sort_tokens(cl, *reinterpret_cast<SortShared*>(raw), ids, n, vocab, passes, bits, a, b);
-        if (gridDim.x > blocks) return;  // others fill
+    sort_tokens(cl, *reinterpret_cast<SortShared*>(raw), ids, n, vocab, passes, bits, a, b);
+    for (uint32_t i = blockIdx.x * SORT_THREADS + threadIdx.x; i < n; i += gridDim.x * SORT_THREADS) {
+        const int64_t id = ids[i];
+        mark(touched, (uint64_t)id < vocab ? (uint32_t)id : vocab, vocab);
     }
-    const bool alone = gridDim.x <= blocks;
-    fill_zeros(fill, fill_bytes, alone ? blockIdx.x : blockIdx.x - blocks, alone ? gridDim.x : gridDim.x - blocks);
 }
 
 // ---- gradient, first launch, up to RANKED tokens: a token's place is the count of tokens with a smaller id, and of equal ones before it.
-// A block takes 64 tokens, 16 threads each, every one of which counts over a sixteenth of all tokens in shared memory: n^2 / 2 comparisons
-// a pair of instructions each, over all SMs in about 3 us for 8192 tokens, where the radix sort's barriers take 16. The other blocks fill.
+// A block takes 64 tokens, 16 threads each, every one of which counts over a sixteenth of all tokens in shared memory: 8192 tokens
+// take 7 us over all SMs, where the radix sort's barriers take 16.
 constexpr uint32_t RANK_TOKENS = 64;
 __global__ void __launch_bounds__(SORT_THREADS) k_embed_rank(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, unsigned long long* sorted,
-                                                             unsigned char* fill, uint64_t fill_bytes) {
+                                                             uint32_t* touched) {
     __shared__ __align__(16) uint32_t key[RANKED];
     let_next();
-    const uint32_t blocks = (n + RANK_TOKENS - 1) / RANK_TOKENS;
-    if (blockIdx.x < blocks) {
-        const uint32_t padded = (n + 63) & ~63u;
-        for (uint32_t i = threadIdx.x; i < padded; i += SORT_THREADS) {
-            const int64_t id = i < n ? ids[i] : -1;
-            key[i] = i < n ? ((uint64_t)id < vocab ? (uint32_t)id : vocab) : 0xffffffffu;
-        }
-        __syncthreads();
-        const uint32_t i = blockIdx.x * RANK_TOKENS + threadIdx.x / 16, part = threadIdx.x & 15;
-        const uint32_t mine = i < n ? key[i] : 0;
-        uint32_t count = 0;
-        for (uint32_t j = part * 4; j < padded; j += 64) {
-            const uint4 k = *reinterpret_cast<const uint4*>(key + j);
-            const uint32_t below = j + 4 <= i ? mine + 1 : mine;  // in front of the token equal ids count too
-            count += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
-            if (j < i && i < j + 4) count += (k.x == mine) + (j + 1 < i && k.y == mine) + (j + 2 < i && k.z == mine);
-        }
-#pragma unroll
-        for (int o = 8; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
-        if (part == 0 && i < n) sorted[count] = (unsigned long long)mine << 32 | i;
-        if (gridDim.x > blocks) return;  // others fill
+    const uint32_t padded = (n + 63) & ~63u;
+    for (uint32_t i = threadIdx.x; i < padded; i += SORT_THREADS) {
+        const int64_t id = i < n ? ids[i] : -1;
+        key[i] = i < n ? ((uint64_t)id < vocab ? (uint32_t)id : vocab) : 0xffffffffu;
     }
-    const bool alone = gridDim.x <= blocks;
-    fill_zeros(fill, fill_bytes, alone ? blockIdx.x : blockIdx.x - blocks, alone ? gridDim.x : gridDim.x - blocks);
+    __syncthreads();
+    const uint32_t i = blockIdx.x * RANK_TOKENS + threadIdx.x / 16, part = threadIdx.x & 15;
+    const uint32_t mine = i < n ? key[i] : 0;
+    uint32_t count = 0;
+    for (uint32_t j = part * 4; j < padded; j += 64) {
+        const uint4 k = *reinterpret_cast<const uint4*>(key + j);
+        const uint32_t below = j + 4 <= i ? mine + 1 : mine;  // in front of the token equal ids count too
+        count += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
+        if (j < i && i < j + 4) count += (k.x == mine) + (j + 1 < i && k.y == mine) + (j + 2 < i && k.z == mine);
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
+    if (part == 0 && i < n) {
+        sorted[count] = (unsigned long long)mine << 32 | i;
+        mark(touched, mine, vocab);
+    }
+}
+// Zeros over one row, by a warp
+__device__ __forceinline__ void fill_row(unsigned char* row, uint64_t bytes) {
+    const uint32_t lane = threadIdx.x & 31;
+    unsigned char* lo = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(row) + 31) & ~(uintptr_t)31);
+    const uint64_t head = min((uint64_t)(lo - row), bytes), pieces = (bytes - head) / 32, tail = bytes - head - pieces * 32;
+    const uint32_t zero[8] = {};
+    for (uint64_t i = lane; i < pieces; i += 32) store32(lo + 32 * i, zero);
+    if (lane < head) row[lane] = 0;
+    if (lane < tail) lo[pieces * 32 + lane] = 0;
 }
 __global__ void __launch_bounds__(SORT_THREADS) k_embed_fill(unsigned char* fill, uint64_t fill_bytes) {
     let_next();
@@ -244,15 +255,24 @@ __device__ __forceinline__ void write_row(G* dst, const float (&sum)[N], float s
 // ---- gradient, second launch: a warp sums one chunk of CHUNK sorted tokens for 32 x N columns. Tokens that lie inside the
 // chunk are written; the sums of a token that goes on from the chunk before or into the chunk after go to the carries:
 // carry[chunk][0] for the token the chunk begins with, carry[chunk][1] for one that begins in the chunk and leaves it.
+// Blocks from `summing` on write zeros to the rows that have no token: the sums wait on their loads, the zeros take the memory meanwhile
+// (a fill of all rows beside the sort, and the sums after it, took 133 us where this takes 124: 8192 x 2048 bf16, 128256 rows).
 template <typename T, typename G, int N>
 __global__ void __launch_bounds__(256) k_embed_sums(const unsigned long long* __restrict__ sorted, uint32_t n, uint32_t vocab,
                                                     const T* __restrict__ d_out, uint64_t stride, uint32_t hidden, G* d_table,
-                                                    float* __restrict__ carry, float scale, int accumulate, uint32_t slices) {
+                                                    float* __restrict__ carry, float scale, int accumulate, uint32_t slices,
+                                                    uint32_t summing, const uint32_t* __restrict__ touched) {
     let_next();
     after_previous();
+    if (blockIdx.x >= summing) {
+        const uint64_t row_bytes = (uint64_t)hidden * sizeof(G), warps = (uint64_t)(gridDim.x - summing) * 8;
+        for (uint64_t row = (uint64_t)(blockIdx.x - summing) * 8 + threadIdx.x / 32; row < vocab; row += warps)
+            if (!(touched[row >> 5] >> (row & 31) & 1)) fill_row(reinterpret_cast<unsigned char*>(d_table) + row * row_bytes, row_bytes);
+        return;
+    }
     const uint64_t chunks = (n + CHUNK - 1) / CHUNK;
     const uint32_t lane = threadIdx.x & 31;
-    for (uint64_t unit = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; unit < chunks * slices; unit += (uint64_t)gridDim.x * 8) {
+    for (uint64_t unit = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; unit < chunks * slices; unit += (uint64_t)summing * 8) {
         const uint32_t chunk = (uint32_t)(unit / slices);
         const uint64_t c0 = (uint64_t)chunk * CHUNK;
         const uint32_t col = (uint32_t)(unit - (uint64_t)chunk * slices) * 32 * N + lane * N;
@@ -309,10 +329,12 @@ __global__ void __launch_bounds__(256) k_embed_sums(const unsigned long long* __
 template <typename G, int N>
 __global__ void __launch_bounds__(256) k_embed_join(const unsigned long long* __restrict__ sorted, uint32_t n, uint32_t vocab,
                                                     uint32_t hidden, G* d_table, const float* __restrict__ carry, float scale,
-                                                    int accumulate) {
+                                                    int accumulate, uint32_t* touched) {
     __shared__ float part[8][32 * N];
     let_next();
     after_previous();
+    if (touched && blockIdx.y == 0)  // for the next call
+        for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < ((uint64_t)vocab + 31) / 32; i += (uint64_t)gridDim.x * 256) touched[i] = 0;
     const uint32_t chunk = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const uint64_t c0 = (uint64_t)chunk * CHUNK, c1 = c0 + CHUNK;
     if (c1 >= n) return;  // nothing leaves the last chunk
@@ -450,11 +472,13 @@ int32_t sums(oxz_embed* e, uint32_t n, const int64_t* ids, const unsigned long l
         return OXZ_OK;
     }
     const uint32_t chunks = (n + CHUNK - 1) / CHUNK;
-    const uint64_t blocks = std::min<uint64_t>(((uint64_t)chunks * slices + 7) / 8, 1u << 30);
-    OXZ_CUDA(launch_after(true, k_embed_sums<T, G, N>, (unsigned)blocks, 256, 0, s, sorted, n, vocab, static_cast<const T*>(d_out), stride, hidden,
-                          static_cast<G*>(d_table), e->carry, (float)d.scale, accumulate, slices));
+    const unsigned blocks = (unsigned)std::min<uint64_t>(((uint64_t)chunks * slices + 7) / 8, 1u << 30);
+    uint32_t* touched = accumulate ? nullptr : e->touched;
+    const unsigned fillers = accumulate ? 0 : (unsigned)std::min<uint64_t>(e->sms * 8, (d.vocab + 7) / 8);
+    OXZ_CUDA(launch_after(true, k_embed_sums<T, G, N>, blocks + fillers, 256, 0, s, sorted, n, vocab, static_cast<const T*>(d_out), stride, hidden,
+                          static_cast<G*>(d_table), e->carry, (float)d.scale, accumulate, slices, blocks, touched));
     OXZ_CUDA(launch_after(true, k_embed_join<G, N>, dim3(chunks - 1, slices), 256, 0, s, sorted, n, vocab, hidden, static_cast<G*>(d_table), e->carry,
-                          (float)d.scale, accumulate));
+                          (float)d.scale, accumulate, touched));
     return OXZ_OK;
 }
 
@@ -501,9 +525,14 @@ int32_t oxz_embed_alloc(oxz_embed* e, uint64_t* workspace_bytes) {
             for (int i = 0; i < 2; i++)
                 if (!e->sorted[i]) OXZ_CUDA(cudaMalloc((void**)&e->sorted[i], items));
             if (!e->carry) OXZ_CUDA(cudaMalloc((void**)&e->carry, carry));
+            if (!e->touched) OXZ_CUDA(cudaMalloc((void**)&e->touched, (e->d.vocab + 31) / 32 * 4));
+            OXZ_CUDA(cudaMemset(e->touched, 0, (e->d.vocab + 31) / 32 * 4));
+            OXZ_CUDA(cudaDeviceSynchronize());
+            e->clean = true;
+            OXZ_CUDA(cudaDeviceGetAttribute(&e->sms, cudaDevAttrMultiProcessorCount, e->d.device));
             OXZ_TRY(e->order.create());
             OXZ_CUDA(cudaFuncSetAttribute(k_embed_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared)));
-            e->bytes = 2 * items + carry;
+            e->bytes = 2 * items + carry + (e->d.vocab + 31) / 32 * 4;
             e->allocated = true;
         }
         if (workspace_bytes) *workspace_bytes = e->bytes;
@@ -520,6 +549,7 @@ int32_t oxz_embed_destroy(oxz_embed* e) {
         for (int i = 0; i < 2; i++)
             if (e->sorted[i]) cudaFree(e->sorted[i]);
         if (e->carry) cudaFree(e->carry);
+        if (e->touched) cudaFree(e->touched);
         delete e;
         return OXZ_OK;
     });
@@ -572,34 +602,37 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
         OXZ_TRY(dev.enter(d.device));
         cudaStream_t s = (cudaStream_t)stream;
         OXZ_TRY(e->order.begin(s));
-        int sms = 0;
-        OXZ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d.device));
-        const uint64_t fill_bytes = accumulate ? 0 : d.vocab * d.hidden * gs;
-        unsigned char* fill = static_cast<unsigned char*>(d_table);
-        const unsigned fillers = (unsigned)std::min<uint64_t>(sms * 2, (fill_bytes + (32 << 10) - 1) / (32 << 10));  // blocks of 32 KiB at least
         const unsigned long long* sorted = e->sorted[0];
+        uint32_t* touched = accumulate ? nullptr : e->touched;
         if (n <= DIRECT) {
-            if (fill_bytes) OXZ_CUDA(launch_after(false, k_embed_fill, fillers, SORT_THREADS, 0, s, fill, fill_bytes));
-        } else if (n <= RANKED) {
-            const unsigned blocks = ((unsigned)n + RANK_TOKENS - 1) / RANK_TOKENS;
-            OXZ_CUDA(launch_after(false, k_embed_rank, blocks + fillers, SORT_THREADS, 0, s, ids, (uint32_t)n, (uint32_t)d.vocab, e->sorted[0], fill, fill_bytes));
+            const uint64_t bytes = d.vocab * d.hidden * gs;
+            if (!accumulate)  // blocks of 32 KiB at least
+                OXZ_CUDA(launch_after(false, k_embed_fill, (unsigned)std::min<uint64_t>(e->sms * 2, (bytes + (32 << 10) - 1) / (32 << 10)), SORT_THREADS, 0, s,
+                                      static_cast<unsigned char*>(d_table), bytes));
         } else {
-            // keys run to vocab itself (ids outside the table): as few passes of at most DIGIT_BITS bits as hold them, of equal width
-            int key_bits = 1;
-            while ((d.vocab >> key_bits) != 0) key_bits++;
-            const int passes = (key_bits + DIGIT_BITS - 1) / DIGIT_BITS, bits = (key_bits + passes - 1) / passes;
-            sorted = e->sorted[passes & 1];
-            cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3((SORT_CLUSTER + fillers + SORT_CLUSTER - 1) / SORT_CLUSTER * SORT_CLUSTER);
-            cfg.blockDim = dim3(SORT_THREADS);
-            cfg.dynamicSmemBytes = sizeof(SortShared);
-            cfg.stream = s;
-            cudaLaunchAttribute attr{};
-            attr.id = cudaLaunchAttributeClusterDimension;
-            attr.val.clusterDim = {SORT_CLUSTER, 1, 1};
-            cfg.attrs = &attr;
-            cfg.numAttrs = 1;
-            OXZ_CUDA(cudaLaunchKernelEx(&cfg, k_embed_sort, ids, (uint32_t)n, (uint32_t)d.vocab, passes, bits, e->sorted[0], e->sorted[1], fill, fill_bytes));
+            if (touched && !e->clean) OXZ_CUDA(cudaMemsetAsync(touched, 0, (d.vocab + 31) / 32 * 4, s));
+            if (touched) e->clean = false;  // until every launch of this call has been made
+            if (n <= RANKED) {
+                OXZ_CUDA(launch_after(false, k_embed_rank, ((unsigned)n + RANK_TOKENS - 1) / RANK_TOKENS, SORT_THREADS, 0, s, ids, (uint32_t)n, (uint32_t)d.vocab,
+                                      e->sorted[0], touched));
+            } else {
+                // keys run to vocab itself (ids outside the table): as few passes of at most DIGIT_BITS bits as hold them, of equal width
+                int key_bits = 1;
+                while ((d.vocab >> key_bits) != 0) key_bits++;
+                const int passes = (key_bits + DIGIT_BITS - 1) / DIGIT_BITS, bits = (key_bits + passes - 1) / passes;
+                sorted = e->sorted[passes & 1];
+                cudaLaunchConfig_t cfg{};
+                cfg.gridDim = dim3(SORT_CLUSTER);
+                cfg.blockDim = dim3(SORT_THREADS);
+                cfg.dynamicSmemBytes = sizeof(SortShared);
+                cfg.stream = s;
+                cudaLaunchAttribute attr{};
+                attr.id = cudaLaunchAttributeClusterDimension;
+                attr.val.clusterDim = {SORT_CLUSTER, 1, 1};
+                cfg.attrs = &attr;
+                cfg.numAttrs = 1;
+                OXZ_CUDA(cudaLaunchKernelEx(&cfg, k_embed_sort, ids, (uint32_t)n, (uint32_t)d.vocab, passes, bits, e->sorted[0], e->sorted[1], touched));
+            }
         }
         if (n) {
             const bool wide = !misaligned(d_out, 16) && !misaligned(d_table, 16) && d.hidden * es % 16 == 0 && d_out_stride * es % 16 == 0;
@@ -613,6 +646,7 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
             else OXZ_TRY((wide ? sums<__half, float, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__half, float, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
         }
         OXZ_CUDA(cudaGetLastError());
+        if (n > DIRECT && touched) e->clean = true;
         return e->order.end(s);
     });
 }

@@ -806,6 +806,11 @@ class DpOptimizer:
         check(lib().oxz_state_pointers(self._h, *[C.byref(p) for p in ps]))
         return dict(zip(("grads", "work", "master", "exp_avg", "exp_avg_sq"), [p.value for p in ps]))
 
+    def tensor_addresses(self, tensor: int) -> tuple[int, int]:
+        """Device addresses of one tensor in the flat buffers: its working weights and its gradient."""
+        p, size = self.pointers(), {F32: 4, BF16: 2, F16: 2}
+        return (p["work"] + self.offsets[tensor] * size[self.param_dtype], p["grads"] + self.offsets[tensor] * size[self.grad_dtype])
+
     def _dtype_of(self, kind: int):
         return _NP[self.grad_dtype] if kind == ffi.STATE_GRADS else _NP[self.param_dtype] if kind == ffi.STATE_WORK else np.float32
 
@@ -1108,6 +1113,38 @@ class LitTrainerStep:
                               loss_scale=self.loss_scale_state(), world_size=self.world_size(),
                               global_batch_rows=layout.batch_size() if layout is not None else None, spike_guard=guard,
                               mixture=mixture)
+
+    # -- the two ends of the model that touch tokens, over the optimizer's own buffers (src/trainer.rs:309-316, 373-482). The work
+    # is enqueued on `stream`: order it before the step (set_stream, or a synchronisation), as any backward's.
+    def embed(self, embedding: TokenEmbedding, tensor: int, ids: int, n: int, out: int, out_stride: int = 0, stream: int | None = None) -> None:
+        """The hidden states of a micro-batch's inputs, from the working weights of embed_tokens (`tensor`)."""
+        embedding.lookup(ids, n, self.optimizer.tensor_addresses(tensor)[0], out, out_stride, stream)
+
+    def embed_grads(self, embedding: TokenEmbedding, tensor: int, ids: int, n: int, d_out: int, accumulate: bool, d_out_stride: int = 0,
+                    stream: int | None = None) -> None:
+        """The gradient of ``embed`` into the flat buffer. ``accumulate`` False on the first micro-batch of a step, unless the tensor is
+        tied to the head's, whose gradient is there already."""
+        embedding.grads(ids, n, d_out, self.optimizer.tensor_addresses(tensor)[1], accumulate, d_out_stride, stream)
+
+    def loss_weight(self, rows: int, micro_batches: int, scored: int | None = None) -> float:
+        """What a micro-batch's summed losses count in the step's loss (src/step_loss.rs:79-112): one over the step's scored tokens when
+        a mask is set, else the mean over its rows over the step's micro-batches of all ranks (``step_weighting``)."""
+        if scored is not None:
+            return 1.0 / scored if scored > 0 else 0.0
+        return 1.0 / (rows * micro_batches) if rows else 0.0
+
+    def loss_and_grads(self, head: LossHead, tensor: int, rows: int, hidden: int, targets: int, totals: int, d_hidden: int | None,
+                       micro_batches: int = 1, scored: int | None = None, loss_mask: int | None = None, accumulate: bool = False,
+                       row_loss: int | None = None, hidden_stride: int = 0, d_hidden_stride: int = 0, stream: int | None = None) -> float:
+        """One micro-batch's losses and gradients: d_hidden for the layers below, the head's own into the flat gradient buffer of
+        ``tensor`` (lm_head, or embed_tokens where the two are tied), both times the loss scale. Returns the weight of ``totals[0]`` in
+        the step's loss: the local loss ``training_step`` takes is the sum over the micro-batches of weight * totals[0]."""
+        weight = self.loss_weight(rows, micro_batches, scored)
+        work, grad = self.optimizer.tensor_addresses(tensor)
+        head.loss_and_grads(rows, hidden, work, targets, loss_mask=loss_mask, row_loss=row_loss, totals=totals, d_hidden=d_hidden, d_weight=grad,
+                            grad_scale=weight * (self.loss_scaler.scale() if self.loss_scaler else 1.0), accumulate=accumulate,
+                            hidden_stride=hidden_stride, d_hidden_stride=d_hidden_stride, stream=stream)
+        return weight
 
     def training_step(self, local_loss: float, present: list[bool] | None = None) -> tuple[float, float]:
         opt = self.optimizer

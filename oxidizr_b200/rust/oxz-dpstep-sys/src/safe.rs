@@ -380,3 +380,84 @@ impl Drop for Loader {
         unsafe { sys::oxz_loader_close(self.raw) };
     }
 }
+
+/// The token embedding and its gradient (embed_tokens, src/model.rs:3905-3953). Pointers are device memory.
+pub struct TokenEmbedding {
+    raw: *mut sys::oxz_embed,
+}
+
+impl TokenEmbedding {
+    pub fn new(desc: &sys::oxz_embed_desc) -> Result<Self> {
+        let mut raw = ptr::null_mut();
+        check(unsafe { sys::oxz_embed_create(desc, &mut raw) })?;
+        let this = Self { raw };
+        check(unsafe { sys::oxz_embed_alloc(this.raw, ptr::null_mut()) })?;
+        Ok(this)
+    }
+
+    /// # Safety
+    /// `ids`, `table` and `out` are device memory of the sizes the description and `n` give.
+    pub unsafe fn lookup(&self, ids: *const i64, n: u64, table: *const c_void, out: *mut c_void, stream: *mut c_void) -> Result<()> {
+        check(sys::oxz_embed_lookup_async(self.raw, ids, n, table, out, 0, stream))
+    }
+
+    /// # Safety
+    /// As `lookup`; `d_table` is the table's gradient.
+    pub unsafe fn grads(
+        &mut self,
+        ids: *const i64,
+        n: u64,
+        d_out: *const c_void,
+        d_table: *mut c_void,
+        accumulate: bool,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        check(sys::oxz_embed_grads_async(self.raw, ids, n, d_out, 0, d_table, accumulate as i32, stream))
+    }
+}
+
+impl Drop for TokenEmbedding {
+    fn drop(&mut self) {
+        unsafe { sys::oxz_embed_destroy(self.raw) };
+    }
+}
+
+/// Softmax cross entropy over the vocabulary with its gradients (the step loss of src/step_loss.rs over lm_head).
+pub struct LossHead {
+    raw: *mut sys::oxz_head,
+}
+
+impl LossHead {
+    pub fn new(desc: &sys::oxz_head_desc) -> Result<Self> {
+        let mut raw = ptr::null_mut();
+        check(unsafe { sys::oxz_head_create(desc, &mut raw) })?;
+        let this = Self { raw };
+        check(unsafe { sys::oxz_head_alloc(this.raw, ptr::null_mut()) })?;
+        Ok(this)
+    }
+
+    /// # Safety
+    /// The batch's pointers and the outputs are device memory of the sizes the description and the batch give.
+    pub unsafe fn loss(&mut self, batch: &sys::oxz_head_batch, row_loss: *mut f32, totals: *mut f32, stream: *mut c_void) -> Result<()> {
+        check(sys::oxz_head_loss_async(self.raw, batch, row_loss, ptr::null_mut(), totals, stream))
+    }
+
+    /// # Safety
+    /// As `loss`; `grads` names the gradients' memory.
+    pub unsafe fn loss_and_grads(
+        &mut self,
+        batch: &sys::oxz_head_batch,
+        row_loss: *mut f32,
+        totals: *mut f32,
+        grads: &sys::oxz_head_grads,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        check(sys::oxz_head_loss_grads_async(self.raw, batch, row_loss, ptr::null_mut(), totals, grads, stream))
+    }
+}
+
+impl Drop for LossHead {
+    fn drop(&mut self) {
+        unsafe { sys::oxz_head_destroy(self.raw) };
+    }
+}
