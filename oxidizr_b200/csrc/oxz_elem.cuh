@@ -23,7 +23,7 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// N consecutive elements as one access of N * sizeof(T) bytes (16 at most; 32 as two).
+// N consecutive elements as one access of N * sizeof(T) bytes (32 as two of 16).
 template <typename T, int N>
 struct Vec {
     static constexpr int BYTES = N * (int)sizeof(T);
@@ -36,8 +36,10 @@ struct Vec {
         if constexpr (BYTES >= 16) {
 #pragma unroll
             for (int i = 0; i < BYTES / 16; i++) q[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        } else if constexpr (BYTES == 8) {
+            *reinterpret_cast<uint2*>(q) = __ldg(reinterpret_cast<const uint2*>(p));
         } else {
-            static_assert(N == 1, "a piece is 16 bytes or one element");
+            static_assert(N == 1, "a piece is 8, 16 or 32 bytes, or one element");
             e[0] = *p;
         }
     }
@@ -47,6 +49,7 @@ struct Vec {
 #pragma unroll
             for (int i = 0; i < BYTES / 16; i++) q[i] = reinterpret_cast<const uint4*>(p)[i];
         } else {
+            static_assert(N == 1, "a piece is 16 or 32 bytes, or one element");
             e[0] = *p;
         }
     }
@@ -54,7 +57,10 @@ struct Vec {
         if constexpr (BYTES >= 16) {
 #pragma unroll
             for (int i = 0; i < BYTES / 16; i++) reinterpret_cast<uint4*>(p)[i] = q[i];
+        } else if constexpr (BYTES == 8) {
+            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(q);
         } else {
+            static_assert(N == 1, "a piece is 8, 16 or 32 bytes, or one element");
             *p = e[0];
         }
     }

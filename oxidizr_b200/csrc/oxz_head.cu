@@ -71,6 +71,21 @@ namespace {
 constexpr uint32_t FINISH_ROWS = 32;  // rows a block of k_head_finish takes
 constexpr uint32_t MMA_M = 256, MMA_N = 256, MMA_K = 64;  // tile of a pair of SMs
 
+__host__ __device__ inline uint32_t tiles_of(uint64_t n, uint32_t of) { return (uint32_t)((n + of - 1) / of); }
+
+__device__ __forceinline__ void describe(HeadMeta* meta, uint32_t n, double weight_sum, float top, int f16, uint64_t vocab, uint64_t l_elems) {
+    meta->n = n;
+    meta->done = 0;
+    meta->weight_sum = weight_sum;
+    // f16 holds 2^-24 .. 65504: the largest weight times one goes to 2^13 .. 2^14, so that probabilities down to 2^-27 of it stay
+    // normal numbers
+    const int up = f16 && top > 0.f && isfinite(top) ? min(max(13 - ilogbf(top), -100), 100) : 0;
+    meta->up = exp2f((float)up);
+    meta->down = exp2f((float)-up);
+    const uint64_t all = (vocab + MMA_N - 1) / MMA_N * MMA_N;
+    meta->kept = n * all <= l_elems ? (uint32_t)all : 0;
+}
+
 // ---- the scored rows, in order, and what the other kernels need to know of them. One block: a warp takes a contiguous run of rows,
 // 32 at a time; a scan over the warps' counts places them.
 __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ targets, const float* __restrict__ mask, uint32_t rows,
@@ -117,16 +132,7 @@ __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ 
             total += wsum[k];
             top = fmaxf(top, wtop[k]);
         }
-        meta->n = n;
-        meta->done = 0;
-        meta->weight_sum = total;
-        // f16 holds 2^-24 .. 65504: the largest weight times one goes to 2^13 .. 2^14, so that probabilities down to 2^-27 of it
-        // stay normal numbers
-        const int up = f16 && top > 0.f && isfinite(top) ? min(max(13 - ilogbf(top), -100), 100) : 0;
-        meta->up = exp2f((float)up);
-        meta->down = exp2f((float)-up);
-        const uint64_t all = (vocab + MMA_N - 1) / MMA_N * MMA_N;
-        meta->kept = n * all <= l_elems ? (uint32_t)all : 0;
+        describe(meta, n, total, top, f16, vocab, l_elems);
     }
     for (uint32_t t = 0; t < turns; t++) {
         const uint64_t i = begin + (uint64_t)t * 32 + lane;
@@ -152,6 +158,11 @@ __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pi
     after_previous();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, row = blockIdx.x * FINISH_ROWS + lane;
     const int32_t slot = row < rows ? slot_of[row] : -1;
+    // the row that the warp ends, asked for now
+    const uint32_t own = blockIdx.x * FINISH_ROWS + warp;
+    const int32_t at = own < rows ? slot_of[own] : -1;
+    const float own_logit = at >= 0 ? target_logit[at] : 0.f;
+    const double own_weight = at >= 0 ? (mask ? (double)mask[own] : 1.0) : 0.0;
     float2 s = make_float2(-INFINITY, 0.f);
     if (slot >= 0) {
         for (uint32_t t = warp; t < tiles; t += 4 * 32) {
@@ -168,16 +179,13 @@ __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pi
     s = share[lane][warp];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) s = join_stats(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
-    const uint32_t own = blockIdx.x * FINISH_ROWS + warp;
     if (lane == 0) {
-        mine[warp] = 0.0;
+        const float loss = at >= 0 ? logf(s.y) - (own_logit - s.x) : 0.f;
         if (own < rows) {
-            const int32_t at = slot_of[own];
-            const float loss = at >= 0 ? logf(s.y) - (target_logit[at] - s.x) : 0.f;
             stats[own] = at >= 0 ? s : make_float2(0.f, 0.f);
             if (row_loss) row_loss[own] = loss;
-            if (at >= 0) mine[warp] = (mask ? (double)mask[own] : 1.0) * (double)loss;
         }
+        mine[warp] = at >= 0 ? own_weight * (double)loss : 0.0;
     }
     if (!totals) return;
     __syncthreads();
@@ -185,6 +193,13 @@ __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pi
     double sum = mine[lane];
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (gridDim.x == 1) {
+        if (lane == 0) {
+            totals[0] = (float)sum;
+            totals[1] = (float)meta->weight_sum;
+        }
+        return;
+    }
     if (lane == 0) {
         loss_part[blockIdx.x] = sum;
         __threadfence();
@@ -229,6 +244,23 @@ __device__ __forceinline__ void pack_piece(const float (&v)[8], S* out, uint64_t
         o.store(out + p * part_stride);
     }
 }
+template <typename T, typename S>
+__device__ __forceinline__ void pack_at(const T* src, bool here, uint32_t col, uint32_t hidden, int wide, S* out, uint64_t part_stride, int parts) {
+    float v[8];
+    if (!here) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = 0.f;
+    } else if (wide && col + 8 <= hidden) {
+        Vec<T, 8> x;
+        x.load(src + col);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = to_f32<T>(x.e[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = col + j < hidden ? to_f32<T>(src[col + j]) : 0.f;
+    }
+    pack_piece<T, S>(v, out, part_stride, parts);
+}
 // rows: the packed rows (row_of null: row i is source row i, `rows` of them; else the scored ones and zeros to the next multiple of 256)
 template <typename T, typename S>
 __global__ void __launch_bounds__(256) k_head_pack(const T* __restrict__ src, uint64_t stride, uint32_t hidden, uint32_t pitch, uint64_t rows,
@@ -237,27 +269,73 @@ __global__ void __launch_bounds__(256) k_head_pack(const T* __restrict__ src, ui
     let_next();
     after_previous();
     const uint32_t n = row_of ? meta->n : (uint32_t)rows, per = pitch / 8;
-    const uint64_t total = (row_of ? (uint64_t)(n + MMA_M - 1) / MMA_M * MMA_M : rows) * per;
+    const uint64_t total = (row_of ? (uint64_t)tiles_of(n, MMA_M) * MMA_M : rows) * per;
     for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
         const uint64_t slot = e / per;
         const uint32_t col = (uint32_t)(e - slot * per) * 8;
-        float v[8];
-        if (slot >= n) {
+        const bool here = slot < n;
+        pack_at<T, S>(here ? src + (row_of ? (uint64_t)row_of[slot] : slot) * stride : nullptr, here, col, hidden, wide, out + slot * pitch + col,
+                      part_stride, parts);
+    }
+}
+// Up to LISTED rows: every block lists the scored ones for itself (a row a thread) and packs its share; the first leaves the list for
+// the other kernels. One launch instead of two.
+constexpr uint32_t LISTED = 1024;
+template <typename T, typename S>
+__global__ void __launch_bounds__(LISTED) k_head_list_pack(const int64_t* __restrict__ targets, const float* __restrict__ mask, uint32_t rows, uint64_t vocab,
+                                                           int32_t* row_of, int32_t* slot_of, HeadMeta* meta, int f16, uint64_t l_elems,
+                                                           const T* __restrict__ src, uint64_t stride, uint32_t hidden, uint32_t pitch, S* out,
+                                                           uint64_t part_stride, int parts, int wide) {
+    __shared__ uint32_t bits_of[32];
+    __shared__ uint16_t list[LISTED];
+    __shared__ double wsum[32];
+    __shared__ float wtop[32];
+    let_next();
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, i = threadIdx.x;
+    const float w = i < rows && (uint64_t)targets[i] < vocab ? (mask ? mask[i] : 1.f) : 0.f;
+    const uint32_t bits = __ballot_sync(0xffffffffu, w != 0.f);
+    double sum = (double)w;
+    float top = fabsf(w);
+    if (blockIdx.x == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = 0.f;
-        } else {
-            const T* from = src + (row_of ? (uint64_t)row_of[slot] : slot) * stride + col;
-            if (wide && col + 8 <= hidden) {
-                Vec<T, 8> x;
-                x.load(from);
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = to_f32<T>(x.e[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = col + j < hidden ? to_f32<T>(from[j]) : 0.f;
-            }
+        for (int o = 16; o; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         }
-        pack_piece<T, S>(v, out + slot * pitch + col, part_stride, parts);
+    }
+    if (lane == 0) {
+        bits_of[warp] = bits;
+        wsum[warp] = sum;
+        wtop[warp] = top;
+    }
+    __syncthreads();
+    uint32_t at = 0, n = 0;
+    for (uint32_t k = 0; k < 32; k++) {
+        const uint32_t c = __popc(bits_of[k]);
+        at += k < warp ? c : 0;
+        n += c;
+    }
+    const bool yes = bits >> lane & 1;
+    at += __popc(bits & ((1u << lane) - 1));
+    if (yes) list[at] = (uint16_t)i;
+    if (blockIdx.x == 0) {
+        if (i < rows) slot_of[i] = yes ? (int32_t)at : -1;
+        if (yes) row_of[at] = (int32_t)i;
+        if (i == 0) {
+            double total = 0.0;
+            for (int k = 0; k < 32; k++) {
+                total += wsum[k];
+                top = fmaxf(top, wtop[k]);
+            }
+            describe(meta, n, total, top, f16, vocab, l_elems);
+        }
+    }
+    __syncthreads();
+    const uint32_t per = pitch / 8, end = tiles_of(n, MMA_M) * MMA_M * per;
+    for (uint32_t e = blockIdx.x * LISTED + i; e < end; e += gridDim.x * LISTED) {
+        const uint32_t slot = e / per, col = (e - slot * per) * 8;
+        const bool here = slot < n;
+        pack_at<T, S>(here ? src + (uint64_t)list[slot] * stride : nullptr, here, col, hidden, wide, out + (uint64_t)slot * pitch + col, part_stride, parts);
     }
 }
 
@@ -302,8 +380,6 @@ struct ProductArgs {
     uint8_t pair_a[6], pair_b[6];
     int32_t* expired;
 };
-
-__host__ __device__ inline uint32_t tiles_of(uint64_t n, uint32_t of) { return (uint32_t)((n + of - 1) / of); }
 
 // How D_HIDDEN's tiles are shared among the pairs of SMs: rounds of whole tiles while there are enough for every pair; the rest,
 // fewer than the pairs, are cut in K into `shares` each, as many as fill one to four more rounds best. The pairs of a round walk K in
@@ -753,6 +829,7 @@ __global__ void __launch_bounds__(256) k_head_grad_kept(const ProductArgs a) {
 }
 
 // ---- d_hidden: the scored rows' sums, their shares in order, times the scale, rounded; zeros for the others
+// N columns a thread: four, so that a small d_hidden spreads over the SMs, or one where rows are not aligned
 template <typename T, int N>
 __global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t hidden, uint32_t dx_pitch, uint64_t piece, uint32_t pairs,
                                                        const int32_t* __restrict__ slot_of, const float* __restrict__ dx,
@@ -774,14 +851,20 @@ __global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t h
             sum.load(dx + (uint64_t)slot * dx_pitch + col);
             const uint32_t tile = slot / MMA_M * nt + col / MMA_N;
             const float* from = dx_shares + ((uint64_t)tile - split.whole) * (MMA_M * MMA_N) + slot % MMA_M * MMA_N + col % MMA_N;
-            if (tile >= split.whole)
-#pragma unroll 4
-                for (uint32_t k = 1; k < split.shares; k++) {
-                    Vec<float, N> v;
-                    v.load(from + (uint64_t)(k - 1) * split.rest * (MMA_M * MMA_N));
+            const uint32_t shares = tile >= split.whole ? split.shares : 1;
+            constexpr int AHEAD = 8;
+            for (uint32_t k = 1; k < shares; k += AHEAD) {
+                Vec<float, N> v[AHEAD];
 #pragma unroll
-                    for (int j = 0; j < N; j++) sum.e[j] += v.e[j];
-                }
+                for (int a = 0; a < AHEAD; a++)
+                    if (k + a < shares) v[a].load(from + (uint64_t)(k + a - 1) * split.rest * (MMA_M * MMA_N));
+#pragma unroll
+                for (int a = 0; a < AHEAD; a++)
+                    if (k + a < shares) {
+#pragma unroll
+                        for (int j = 0; j < N; j++) sum.e[j] += v[a].e[j];
+                    }
+            }
         }
         Vec<T, N> o;
 #pragma unroll
@@ -902,15 +985,19 @@ struct Products {
         constexpr bool F32 = sizeof(T) == 4, BF16 = std::is_same<S, __nv_bfloat16>::value;
         const size_t es = sizeof(T);
         const unsigned many = (unsigned)h->clusters * 2 * 8;  // blocks of the elementwise kernels
-        k_head_rows<<<1, 1024, 0, s>>>(b.targets, b.loss_mask, (uint32_t)b.rows, d.vocab, h->row_of, h->slot_of, h->meta, !BF16,
-                                    want_loss && gr ? h->l_elems : 0);
-        const uint64_t x_part = h->cap * h->pitch, w_part = d.vocab * h->pitch;
+        const uint64_t x_part = h->cap * h->pitch, w_part = d.vocab * h->pitch, l_elems = want_loss && gr ? h->l_elems : 0;
         const bool x_wide = !misaligned(b.hidden, 16) && b.hidden_stride * es % 16 == 0;
-        if (b.rows) {
-            const uint64_t work = (b.rows + MMA_M) * (h->pitch / 8);
-            OXZ_CUDA(launch_after(true, k_head_pack<T, S>, (unsigned)std::min<uint64_t>((work + 255) / 256, many), 256, 0, s,
-                                  static_cast<const T*>(b.hidden), b.hidden_stride, (uint32_t)d.hidden, h->pitch, b.rows, h->row_of, h->meta,
-                                  static_cast<S*>(h->x), x_part, h->parts, x_wide));
+        const T* x = static_cast<const T*>(b.hidden);
+        const uint64_t pack = (b.rows + MMA_M) * (h->pitch / 8);  // 16-byte pieces at most
+        if (b.rows <= LISTED) {
+            OXZ_CUDA(launch_after(false, k_head_list_pack<T, S>, (unsigned)std::min<uint64_t>((pack + LISTED - 1) / LISTED, h->sms), LISTED, 0, s, b.targets,
+                                  b.loss_mask, (uint32_t)b.rows, d.vocab, h->row_of, h->slot_of, h->meta, !BF16, l_elems, x, b.hidden_stride,
+                                  (uint32_t)d.hidden, h->pitch, static_cast<S*>(h->x), x_part, h->parts, x_wide));
+        } else {
+            OXZ_CUDA(launch_after(false, k_head_rows, 1, 1024, 0, s, b.targets, b.loss_mask, (uint32_t)b.rows, d.vocab, h->row_of, h->slot_of, h->meta, !BF16,
+                                  l_elems));
+            OXZ_CUDA(launch_after(true, k_head_pack<T, S>, (unsigned)std::min<uint64_t>((pack + 255) / 256, many), 256, 0, s, x, b.hidden_stride,
+                                  (uint32_t)d.hidden, h->pitch, b.rows, h->row_of, h->meta, static_cast<S*>(h->x), x_part, h->parts, x_wide));
         }
         if (h->w)
             OXZ_CUDA(launch_after(true, k_head_pack<T, S>, many, 256, 0, s, static_cast<const T*>(b.weight), d.hidden, (uint32_t)d.hidden, h->pitch, d.vocab,
@@ -990,8 +1077,8 @@ struct Products {
             a.beside = 0;
         }
         if (gr->d_hidden && b.rows) {
-            constexpr int N = 16 / (int)sizeof(T);
-            const bool wide = !misaligned(gr->d_hidden, 16) && gr->d_hidden_stride * es % 16 == 0 && d.hidden % N == 0;
+            constexpr int N = 4;
+            const bool wide = !misaligned(gr->d_hidden, N * es) && gr->d_hidden_stride % N == 0 && d.hidden % N == 0;
             auto k = wide ? k_head_d_hidden<T, N> : k_head_d_hidden<T, 1>;
             OXZ_CUDA(launch_after(true, k, (unsigned)std::min<uint64_t>((b.rows * d.hidden / (wide ? N : 1) + 255) / 256, many), 256, 0, s, (uint32_t)b.rows,
                                   (uint32_t)d.hidden, h->dx_pitch, h->piece, (uint32_t)h->clusters, h->slot_of, h->dx, h->dx_shares, h->meta, a.scale,
