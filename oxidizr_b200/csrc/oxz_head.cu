@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(LISTED) k_head_list_pack(const int64_t* __rest
 // Operands come as K runs in memory: G and X are K-major in the first three, W in the first two; the others are read with K along
 // the lines of their tiles. Values of more than 16 bits come in parts; a product of such operands is the sum over `pairs` of parts.
 enum Product { LOGITS_STATS, LOGITS_GRAD, D_HIDDEN, D_WEIGHT };
-constexpr int STAGES = 6, MMA_THREADS = 320, EPILOGUE_WARPS = 8;
-constexpr uint32_t STAGE_BYTES = 4 * BOX_BYTES, OUT_BYTES = 32 * 128;
+constexpr int STAGES = 5, MMA_THREADS = 320, EPILOGUE_WARPS = 8;
+constexpr uint32_t STAGE_BYTES = 4 * BOX_BYTES, OUT_BYTES = 2 * 32 * 128;
 constexpr uint32_t MMA_SMEM = STAGES * STAGE_BYTES + EPILOGUE_WARPS * OUT_BYTES + 1024 + 256;
 
 struct ProductArgs {
@@ -613,19 +613,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     } else if (warp >= 2) {
         // ---- the finished tiles: a warp reads the 32 lanes of its quarter, half of the columns each
         const uint32_t quarter = warp & 3, side = (warp - 2) / 4, row_in = quarter * 32 + lane;
-        const uint32_t out_at = base + STAGES * STAGE_BYTES + (warp - 2) * OUT_BYTES;
+        const uint32_t out_base = base + STAGES * STAGE_BYTES + (warp - 2) * OUT_BYTES;
+        uint32_t out_now = 0;  // which of the warp's two buffers the last box left from
         const float scale = P == D_WEIGHT ? a.scale * a.meta->down : 1.f;
         const uint32_t kept = P == LOGITS_STATS && a.keep ? a.meta->kept : 0;
         uint32_t round = 0;
         bool ok = true;
+        // what a tile's rows need is fetched a tile ahead
+        RowOfG next_row;
+        auto fetch_row = [&](uint32_t t) {
+            if (!LOGITS || t >= items) return;
+            const uint32_t i = (t % mt) * MMA_M + rank * 128 + row_in;
+            if (i >= M) next_row = RowOfG();
+            else if (P == LOGITS_GRAD) next_row = RowOfG(a, i);
+            else next_row.target = (uint32_t)a.targets[a.row_of[i]];
+        };
+        fetch_row(blockIdx.x / 2);
         for (uint32_t t = blockIdx.x / 2; t < items && ok; t += pairs) {
             const Tile c = tile_at(t);
             const uint32_t i = c.m0 + rank * 128 + row_in;
             const bool in = i < M;
-            // what the row needs is fetched while the tile is still being made
-            RowOfG row;
-            if (P == LOGITS_GRAD && in) row = RowOfG(a, i);
-            if (P == LOGITS_STATS && in) row.target = (uint32_t)a.targets[a.row_of[i]];
+            const RowOfG row = next_row;
+            fetch_row(t + pairs);
             // column of the tile that the target has; far outside it where another tile has it
             const uint32_t target = LOGITS && in ? row.target - a.first - c.n0 : 0xffffffffu;
             const ExpFrom<F32> ex(row.m);
@@ -633,38 +642,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             const uint32_t from = side * 128, to = min(from + 128, P == LOGITS_GRAD ? (valid + 63) & ~63u : valid);
             // the tile's 128 columns of this warp leave tensor memory at once, which frees the accumulator for the next tile
             float acc[4][32];
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-#pragma unroll
-                for (int j = 0; j < 32; j++) acc[q][j] = 0.f;
-            for (uint32_t k1 = 0; k1 < c.steps; k1 += RUN ? RUN : c.steps, round++) {
-                const uint32_t buf = round & 1;
-                ok = __all_sync(0xffffffffu, mbar_wait(done(buf), (round >> 1) & 1, ws));
-                if (!ok) break;
+            auto run_done = [&]() {  // a run is in the accumulator buffer
+                ok = __all_sync(0xffffffffu, mbar_wait(done(round & 1), (round >> 1) & 1, ws));
                 fence_after_sync();
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    if (from + 32 * q >= c.width) break;
-#pragma unroll
-                    for (int e = 0; e < 32; e += 16) {
-                        uint32_t x[16];
-                        tmem_load16(tmem + buf * 256 + from + 32 * q + e + (quarter << 21), x);
-                        tmem_wait(x);
-#pragma unroll
-                        for (int j = 0; j < 16; j++) acc[q][e + j] = RUN ? acc[q][e + j] + __uint_as_float(x[j]) : __uint_as_float(x[j]);
-                    }
-                }
+                return tmem + (round & 1) * 256 + from + (quarter << 21);
+            };
+            auto run_taken = [&]() {
                 fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(peer_smem(taken(buf), 0));
+                if (lane == 0) mbar_arrive_peer(peer_smem(taken(round & 1), 0));
+                round++;
+            };
+            if (LOGITS || c.steps) {
+                // columns past the tile's width hold what an earlier tile left, and are not used
+                const uint32_t at = run_done();
+                if (!ok) break;
+#pragma unroll
+                for (int q = 0; q < 4; q++) tmem_load(at + 32 * q, acc[q]);
+                tmem_wait();
+#pragma unroll
+                for (int q = 0; q < 4; q++) arrived(acc[q]);
+                run_taken();
+            } else {  // no scored row: a sum of nothing
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int j = 0; j < 32; j++) acc[q][j] = 0.f;
             }
-            if (!ok) break;
+            if constexpr (RUN > 0) {
+                for (uint32_t k1 = RUN; k1 < c.steps; k1 += RUN) {
+                    const uint32_t at = run_done();
+                    if (!ok) break;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        float x[16];
+                        tmem_load(at + 16 * e, x);
+                        tmem_wait();
+                        arrived(x);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) acc[e / 2][16 * (e & 1) + j] += x[j];
+                    }
+                    run_taken();
+                }
+                if (!ok) break;
+            }
             const int32_t line = (int32_t)(c.m0 + rank * 128 + quarter * 32);  // the warp's first row
             // 128 bytes of each of the warp's rows go out as one box: 16-byte pieces in the order of the 128-byte swizzle, no two lanes of
             // a quarter warp in one bank
             auto box = [&](const CUtensorMap& map, int32_t x, int32_t y, int32_t z, const uint32_t (&w)[32], bool add) {
-                if (lane == 0) store_read();
+                if (lane == 0) store_read<1>();
                 __syncwarp();
+                out_now ^= OUT_BYTES / 2;
+                const uint32_t out_at = out_base + out_now;
 #pragma unroll
                 for (int p = 0; p < 8; p++) st_shared16(out_at + lane * 128 + ((p ^ (lane & 7)) << 4), w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
                 store_fence();
@@ -679,20 +708,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                 for (int j = 0; j < 32; j++) w[j] = __float_as_uint(acc[q][j]);
             };
             if constexpr (P == LOGITS_STATS) {
-                float2 run_stats = make_float2(-INFINITY, 0.f);
+                float m8[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) m8[k] = -INFINITY;
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const uint32_t c0 = from + 32 * q;
-                    if (c0 >= to) break;
-                    if (kept) {
+                    if (kept && c0 < to) {
                         uint32_t w[32];
                         words(q, w);
                         box(map_out, (int32_t)(c.n0 + c0), line, 0, w, false);
-                    }
-                    if (c0 + 32 > valid) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (c0 + j >= valid) acc[q][j] = -INFINITY;  // no word of the vocabulary
                     }
                     if (target - c0 < 32) {
                         float tl = 0.f;
@@ -700,16 +725,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                         for (int j = 0; j < 32; j++) tl = target - c0 == (uint32_t)j ? acc[q][j] : tl;
                         a.target_logit[i] = tl;
                     }
-                    float m = run_stats.x;
+                    if (c0 + 32 > valid) {
 #pragma unroll
-                    for (int j = 0; j < 32; j++) m = fmaxf(m, acc[q][j]);
-                    const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf yet: exp(-inf - 0) is the zero it should be
-                    const ExpFrom<F32> e(ref);
-                    float part[4] = {run_stats.x == -INFINITY ? run_stats.y : run_stats.y * e(run_stats.x), 0.f, 0.f, 0.f};
+                        for (int j = 0; j < 32; j++)
+                            if (c0 + j >= valid) acc[q][j] = -INFINITY;  // no word of the vocabulary
+                    }
 #pragma unroll
-                    for (int j = 0; j < 32; j++) part[j & 3] += e(acc[q][j]);
-                    run_stats = make_float2(m, (part[0] + part[1]) + (part[2] + part[3]));
+                    for (int j = 0; j < 32; j++) m8[j & 7] = fmaxf(m8[j & 7], acc[q][j]);
                 }
+                // eight sums side by side: the chains, not the instructions, are what a tile waits for
+                const float m = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+                const ExpFrom<F32> e(m == -INFINITY ? 0.f : m);  // nothing above -inf: exp(-inf - 0) is the zero it should be
+                float s8[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) s8[k] = 0.f;
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int j = 0; j < 32; j++) s8[j & 7] += e(acc[q][j]);
+                const float2 run_stats = make_float2(m, ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7])));
                 if (in) a.part[(uint64_t)(2 * (c.n0 / MMA_N) + side) * a.pitch + i] = run_stats;
             } else if constexpr (P == LOGITS_GRAD) {
 #pragma unroll
@@ -764,7 +798,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 32; j++) {
-                        const uint32_t at = out_at + lane * 128 + ((j ^ lane) << 2);
+                        const uint32_t at = out_base + lane * 128 + ((j ^ lane) << 2);
                         asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(acc[q][j] * scale) : "memory");
                     }
                     __syncwarp();
@@ -773,7 +807,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
 #pragma unroll 8
                     for (uint32_t k = 0; k < rows; k++, out += a.hidden) {
                         float v;
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(out_at + k * 128 + ((lane ^ k) << 2)) : "memory");
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(out_base + k * 128 + ((lane ^ k) << 2)) : "memory");
                         if (here) *out = from_f32<G>(a.accumulate ? to_f32<G>(*out) + v : v);
                     }
                 }
