@@ -536,8 +536,8 @@ int32_t oxz_loader_next_batch_async(oxz_loader* loader, void* stream, int64_t** 
  *   lookup     out[i] = scale * table[ids[i]]
  *   gradient   d_table[v] = scale * sum over i with ids[i] = v of d_out[i]      (+ what d_table held, when accumulating)
  *
- * Sums run in f32, in the order of the tokens, whatever the launch: equal inputs give equal bits. Each result is rounded once
- * to its type. An id outside [0, vocab) reads as a row of zeros and receives no gradient.
+ * Sums run in f32, in an order that the tokens alone decide: equal inputs give equal bits. Each result is rounded once to its
+ * type. An id outside [0, vocab) reads as a row of zeros and receives no gradient.
  * The handle holds the workspace of the gradient. It is used by one thread at a time; calls on different streams are ordered by
  * the handle, but graphs captured from its gradient calls share the workspace, so their replays must not overlap each other or
  * other gradient calls of the handle. No call allocates, synchronises or copies to the host. */
@@ -582,17 +582,22 @@ int32_t oxz_embed_grads_async(oxz_embed* embed, const int64_t* ids, uint64_t n, 
  * A row is scored when its loss_mask is not zero and its target lies in [0, vocab). Nothing of another row is used - not its
  * hidden state either, which may hold anything - and it gets loss 0, statistics 0 and a gradient of zeros.
  * Products are summed in f32 and softmax statistics kept in f32. g is rounded to dtype before it is multiplied (f16: scaled by a
- * power of two into its range first); d_hidden and d_weight are rounded once. There are no atomics: equal inputs give equal bits.
+ * power of two into its range first; with an f32 d_weight, for that gradient, to 24 bits; with up to 16 rows to twice the digits);
+ * d_hidden and d_weight are rounded once. The order of every sum is fixed: equal inputs give equal bits. 16-bit weights with hidden
+ * a multiple of 8 are read where they lie; others, and f32 ones, are first copied into the workspace in 16-bit parts.
+ * d_hidden may be the memory of hidden itself.
  * The handle holds the workspace. It is used by one thread at a time; calls on different streams are ordered by the handle, but
  * graphs captured from its calls share the workspace, so their replays must not overlap each other or other calls of the
  * handle. No call allocates, synchronises or copies to the host. OXZ_ERR_TIMEOUT: a bounded wait inside a kernel of an earlier call
  * ran out, its results are not valid, and the handle serves no further call. */
 typedef struct oxz_head oxz_head;
 typedef struct oxz_head_desc {
-    uint64_t max_rows;     /* the most tokens of one call, below 2^31 */
-    uint64_t hidden;       /* elements of a row */
-    uint64_t vocab;        /* rows of the weight, below 2^31 */
-    uint64_t piece_bytes;  /* the most workspace for one piece's gradient of the logits; 0 = 512 MiB */
+    uint64_t max_rows;     /* the most tokens of one call, at most 2^30 */
+    uint64_t hidden;       /* elements of a row, at most 2^20 */
+    uint64_t vocab;        /* rows of the weight, at most 2^30 */
+    uint64_t piece_bytes;  /* the most workspace for pieces; 0 = 2 GiB. A third holds one piece's gradient of the logits; the rest,
+                              where hidden is large enough for that to pay and all logits of a batch fit it in f32, the logits
+                              between the losses and the gradients of one call, which else are formed again */
     int32_t dtype;         /* oxz_dtype of hidden, weight and d_hidden */
     int32_t grad_dtype;    /* oxz_dtype of d_weight: dtype or OXZ_F32 */
     int32_t device;        /* CUDA device ordinal */

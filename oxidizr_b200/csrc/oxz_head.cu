@@ -419,6 +419,15 @@ template <bool EXACT> struct ExpFrom {
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(x, LOG2E, -m)));
         return r;
     }
+    // of two, the same bits as of each
+    __device__ __forceinline__ float2 operator()(float2 x) const {
+        if constexpr (EXACT) return make_float2(expf(x.x - m), expf(x.y - m));
+        const float2 t = fma2(x, make_float2(LOG2E, LOG2E), make_float2(-m, -m));
+        float2 r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(t.x));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(t.y));
+        return r;
+    }
 };
 
 // G from 32 logits of a row: weight * up / s * (exp(l - m) - [v = t] s). `target`, `valid`: column of the target, columns that exist,
@@ -432,7 +441,11 @@ __device__ __forceinline__ void logits_to_g(float (&x)[32], const ExpFrom<EXACT>
         hit = (ex(hit) - s) * factor;
     }
 #pragma unroll
-    for (int j = 0; j < 32; j++) x[j] = ex(x[j]) * factor;
+    for (int j = 0; j < 32; j += 2) {
+        const float2 g = mul2(ex(make_float2(x[j], x[j + 1])), make_float2(factor, factor));
+        x[j] = g.x;
+        x[j + 1] = g.y;
+    }
     if (target < 32) {
 #pragma unroll
         for (int j = 0; j < 32; j++) x[j] = target == (uint32_t)j ? hit : x[j];
@@ -736,14 +749,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                 // eight sums side by side: the chains, not the instructions, are what a tile waits for
                 const float m = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
                 const ExpFrom<F32> e(m == -INFINITY ? 0.f : m);  // nothing above -inf: exp(-inf - 0) is the zero it should be
-                float s8[8];
+                float2 s4[4];
 #pragma unroll
-                for (int k = 0; k < 8; k++) s8[k] = 0.f;
+                for (int k = 0; k < 4; k++) s4[k] = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int q = 0; q < 4; q++)
 #pragma unroll
-                    for (int j = 0; j < 32; j++) s8[j & 7] += e(acc[q][j]);
-                const float2 run_stats = make_float2(m, ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7])));
+                    for (int j = 0; j < 32; j += 2) s4[j / 2 & 3] = add2(s4[j / 2 & 3], e(make_float2(acc[q][j], acc[q][j + 1])));
+                const float2 s1 = add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])), run_stats = make_float2(m, s1.x + s1.y);
                 if (in) a.part[(uint64_t)(2 * (c.n0 / MMA_N) + side) * a.pitch + i] = run_stats;
             } else if constexpr (P == LOGITS_GRAD) {
 #pragma unroll
@@ -1185,10 +1198,10 @@ int32_t oxz_head_create(const oxz_head_desc* desc, oxz_head** out) {
         if (!desc || !out) return fail(OXZ_ERR_INVALID, "oxz_head_create: null argument");
         *out = nullptr;
         const oxz_head_desc& d = *desc;
-        if (d.max_rows == 0 || d.max_rows > 0x7fffffffull)
-            return fail(OXZ_ERR_INVALID, "oxz_head_create: max_rows %llu is outside 1..2^31-1", (unsigned long long)d.max_rows);
-        if (d.vocab == 0 || d.vocab > 0x7fffffffull)
-            return fail(OXZ_ERR_INVALID, "oxz_head_create: vocab %llu is outside 1..2^31-1", (unsigned long long)d.vocab);
+        if (d.max_rows == 0 || d.max_rows > (1ull << 30))
+            return fail(OXZ_ERR_INVALID, "oxz_head_create: max_rows %llu is outside 1..2^30", (unsigned long long)d.max_rows);
+        if (d.vocab == 0 || d.vocab > (1ull << 30))
+            return fail(OXZ_ERR_INVALID, "oxz_head_create: vocab %llu is outside 1..2^30", (unsigned long long)d.vocab);
         if (d.hidden == 0 || d.hidden > (1u << 20))
             return fail(OXZ_ERR_INVALID, "oxz_head_create: hidden %llu is outside 1..2^20", (unsigned long long)d.hidden);
         if (d.dtype != OXZ_F32 && d.dtype != OXZ_BF16 && d.dtype != OXZ_F16)

@@ -495,7 +495,7 @@ def _ptr(address: int | None):
 class TokenEmbedding:
     """The token embedding and its gradient (embed_tokens, [vocab, hidden]): ``out[i] = scale * table[ids[i]]`` and
     ``d_table[v] = scale * sum of d_out[i] over the tokens i with ids[i] = v``. All arguments are device addresses; sums run
-    in f32 in the order of the tokens, so equal inputs give equal bits. An id outside the table reads as zeros and receives
+    in f32 in an order that the tokens alone decide, so equal inputs give equal bits. An id outside the table reads as zeros and receives
     no gradient."""
 
     def __init__(self, vocab: int, hidden: int, max_tokens: int, dtype: int = BF16, grad_dtype: int | None = None,

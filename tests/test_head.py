@@ -391,3 +391,63 @@ def test_one_handle_serves_batches_of_every_size():
         torch.cuda.synchronize()
         assert bool(torch.isnan(q["d_weight"]).all())
     h.destroy()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, grad", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("bf16", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("rows, hidden, vocab, mask, gap", [
+    (1, 2056, 700, None, 0), (4, 64, 3000, None, 0), (5, 130, 1111, "half", 6), (8, 128, 257, "weights", 8), (9, 96, 5000, "both", 0), (13, 1500, 900, None, 0),
+    (16, 1024, 2100, "half", 16), (16, 40, 33, None, 0), (16, 16, 1, None, 0), (12, 3, 4100, "weights", 1), (16, 2048, 3, None, 0)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_a_handful_of_rows(dtype, grad, rows, hidden, vocab, mask, gap, accumulate):
+    """Up to 16 rows, on and off 16-byte bounds, short rows that several threads share, one word, more rows than words."""
+    import torch
+    rng = np.random.default_rng(8)
+    before = torch.from_numpy(rng.standard_normal((vocab, hidden)) * 0.01).cuda().to(torch_type(grad)) if accumulate else None
+    pr = Problem(dtype, rows, hidden, vocab, mask, seed=rows, grad=grad, gap=gap).solve(scale=0.5, before=before.double().cpu().numpy() if accumulate else None)
+    h = ox.LossHead(vocab, hidden, rows, dtype=NAMES[dtype], grad_dtype=NAMES[grad])
+    o = pr.outputs(before=before)
+    h.loss_and_grads(**pr.batch(), **ptrs(o), grad_scale=0.5, accumulate=accumulate)
+    torch.cuda.synchronize()
+    pr.check(o, o)
+    h.destroy()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, grad", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("rows, hidden, vocab, piece_bytes", [(40, 1024, 1500, 0), (600, 1040, 2500, 0), (600, 1040, 2500, 4 << 20), (1300, 264, 3000, 5 << 20),
+                                                             (2100, 72, 5000, 0), (1025, 512, 700, 1)])
+def test_many_tiles(dtype, grad, rows, hidden, vocab, piece_bytes):
+    """Several tiles each way: kept logits and logits formed again, d_hidden cut in shares and not, more rows than one block lists."""
+    import torch
+    pr = Problem(dtype, rows, hidden, vocab, "half", seed=rows, grad=grad).solve(scale=0.5)
+    h = ox.LossHead(vocab, hidden, rows, dtype=NAMES[dtype], grad_dtype=NAMES[grad], piece_bytes=piece_bytes)
+    o = pr.outputs()
+    h.loss_and_grads(**pr.batch(), **ptrs(o), grad_scale=0.5)
+    torch.cuda.synchronize()
+    pr.check(o, o)
+    q = pr.outputs()
+    h.loss(**pr.batch(), row_loss=q["row_loss"].data_ptr(), row_stats=q["row_stats"].data_ptr(), totals=q["totals"].data_ptr())
+    h.grads(**pr.batch(), row_stats=q["row_stats"].data_ptr(), d_hidden=q["d_hidden"].data_ptr(), d_weight=q["d_weight"].data_ptr(), grad_scale=0.5)
+    torch.cuda.synchronize()
+    for k in o:
+        assert torch.equal(o[k], q[k]), k
+    h.destroy()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [7, 300])
+def test_d_hidden_in_place_of_hidden(rows):
+    import torch
+    pr = Problem("bf16", rows, 136, 500, "half", seed=2).solve()
+    h = ox.LossHead(500, 136, rows, dtype=ox.BF16)
+    o = pr.outputs()
+    h.loss_and_grads(**pr.batch(), **ptrs(o))
+    torch.cuda.synchronize()
+    x = pr.d_x.clone()
+    q = pr.outputs()
+    torch.cuda.synchronize()
+    h.loss_and_grads(**dict(pr.batch(), hidden=x.data_ptr()), **dict(ptrs(q), d_hidden=x.data_ptr()))
+    torch.cuda.synchronize()
+    assert torch.equal(x, o["d_hidden"]) and torch.equal(q["d_weight"], o["d_weight"])
+    h.destroy()
