@@ -582,7 +582,7 @@ int32_t oxz_embed_grads_async(oxz_embed* embed, const int64_t* ids, uint64_t n, 
  * A row is scored when its loss_mask is not zero and its target lies in [0, vocab). Nothing of another row is used - not its
  * hidden state either, which may hold anything - and it gets loss 0, statistics 0 and a gradient of zeros.
  * Products are summed in f32 and softmax statistics kept in f32. g is rounded to dtype before it is multiplied (f16: scaled by a
- * power of two into its range first; with an f32 d_weight, for that gradient, to 24 bits; with up to 16 rows to twice the digits);
+ * power of two into its range first; with an f32 d_weight, for that gradient, to 24 bits; with up to 8 rows to twice the digits or more);
  * d_hidden and d_weight are rounded once. The order of every sum is fixed: equal inputs give equal bits. 16-bit weights with hidden
  * a multiple of 8 are read where they lie; others, and f32 ones, are first copied into the workspace in 16-bit parts.
  * d_hidden may be the memory of hidden itself.

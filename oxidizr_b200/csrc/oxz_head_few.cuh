@@ -535,8 +535,8 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_grads(const FewArgs a, uint
 
 // Gradients of 16-bit operands on 16 bytes, by warp products. A block has 64 x across columns, a warp 64 of them; `along` = 4 / across
 // warps share a stretch of 16 x along words. A stretch's piece of the weight (8 KiB) and its kept logits come by asynchronous copies
-// GRAD_DEPTH stretches ahead; the block turns the logits into G, in two 16-bit parts (2^-16 of it is lost, where one part would
-// leave 2^-9: with few rows nothing averages that out), and each warp multiplies
+// GRAD_DEPTH stretches ahead; the block turns the logits into G - of up to 8 rows in two 16-bit parts, the second in the place of rows
+// 8 .. 15 (2^-16 of it is lost, where one part leaves 2^-9, which so few rows do not average out) - and each warp multiplies
 //   dX[i][h] += sum_v G[v][i] W[v][h]    A = G^T (words along K) and B = W, both through transposing loads
 //   dW[v][h]  = sum_i G[v][i] x[i][h]    A = G as it lies, B = x in registers for good
 // dW's columns are dealt to the product's so that a lane's 16 results of a word are neighbours: 32 bytes written at once.
@@ -547,17 +547,16 @@ __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
 __device__ __forceinline__ void load_matrices_turned(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
-template <typename T, typename G, int R>
-__global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, uint32_t across_log) {
+template <typename T, typename G, int R, int ACROSS_LOG>
+__global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a) {
     extern __shared__ __align__(128) unsigned char raw16[];
-    const uint32_t across = 1u << across_log, along = 4 >> across_log, words = 16 * along;  // of a stretch
+    constexpr uint32_t across_log = ACROSS_LOG, across = 1u << ACROSS_LOG, along = 4 >> ACROSS_LOG, words = 16 * along;  // of a stretch
     constexpr uint32_t PIECE = 8192;
-    constexpr int PARTS = R == 8 ? 1 : 2;  // 8 rows: both parts of G fill one product, the second as rows 8 .. 15
     constexpr bool SCALED = __is_same(T, __nv_bfloat16);  // bf16 has f32's range: the scale goes into G
-    const uint32_t l_bytes = words * R * 4;
+    constexpr uint32_t l_bytes = words * R * 4;
     unsigned char* wp = raw16;                                                 // [GRAD_DEPTH][words][64 * across], 16-byte chunks turned by the word
     float* lp = reinterpret_cast<float*>(raw16 + GRAD_DEPTH * PIECE);          // [GRAD_DEPTH][words][R]
-    T* gp = reinterpret_cast<T*>(raw16 + GRAD_DEPTH * (PIECE + l_bytes));      // [2][words][16]
+    T* gp = reinterpret_cast<T*>(raw16 + GRAD_DEPTH * (PIECE + l_bytes));      // [words][16]
     __shared__ float row_m[16], row_f[16], row_s[16];
     __shared__ uint32_t row_t[16];
     let_next();
@@ -638,17 +637,13 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
             const T hi = from_f32<T>(y), lo = from_f32<T>(isfinite(y) ? y - to_f32<T>(hi) : 0.f);
             gp[d * 16 + i] = hi;
             if (R == 8) gp[d * 16 + 8 + i] = lo;
-            else gp[(words + d) * 16 + i] = lo;
         }
         __syncthreads();
         if (col >= a.hidden) continue;
-        uint32_t gt[PARTS][4], gn[PARTS][4];  // G^T and G of the warp's 16 words, both parts
-#pragma unroll
-        for (int p = 0; p < PARTS; p++) {
-            const T* from = gp + (p * words + mine * 16) * 16;
-            load_matrices_turned(gt[p], smem_address(from + ((lane >> 4) * 8 + (lane & 7)) * 16 + ((lane >> 3) & 1) * 8));
-            load_matrices(gn[p], smem_address(from + (((lane >> 3) & 1) * 8 + (lane & 7)) * 16 + (lane >> 4) * 8));
-        }
+        uint32_t gt[4], gn[4];  // G^T and G of the warp's 16 words
+        const T* from = gp + mine * 16 * 16;
+        load_matrices_turned(gt, smem_address(from + ((lane >> 4) * 8 + (lane & 7)) * 16 + ((lane >> 3) & 1) * 8));
+        load_matrices(gn, smem_address(from + (((lane >> 3) & 1) * 8 + (lane & 7)) * 16 + (lane >> 4) * 8));
         if (a.want_dx) {
             const unsigned char* piece = wp + st * PIECE;
             const uint32_t d = mine * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);  // the word this lane points at
@@ -657,11 +652,8 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
                 uint32_t b[4];
                 const uint32_t c = j + (lane >> 4);
                 load_matrices_turned(b, smem_address(piece + d * 128 * across + group * 128 + (((c ^ d) & 7) << 4)));
-#pragma unroll
-                for (int p = PARTS - 1; p >= 0; p--) {
-                    warp_product<T>(dx[j], gt[p], b[0], b[1]);
-                    warp_product<T>(dx[j + 1], gt[p], b[2], b[3]);
-                }
+                warp_product<T>(dx[j], gt, b[0], b[1]);
+                warp_product<T>(dx[j + 1], gt, b[2], b[3]);
             }
         }
         if (dw) {
@@ -669,8 +661,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a, 
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 out[j][0] = out[j][1] = out[j][2] = out[j][3] = 0.f;
-#pragma unroll
-                for (int p = PARTS - 1; p >= 0; p--) warp_product<T>(out[j], gn[p], xb[j][0], xb[j][1]);
+                warp_product<T>(out[j], gn, xb[j][0], xb[j][1]);
             }
             const uint32_t h = col + 16 * q;
 #pragma unroll
@@ -792,14 +783,15 @@ int32_t few_run_rows(FewArgs a, bool wide, bool out_wide, bool grads, int sms, c
     if (!grads) return OXZ_OK;
     uint32_t parts = 0;
     bool scaled = false;  // the partial sums carry the scale already
-    if constexpr (sizeof(T) == 2 && R >= 8) {
+    if constexpr (sizeof(T) == 2 && sizeof(G) == 2 && R >= 8) {  // (an f32 d_weight wants G in f32)
         if (wide) {
             const uint32_t across = few_across_16(a.hidden), columns = (a.hidden + 64 * across - 1) / (64 * across), words = 64 / across;
             parts = few_parts_16(a.hidden, a.vocab, sms);
             a.words = ((a.vocab + parts - 1) / parts + words - 1) / words * words;
             parts = (a.vocab + a.words - 1) / a.words;
-            const size_t shared = (size_t)GRAD_DEPTH * (8192 + words * R * 4) + 2 * words * 16 * 2;
-            OXZ_CUDA(launch_after(true, k_few_grads_16<T, G, R>, dim3(parts, columns), GRAD_THREADS, shared, s, a, across == 4 ? 2u : across == 2 ? 1u : 0u));
+            const size_t shared = (size_t)GRAD_DEPTH * (8192 + words * R * 4) + words * 16 * 2;
+            auto k = across == 4 ? k_few_grads_16<T, G, R, 2> : across == 2 ? k_few_grads_16<T, G, R, 1> : k_few_grads_16<T, G, R, 0>;
+            OXZ_CUDA(launch_after(true, k, dim3(parts, columns), GRAD_THREADS, shared, s, a));
             scaled = true;
         }
     }
@@ -830,7 +822,11 @@ int32_t few_prepare_rows() {
     OXZ_CUDA(cudaFuncSetAttribute(k_few_grads<T, G, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_GRAD_BYTES));
     OXZ_CUDA(cudaFuncSetAttribute(k_few_grads<T, G, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_GRAD_BYTES));
     if constexpr (sizeof(T) == 2 && R >= 8) OXZ_CUDA(cudaFuncSetAttribute(k_few_logits_16<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 2048));
-    if constexpr (sizeof(T) == 2 && R >= 8) OXZ_CUDA(cudaFuncSetAttribute(k_few_grads_16<T, G, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 << 10));
+    if constexpr (sizeof(T) == 2 && sizeof(G) == 2 && R >= 8) {
+        OXZ_CUDA(cudaFuncSetAttribute(k_few_grads_16<T, G, R, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 << 10));
+        OXZ_CUDA(cudaFuncSetAttribute(k_few_grads_16<T, G, R, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 << 10));
+        OXZ_CUDA(cudaFuncSetAttribute(k_few_grads_16<T, G, R, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 << 10));
+    }
     return OXZ_OK;
 }
 template <typename T, typename G>
