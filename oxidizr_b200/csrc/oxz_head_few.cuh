@@ -73,15 +73,15 @@ __device__ __forceinline__ void add_logit(float2& s, float l) {
 }
 
 // The block's rows' sets, one per warp and row in `by_warp`, to part[block]; the last block makes the batch's results of all of them.
-template <int R>
-__device__ void few_finish(const FewArgs& a, float2 (&by_warp)[FEW_THREADS / 32][R]) {
+template <int R, int WARPS>
+__device__ void few_finish(const FewArgs& a, float2 (&by_warp)[WARPS][R]) {
     __shared__ uint32_t last;
     __shared__ double sums[2][R];
     __syncthreads();
     if (threadIdx.x < R) {
         float2 s = by_warp[0][threadIdx.x];
 #pragma unroll
-        for (int w = 1; w < FEW_THREADS / 32; w++) s = join_stats(s, by_warp[w][threadIdx.x]);
+        for (int w = 1; w < WARPS; w++) s = join_stats(s, by_warp[w][threadIdx.x]);
         a.part[(uint64_t)blockIdx.x * R + threadIdx.x] = s;
     }
     __threadfence();
@@ -90,11 +90,17 @@ __device__ void few_finish(const FewArgs& a, float2 (&by_warp)[FEW_THREADS / 32]
     __syncthreads();
     if (!last) return;
     __threadfence();
-    // 16 threads a row, each every 16th block
+    // 16 threads a row, each every 16th block, eight at a time
     const uint32_t row = threadIdx.x / 16, k = threadIdx.x & 15;
     float2 s = make_float2(-INFINITY, 0.f);
     if (row < R)
-        for (uint32_t b = k; b < gridDim.x; b += 16) s = join_stats(s, __ldcg(&a.part[(uint64_t)b * R + row]));
+        for (uint32_t b = k; b < gridDim.x; b += 128) {
+            float2 p[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) p[e] = b + 16 * e < gridDim.x ? __ldcg(&a.part[(uint64_t)(b + 16 * e) * R + row]) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) s = join_stats(s, p[e]);
+        }
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) s = join_stats(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
     if (k == 0 && row < R) {
@@ -154,30 +160,30 @@ __device__ __forceinline__ void warp_product(float (&c)[4], const uint32_t (&a)[
 // lane make one warp product and 4..7 the next, which is how their fragments lie, with no exchange. The weight's pieces come by
 // asynchronous copies into a ring of the thread's own, LOGIT_DEPTH steps of 128 elements ahead across the words' bounds; x lies in
 // shared memory. The products of a step are added in f32 (the units cut what they add).
-constexpr int LOGIT_DEPTH = 3, LOGIT_STEP = 128;
+constexpr int LOGIT_DEPTH = 2, LOGIT_STEP = 128, LOGIT_THREADS = 512;
 inline uint32_t few_x_pitch(uint64_t hidden) { return (uint32_t)((hidden + 127) / 128 * 128 + 32); }  // 64 bytes off a multiple of 128: no bank twice
 template <typename T, int R>
-__global__ void __launch_bounds__(FEW_THREADS) k_few_logits_16(const FewArgs a, uint32_t x_pitch) {
+__global__ void __launch_bounds__(LOGIT_THREADS) k_few_logits_16(const FewArgs a, uint32_t x_pitch) {
     static_assert(R == 8 || R == 16, "8 rows a product");
     extern __shared__ __align__(16) unsigned char ring[];  // [LOGIT_DEPTH][8][threads] 16 bytes, then x [R][x_pitch]
-    __shared__ float2 by_warp[FEW_THREADS / 32][R];
+    __shared__ float2 by_warp[LOGIT_THREADS / 32][R];
     let_next();
     after_previous();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
     const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.w);
-    T* xs = reinterpret_cast<T*>(ring + LOGIT_DEPTH * 8 * FEW_THREADS * 16);
-    const uint32_t tiles = (a.vocab + 15) / 16, steps = (a.hidden + LOGIT_STEP - 1) / LOGIT_STEP, stride = gridDim.x * (FEW_THREADS / 32);
-    const uint32_t first = blockIdx.x * (FEW_THREADS / 32) + warp;
+    T* xs = reinterpret_cast<T*>(ring + LOGIT_DEPTH * 8 * LOGIT_THREADS * 16);
+    const uint32_t tiles = (a.vocab + 15) / 16, steps = (a.hidden + LOGIT_STEP - 1) / LOGIT_STEP, stride = gridDim.x * (LOGIT_THREADS / 32);
+    const uint32_t first = warp * gridDim.x + blockIdx.x;  // neighbours on neighbouring SMs
     uint32_t ft = first, fk = 0;  // what is fetched next: tile, step
     auto fetch = [&](uint32_t slot) {
         if (ft < tiles) {
             const T *w0 = w + (uint64_t)min(ft * 16 + r, a.vocab - 1) * a.hidden, *w1 = w + (uint64_t)min(ft * 16 + r + 8, a.vocab - 1) * a.hidden;
-            const uint32_t to = smem_address(ring + (slot * 8 * FEW_THREADS + threadIdx.x) * 16), k = fk * LOGIT_STEP + 8 * q;
+            const uint32_t to = smem_address(ring + (slot * 8 * LOGIT_THREADS + threadIdx.x) * 16), k = fk * LOGIT_STEP + 8 * q;
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 if (k + 32 * e < a.hidden) {
-                    copy_async<16>(to + 2 * e * FEW_THREADS * 16, w0 + k + 32 * e);
-                    copy_async<16>(to + (2 * e + 1) * FEW_THREADS * 16, w1 + k + 32 * e);
+                    copy_async<16>(to + 2 * e * LOGIT_THREADS * 16, w0 + k + 32 * e);
+                    copy_async<16>(to + (2 * e + 1) * LOGIT_THREADS * 16, w1 + k + 32 * e);
                 }
         }
         copies_end();
@@ -188,7 +194,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits_16(const FewArgs a, 
     };
 #pragma unroll
     for (int e = 0; e < LOGIT_DEPTH; e++) fetch(e);
-    for (uint32_t e = threadIdx.x; e < R * (x_pitch / 8); e += FEW_THREADS) {
+    for (uint32_t e = threadIdx.x; e < R * (x_pitch / 8); e += LOGIT_THREADS) {
         const uint32_t i = e / (x_pitch / 8), k = (e - i * (x_pitch / 8)) * 8;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (k < a.hidden && few_scored(a, i)) v = __ldg(reinterpret_cast<const uint4*>(x + (uint64_t)i * a.x_stride + k));
@@ -204,15 +210,15 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits_16(const FewArgs a, 
         float acc[R / 8][4] = {};
         for (uint32_t k0 = 0; k0 < a.hidden; k0 += LOGIT_STEP) {
             copies_but<LOGIT_DEPTH - 1>();
-            const unsigned char* from = ring + (slot * 8 * FEW_THREADS + threadIdx.x) * 16;
+            const unsigned char* from = ring + (slot * 8 * LOGIT_THREADS + threadIdx.x) * 16;
             float c[R / 8][4] = {};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t k = k0 + 32 * e + 8 * q;
                 uint4 p = make_uint4(0, 0, 0, 0), u = p;
                 if (k < a.hidden) {
-                    p = *reinterpret_cast<const uint4*>(from + 2 * e * FEW_THREADS * 16);
-                    u = *reinterpret_cast<const uint4*>(from + (2 * e + 1) * FEW_THREADS * 16);
+                    p = *reinterpret_cast<const uint4*>(from + 2 * e * LOGIT_THREADS * 16);
+                    u = *reinterpret_cast<const uint4*>(from + (2 * e + 1) * LOGIT_THREADS * 16);
                 }
 #pragma unroll
                 for (int j = 0; j < R / 8; j++) {
@@ -253,7 +259,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits_16(const FewArgs a, 
                 s[j][m] = join_stats(s[j][m], make_float2(__shfl_xor_sync(0xffffffffu, s[j][m].x, o), __shfl_xor_sync(0xffffffffu, s[j][m].y, o)));
             if (r == 0) by_warp[warp][8 * j + 2 * q + m] = s[j][m];
         }
-    few_finish<R>(a, by_warp);
+    few_finish(a, by_warp);
 }
 
 // Any type and alignment: a warp takes WORDS words, lanes along hidden; the rows of x are in shared memory as f32. A lane has 16 bytes of
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_logits(const FewArgs a) {
             s[m] = join_stats(s[m], make_float2(__shfl_xor_sync(0xffffffffu, s[m].x, o), __shfl_xor_sync(0xffffffffu, s[m].y, o)));
         if (lane < R / 2) by_warp[warp][2 * lane + m] = s[m];
     }
-    few_finish<R>(a, by_warp);
+    few_finish(a, by_warp);
 }
 
 // Four columns of a row: neighbours (WIDE: 4 elements as one access), or `across` apart.
@@ -631,7 +637,8 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a) 
             const uint32_t d = e / R, i = e % R, v = v0 + d;
             float y = 0.f;
             if (v < end && row_t[i] != 0xffffffffu) {
-                const float p = expf(lp[st * words * R + e] - row_m[i]);
+                float p;  // 2^-22 is ample for 16 bits, twice
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"((lp[st * words * R + e] - row_m[i]) * 1.4426950408889634f));
                 y = (v == row_t[i] ? p - row_s[i] : p) * row_f[i] * up;
             }
             const T hi = from_f32<T>(y), lo = from_f32<T>(isfinite(y) ? y - to_f32<T>(hi) : 0.f);
@@ -676,9 +683,12 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a) 
 #pragma unroll
                     for (int c = 0; c < 8; c++) y[c] = SCALED ? out[4 * e + c / 2][2 * k + (c & 1)] : out[4 * e + c / 2][2 * k + (c & 1)] * out_scale;
                     Vec<G, 8> o;
-                    if (a.accumulate) o.load_coherent(to + 8 * e);
+                    if (a.accumulate) {
+                        o.load_coherent(to + 8 * e);
 #pragma unroll
-                    for (int c = 0; c < 8; c++) o.e[c] = from_f32<G>(a.accumulate ? to_f32<G>(o.e[c]) + y[c] : y[c]);
+                        for (int c = 0; c < 8; c++) y[c] += to_f32<G>(o.e[c]);
+                    }
+                    o.q[0] = make_uint4(pack2<G>(y[0], y[1]), pack2<G>(y[2], y[3]), pack2<G>(y[4], y[5]), pack2<G>(y[6], y[7]));
                     o.store(to + 8 * e);
                 }
             }
@@ -753,7 +763,7 @@ constexpr size_t FEW_SHARED = 227 << 10;   // what a block can have
 inline int few_kernel_rows(uint64_t rows, size_t size, bool wide) { return rows <= 4 && !(size == 2 && wide) ? 4 : rows <= 8 ? 8 : 16; }
 // Shared memory of the logits' kernel: the rows of x and the ring of copies.
 inline size_t few_logit_bytes(int r, uint64_t hidden, size_t size, bool wide) {
-    if (size == 2 && wide) return LOGIT_DEPTH * 8 * FEW_THREADS * 16 + (size_t)r * few_x_pitch(hidden) * 2;
+    if (size == 2 && wide) return LOGIT_DEPTH * 8 * LOGIT_THREADS * 16 + (size_t)r * few_x_pitch(hidden) * 2;
     const uint64_t n = wide ? 16 / size : 1, pitch = (hidden + 32 * n - 1) / (32 * n) * (32 * n);
     return (size_t)r * pitch * 4 + (wide ? (size_t)(r == 4 ? 2 : r == 8 ? 3 : 4) * (64 / r) * FEW_THREADS * 16 : 0);
 }
@@ -767,7 +777,7 @@ int32_t few_logits(const FewArgs& a, bool wide, int sms, cudaStream_t s) {
     auto blocks = [&](uint32_t words) { return std::min<uint32_t>(((a.vocab + words - 1) / words + 7) / 8, sms * fit); };
     if constexpr (sizeof(T) == 2 && R >= 8) {
         if (wide) {
-            OXZ_CUDA(launch_after(false, k_few_logits_16<T, R>, blocks(16), FEW_THREADS, shared, s, a, few_x_pitch(a.hidden)));
+            OXZ_CUDA(launch_after(false, k_few_logits_16<T, R>, std::min<uint32_t>((a.vocab + 15) / 16, sms), LOGIT_THREADS, shared, s, a, few_x_pitch(a.hidden)));
             return OXZ_OK;
         }
     }
@@ -817,11 +827,11 @@ int32_t few_run(const FewArgs& a, bool wide, bool out_wide, bool grads, int sms,
 // The shared memory that the kernels may need, granted once.
 template <typename T, typename G, int R>
 int32_t few_prepare_rows() {
-    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 2048));
-    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 2048));
+    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 4096));
+    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 4096));
     OXZ_CUDA(cudaFuncSetAttribute(k_few_grads<T, G, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_GRAD_BYTES));
     OXZ_CUDA(cudaFuncSetAttribute(k_few_grads<T, G, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_GRAD_BYTES));
-    if constexpr (sizeof(T) == 2 && R >= 8) OXZ_CUDA(cudaFuncSetAttribute(k_few_logits_16<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 2048));
+    if constexpr (sizeof(T) == 2 && R >= 8) OXZ_CUDA(cudaFuncSetAttribute(k_few_logits_16<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 4096));
     if constexpr (sizeof(T) == 2 && sizeof(G) == 2 && R >= 8) {
         OXZ_CUDA(cudaFuncSetAttribute(k_few_grads_16<T, G, R, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 << 10));
         OXZ_CUDA(cudaFuncSetAttribute(k_few_grads_16<T, G, R, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 << 10));
