@@ -50,7 +50,7 @@ struct oxz_head {
     int clusters = 0;                // pairs of SMs the device runs at once
     void* x = nullptr;               // [parts][cap][pitch] packed hidden states
     void* w = nullptr;               // [parts][vocab][pitch] packed weight, where TMA cannot read the caller's
-    void* g = nullptr;               // [g_parts][cap][piece]
+    void* g = nullptr;               // [g_parts][piece / 64][cap][64]: every box that is written or read is one stretch of memory
     float* l = nullptr;              // [scored rows][kept] logits
     uint64_t l_elems = 0, kept_pitch = 0;
     float* dx = nullptr;             // [scored rows][dx_pitch] sums over the pieces
@@ -362,8 +362,7 @@ constexpr uint32_t MMA_SMEM = STAGES * STAGE_BYTES + EPILOGUE_WARPS * OUT_BYTES 
 struct ProductArgs {
     const HeadMeta* meta;
     const int32_t* row_of;
-    uint32_t hidden, first, columns, piece, pitch, g_pitch, dx_pitch, keep;  // the piece [first, first + columns) of the vocabulary
-    uint64_t g_part;
+    uint32_t hidden, first, columns, piece, pitch, cap, g_blocks, dx_pitch, keep;  // the piece [first, first + columns) of the vocabulary
     const int64_t* targets;
     const float* mask;
     const float2* stats;
@@ -583,7 +582,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                         const int32_t bn = (int32_t)(c.n0 + rank * c.half + (LOGITS ? a.first : 0));
                         const int32_t bk = kk + (int32_t)(P == D_HIDDEN ? a.first : 0);
                         for (int i = 0; i < 2; i++) {
-                            if (A_LINES) tma_load_pair(to + i * BOX_BYTES, &map_a, m + 64 * i, kk, za, bar);
+                            if (P == D_WEIGHT) tma_load_pair(to + i * BOX_BYTES, &map_a, 0, kk, za * (int32_t)a.g_blocks + m / 64 + i, bar);
+                            else if (P == D_HIDDEN) tma_load_pair(to + i * BOX_BYTES, &map_a, 0, m + 64 * i, za * (int32_t)a.g_blocks + kk / 64, bar);
                             else tma_load_pair(to + i * BOX_BYTES, &map_a, kk, m + 64 * i, za, bar);
                         }
                         for (int i = 0; i < (int)b_boxes; i++) {
@@ -771,7 +771,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                         uint32_t w[32];
 #pragma unroll
                         for (int j = 0; j < 32; j++) w[j] = next_part<S>(acc[q + j / 16][2 * (j & 15)], acc[q + j / 16][2 * (j & 15) + 1], p + 1 < PARTS);
-                        box(map_out, (int32_t)(c.n0 + c0), line, p, w, false);
+                        box(map_out, 0, line, (int32_t)(p * a.g_blocks + (c.n0 + c0) / 64), w, false);
                     }
                 }
             } else if constexpr (P == D_HIDDEN) {
@@ -863,14 +863,14 @@ __global__ void __launch_bounds__(256) k_head_grad_kept(const ProductArgs a) {
         }
         const ExpFrom<sizeof(T) == 4> ex(row.m);
         logits_to_g(g, ex, row.s, row.factor, in ? row.target - a.first - c0 : 0xffffffffu, a.columns - min(a.columns, c0), in);
-        S* out = static_cast<S*>(a.g) + (uint64_t)slot * a.g_pitch + c0;
 #pragma unroll
         for (int p = 0; p < PARTS; p++) {
+            S* out = static_cast<S*>(a.g) + ((uint64_t)(p * a.g_blocks + c0 / 64) * a.cap + slot) * 64 + c0 % 64;
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) w[j] = next_part<S>(g[2 * j], g[2 * j + 1], p + 1 < PARTS);
-            store32(out + p * a.g_part, w);
-            store32(out + p * a.g_part + 16, w + 8);
+            store32(out, w);
+            store32(out + 16, w + 8);
         }
     }
 }
@@ -1097,11 +1097,11 @@ struct Products {
         a.scale = (float)gr->grad_scale;
         a.accumulate = gr->accumulate;
         a.dw = gr->d_weight;
-        a.g_pitch = (uint32_t)h->piece;
-        a.g_part = h->cap * h->piece;
-        OXZ_TRY(tensor_map(&mg, ST, h->g, h->piece, h->cap, h->g_parts, a.g_part));
+        a.g_blocks = (uint32_t)(h->piece / 64);
+        a.cap = (uint32_t)h->cap;
+        OXZ_TRY(tensor_map(&mg, ST, h->g, 64, h->cap, h->piece / 64 * h->g_parts, h->cap * 64));
         CUtensorMap mgo, mdx, mds, mdw = mg;
-        OXZ_TRY(tensor_map(&mgo, ST, h->g, h->piece, h->cap, h->g_parts, a.g_part, 32));
+        OXZ_TRY(tensor_map(&mgo, ST, h->g, 64, h->cap, h->piece / 64 * h->g_parts, h->cap * 64, 32));
         OXZ_TRY(tensor_map(&mdx, OXZ_F32, h->dx, h->dx_pitch, h->cap, 1, h->cap * h->dx_pitch, 32));
         const uint64_t share_lines = (uint64_t)MAX_ROUNDS * h->clusters * MMA_M;
         OXZ_TRY(tensor_map(&mds, OXZ_F32, h->dx_shares, MMA_N, share_lines, 1, share_lines * MMA_N, 32));

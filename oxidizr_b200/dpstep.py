@@ -488,10 +488,6 @@ class LitDataLoader:
 
 
 # ------------------------------------------------------------------ the token operators
-def _ptr(address: int | None):
-    return C.c_void_p(address) if address else None
-
-
 class TokenEmbedding:
     """The token embedding and its gradient (embed_tokens, [vocab, hidden]): ``out[i] = scale * table[ids[i]]`` and
     ``d_table[v] = scale * sum of d_out[i] over the tokens i with ids[i] = v``. All arguments are device addresses; sums run
@@ -516,13 +512,13 @@ class TokenEmbedding:
         self.workspace_bytes = v.value
 
     def lookup(self, ids: int, n: int, table: int, out: int, out_stride: int = 0, stream: int | None = None) -> None:
-        check(lib().oxz_embed_lookup_async(self._h, _ptr(ids), n, _ptr(table), _ptr(out), out_stride, _ptr(stream)))
+        check(lib().oxz_embed_lookup_async(self._h, ids, n, table, out, out_stride, stream))
 
     def grads(self, ids: int, n: int, d_out: int, d_table: int, accumulate: bool = False, d_out_stride: int = 0,
               stream: int | None = None) -> None:
         """accumulate False writes every row of d_table (zeros where no token is), True adds to the rows that have tokens."""
-        check(lib().oxz_embed_grads_async(self._h, _ptr(ids), n, _ptr(d_out), d_out_stride, _ptr(d_table), int(accumulate),
-                                          _ptr(stream)))
+        check(lib().oxz_embed_grads_async(self._h, ids, n, d_out, d_out_stride, d_table, int(accumulate),
+                                          stream))
 
     def destroy(self) -> None:
         if self._h:
