@@ -5,6 +5,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -36,12 +38,15 @@ def needs_build() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB
-    cmd = [_nvcc(), *ARCH, "-O3", "-std=c++17", "-lineinfo", "-shared", "-Xcompiler", "-fPIC,-Wall,-Wextra",
-           *_host_compiler(), "-cudart", "static", "-o", LIB, *[os.path.join(CSRC, s) for s in SOURCES], "-ldl"]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    # one nvcc per source, side by side: the kernels' template instances are most of the time
+    flags = [*ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-Wall,-Wextra", *_host_compiler(), *(["-Xptxas=-v"] if verbose else [])]
+    with tempfile.TemporaryDirectory() as out, ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        objects = [os.path.join(out, s + ".o") for s in SOURCES]
+        cmds = [[_nvcc(), *flags, "-c", "-o", o, os.path.join(CSRC, s)] for s, o in zip(SOURCES, objects)]
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds))
+        list(pool.map(lambda c: subprocess.run(c, check=True), cmds))
+        subprocess.run([_nvcc(), *ARCH, "-shared", *_host_compiler(), "-cudart", "static", "-o", LIB, *objects, "-ldl"], check=True)
     return LIB
 
 
