@@ -596,8 +596,9 @@ typedef struct oxz_head_desc {
     uint64_t hidden;       /* elements of a row, at most 2^20 */
     uint64_t vocab;        /* rows of the weight, at most 2^30 */
     uint64_t piece_bytes;  /* the most workspace for pieces; 0 = 2 GiB. A third holds one piece's gradient of the logits; the rest,
-                              where hidden is large enough for that to pay and all logits of a batch fit it in f32, the logits
-                              between the losses and the gradients of one call, which else are formed again */
+                              where all logits of a batch fit it in f32 (and hidden is large enough for that to pay, or the logits
+                              are at most 2^22), the logits between the losses and the gradients of one call, which else are
+                              formed again */
     int32_t dtype;         /* oxz_dtype of hidden, weight and d_hidden */
     int32_t grad_dtype;    /* oxz_dtype of d_weight: dtype or OXZ_F32 */
     int32_t device;        /* CUDA device ordinal */

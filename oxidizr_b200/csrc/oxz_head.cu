@@ -53,6 +53,7 @@ struct oxz_head {
     void* g = nullptr;               // [g_parts][piece / 64][cap][64]: every box that is written or read is one stretch of memory
     float* l = nullptr;              // [scored rows][kept] logits
     uint64_t l_elems = 0, kept_pitch = 0;
+    bool keep_large = false;         // also batches of more than FEW_LOGITS logits keep them
     float* dx = nullptr;             // [scored rows][dx_pitch] sums over the pieces
     float* dx_shares = nullptr;      // tiles of 256 x 256: the shares after the first of the tiles that are cut
     int sms = 0;
@@ -68,6 +69,7 @@ struct oxz_head {
 namespace oxz {
 namespace {
 
+constexpr uint64_t FEW_LOGITS = 1ull << 22;
 constexpr uint32_t FINISH_ROWS = 32;  // rows a block of k_head_finish takes
 constexpr uint32_t MMA_M = 256, MMA_N = 256, MMA_K = 64;  // tile of a pair of SMs
 
@@ -1032,7 +1034,9 @@ struct Products {
         constexpr bool F32 = sizeof(T) == 4, BF16 = std::is_same<S, __nv_bfloat16>::value;
         const size_t es = sizeof(T);
         const unsigned many = (unsigned)h->clusters * 2 * 8;  // blocks of the elementwise kernels
-        const uint64_t x_part = h->cap * h->pitch, w_part = d.vocab * h->pitch, l_elems = want_loss && gr ? h->l_elems : 0;
+        const bool sure = b.rows * h->kept_pitch <= h->l_elems;  // all logits fit, whatever the mask
+        const bool keep = want_loss && gr && h->l_elems && (sure || h->keep_large);
+        const uint64_t x_part = h->cap * h->pitch, w_part = d.vocab * h->pitch, l_elems = keep ? h->l_elems : 0;
         const bool x_wide = !misaligned(b.hidden, 16) && b.hidden_stride * es % 16 == 0;
         const T* x = static_cast<const T*>(b.hidden);
         const uint64_t pack = (b.rows + MMA_M) * (h->pitch / 8);  // 16-byte pieces at most
@@ -1070,7 +1074,7 @@ struct Products {
         a.bf16 = BF16;
         a.dx_shares = h->dx_shares;
         a.piece = (uint32_t)h->piece;
-        a.keep = want_loss && gr;
+        a.keep = keep;
         a.expired = h->d_expired;
         // an f32 operand is hi + mid + lo; of the nine products the six above 2^-24 are formed, the small ones first
         static const uint8_t six[2][6] = {{2, 1, 0, 1, 0, 0}, {0, 1, 2, 0, 1, 0}};
@@ -1086,7 +1090,7 @@ struct Products {
         if (want_loss) {
             a.columns = (uint32_t)d.vocab;
             CUtensorMap ml = mx;  // not used where nothing is kept
-            if (a.keep && h->l_elems) OXZ_TRY(tensor_map(&ml, OXZ_F32, h->l, h->kept_pitch, h->l_elems / h->kept_pitch, 1, h->l_elems / h->kept_pitch * h->kept_pitch, 32));
+            if (a.keep) OXZ_TRY(tensor_map(&ml, OXZ_F32, h->l, h->kept_pitch, h->l_elems / h->kept_pitch, 1, h->l_elems / h->kept_pitch * h->kept_pitch, 32));
             OXZ_TRY(launch<LOGITS_STATS>(h, mx, mw, ml, ml, a, b.rows, d.vocab, s));
             const unsigned blocks = std::max<unsigned>(1, (unsigned)((b.rows + FINISH_ROWS - 1) / FINISH_ROWS));
             OXZ_CUDA(launch_after(true, k_head_finish, blocks, 1024, 0, s, (uint32_t)b.rows, a.pitch, 2 * tiles_of(d.vocab, MMA_N), h->slot_of, h->part,
@@ -1108,14 +1112,13 @@ struct Products {
         // d_weight leaves by TMA where its rows are whole 16-byte pieces; 16-bit sums with what was there are made by the threads
         a.boxes = gr->d_weight && d.hidden * sizeof(G) % 16 == 0 && (sizeof(G) == 4 || !gr->accumulate);
         if (a.boxes) OXZ_TRY(tensor_map(&mdw, d.grad_dtype, gr->d_weight, d.hidden, d.vocab, 1, d.vocab * d.hidden, 32));
-        const bool sure = b.rows * h->kept_pitch <= h->l_elems;  // kept whatever the mask
         for (uint64_t v = 0; v < d.vocab; v += h->piece) {
             a.first = (uint32_t)v;
             a.columns = (uint32_t)std::min(h->piece, d.vocab - v);
             a.add = v > 0;
             pairs(1);
             // the scored rows' count decides on the device which of the two has work
-            if (a.keep && b.rows && h->l_elems) OXZ_CUDA(launch_after(true, k_head_grad_kept<T, S, PARTS>, many, 256, 0, s, a));
+            if (a.keep && b.rows) OXZ_CUDA(launch_after(true, k_head_grad_kept<T, S, PARTS>, many, 256, 0, s, a));
             if (!a.keep || !sure) OXZ_TRY(launch<LOGITS_GRAD>(h, mx, mw, mgo, mgo, a, b.rows, a.columns, s));
             if (gr->d_hidden) OXZ_TRY(launch<D_HIDDEN>(h, mg, mw, mdx, mds, a, b.rows, d.hidden, s));
             pairs(h->g_parts);
@@ -1251,9 +1254,12 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             if (d.dtype == OXZ_F32 || d.hidden % 8) OXZ_TRY(get(&h->w, d.vocab * h->pitch * h->parts * 2));
             OXZ_TRY(get(&h->g, h->cap * h->piece * h->g_parts * 2));
             h->kept_pitch = all;
-            // kept logits are written and read once (10 bytes of traffic an element with G's 2: 1.6 ps measured); forming them again
-            // takes 2 x hidden operations on the tensor cores, six times that for f32 (0.85 ps at hidden 384, 2.9 at 2048, 16 bits)
-            h->l_elems = d.hidden * (d.dtype == OXZ_F32 ? 6 : 1) >= 1024 ? std::min(budget / 3 * 2 / 4, h->cap * all) : 0;
+            // Kept logits are written and read once (10 bytes of traffic an element with G's 2: 1.6 ps measured); forming them again
+            // takes 2 x hidden operations on the tensor cores, six times that for f32 (0.85 ps at hidden 384, 2.9 at 2048, 16 bits).
+            // A batch of few logits keeps them at any width: its time is launches, and G from them takes a light one
+            // (100 x 360 x 12300 bf16: 42 us, 48 when they are formed again).
+            h->keep_large = d.hidden * (d.dtype == OXZ_F32 ? 6 : 1) >= 1024;
+            h->l_elems = std::min(budget / 3 * 2 / 4, std::min<uint64_t>(h->cap * all, h->keep_large ? ~uint64_t(0) : FEW_LOGITS));
             if (h->l_elems < all) h->l_elems = 0;  // not a single row
             if (h->l_elems) OXZ_TRY(get(&h->l, h->l_elems * 4));
             OXZ_TRY(get(&h->dx, h->cap * h->dx_pitch * 4));
