@@ -38,7 +38,7 @@ struct oxz_head {
     uint64_t piece = 0;              // columns of the vocabulary in a piece
     int32_t* row_of = nullptr;       // [max_rows] slot -> row of the batch, scored rows in order
     int32_t* slot_of = nullptr;      // [max_rows] row -> slot, -1: not scored
-    float2* part = nullptr;          // [2 * tiles][max_rows] {max, sum of exp} of a slot over half a tile of the vocabulary
+    float2* part = nullptr;          // [2 * tiles][rows] {max, sum of exp} of a slot over half a tile of the vocabulary
     float* target_logit = nullptr;   // [max_rows] by slot
     float2* stats = nullptr;         // [max_rows] by row, where the caller keeps none
     double* loss_part = nullptr;     // [blocks of k_head_finish]
@@ -70,8 +70,8 @@ namespace oxz {
 namespace {
 
 constexpr uint64_t FEW_LOGITS = 1ull << 22;
-constexpr uint32_t FINISH_ROWS = 32;  // rows a block of k_head_finish takes
-constexpr uint32_t MMA_M = 256, MMA_N = 256, MMA_K = 64;  // tile of a pair of SMs
+constexpr uint32_t FINISH_ROWS = 8;  // rows a block of k_head_finish takes at least
+constexpr uint32_t MMA_M = 256, MMA_N = 256, MMA_K = 64;  // tile of a pair of SMs (the logits' may be narrower: see tile_width)
 
 __host__ __device__ inline uint32_t tiles_of(uint64_t n, uint32_t of) { return (uint32_t)((n + of - 1) / of); }
 
@@ -148,51 +148,57 @@ __global__ void __launch_bounds__(1024) k_head_rows(const int64_t* __restrict__ 
 }
 
 // ---- the rows' statistics from their tiles', their losses, and the totals (by the block that ends last, in block order). A block
-// takes 32 rows, a lane each; its warps take every 32nd tile and are joined in order.
+// takes ROWS rows, a thread every few tiles of one of them, four at once; the threads of a row are joined in order. ROWS is 8, and 32
+// for many rows: 32 would leave a batch of some hundred rows to a handful of blocks, each a long chain of loads.
+template <int ROWS>
 __global__ void __launch_bounds__(1024) k_head_finish(uint32_t rows, uint32_t pitch, uint32_t tiles, const int32_t* __restrict__ slot_of,
                                                       const float2* __restrict__ part, const float* __restrict__ target_logit,
                                                       const float* __restrict__ mask, float2* stats, float* row_loss, double* loss_part,
                                                       HeadMeta* meta, float* totals) {
-    __shared__ float2 share[32][33];
-    __shared__ double mine[32];
+    __shared__ float2 share[1024 / ROWS][ROWS + 1];
+    __shared__ double mine[ROWS];
     __shared__ uint32_t last;
     let_next();
     after_previous();
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, row = blockIdx.x * FINISH_ROWS + lane;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, row = blockIdx.x * ROWS + lane % ROWS, first = threadIdx.x / ROWS;
     const int32_t slot = row < rows ? slot_of[row] : -1;
     // the row that the warp ends, asked for now
-    const uint32_t own = blockIdx.x * FINISH_ROWS + warp;
-    const int32_t at = own < rows ? slot_of[own] : -1;
+    const uint32_t own = blockIdx.x * ROWS + warp;
+    const int32_t at = warp < ROWS && own < rows ? slot_of[own] : -1;
     const float own_logit = at >= 0 ? target_logit[at] : 0.f;
     const double own_weight = at >= 0 ? (mask ? (double)mask[own] : 1.0) : 0.0;
     float2 s = make_float2(-INFINITY, 0.f);
     if (slot >= 0) {
-        for (uint32_t t = warp; t < tiles; t += 4 * 32) {
+        const uint32_t step = blockDim.x / ROWS;
+        for (uint32_t t = first; t < tiles; t += 4 * step) {
             float2 p[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) p[k] = t + 32 * k < tiles ? part[(uint64_t)(t + 32 * k) * pitch + slot] : make_float2(-INFINITY, 0.f);
+            for (int k = 0; k < 4; k++) p[k] = t + step * k < tiles ? part[(uint64_t)(t + step * k) * pitch + slot] : make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int k = 0; k < 4; k++) s = join_stats(s, p[k]);
         }
     }
-    share[warp][lane] = s;
+    share[first][lane % ROWS] = s;
     __syncthreads();
-    // now a warp has one row, a lane one of its parts
-    s = share[lane][warp];
+    // now a warp has one row, a lane four of its parts
+    if (warp < ROWS) {
+        s = share[lane][warp];
+        for (uint32_t k = lane + 32; k < blockDim.x / ROWS; k += 32) s = join_stats(s, share[k][warp]);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) s = join_stats(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
-    if (lane == 0) {
-        const float loss = at >= 0 ? logf(s.y) - (own_logit - s.x) : 0.f;
-        if (own < rows) {
-            stats[own] = at >= 0 ? s : make_float2(0.f, 0.f);
-            if (row_loss) row_loss[own] = loss;
+        for (int o = 1; o < 32; o <<= 1) s = join_stats(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
+        if (lane == 0) {
+            const float loss = at >= 0 ? logf(s.y) - (own_logit - s.x) : 0.f;
+            if (own < rows) {
+                stats[own] = at >= 0 ? s : make_float2(0.f, 0.f);
+                if (row_loss) row_loss[own] = loss;
+            }
+            mine[warp] = at >= 0 ? own_weight * (double)loss : 0.0;
         }
-        mine[warp] = at >= 0 ? own_weight * (double)loss : 0.0;
     }
     if (!totals) return;
     __syncthreads();
     if (warp) return;
-    double sum = mine[lane];
+    double sum = lane < ROWS ? mine[lane] : 0.0;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (gridDim.x == 1) {
@@ -364,7 +370,7 @@ constexpr uint32_t MMA_SMEM = STAGES * STAGE_BYTES + EPILOGUE_WARPS * OUT_BYTES 
 struct ProductArgs {
     const HeadMeta* meta;
     const int32_t* row_of;
-    uint32_t hidden, first, columns, piece, pitch, cap, g_blocks, dx_pitch, keep;  // the piece [first, first + columns) of the vocabulary
+    uint32_t hidden, first, columns, piece, pitch, cap, g_blocks, dx_pitch, keep, width;  // the piece [first, first + columns) of the vocabulary
     const int64_t* targets;
     const float* mask;
     const float2* stats;
@@ -386,15 +392,16 @@ struct ProductArgs {
 // fewer than the pairs, are cut in K into `shares` each, as many as fill one to four more rounds best. The pairs of a round walk K in
 // step, so that what they read is read once from memory (tiles cut at any step balance as well and read G six times over: 835 -> 1035
 // us a piece of 16384 words, 8192 rows, hidden 2048).
-constexpr uint32_t MIN_SHARE = 8, MAX_ROUNDS = 4;  // steps of K in a share at least
+constexpr uint32_t MAX_ROUNDS = 4;
+__host__ __device__ constexpr uint32_t min_share(size_t size) { return size == 4 ? 2 : 8; }  // steps of K in a share at least; one of f32 is six products
 struct Split {
     uint32_t tiles, whole, rest, shares;
-    __host__ __device__ Split(uint64_t rows, uint32_t hidden, uint64_t piece, uint32_t pairs) {
+    __host__ __device__ Split(uint64_t rows, uint32_t hidden, uint64_t piece, uint32_t pairs, uint32_t least) {
         tiles = tiles_of(rows, MMA_M) * tiles_of(hidden, MMA_N);
         rest = tiles % pairs;
         whole = tiles - rest;
         shares = 1;
-        const uint32_t top = tiles_of(piece, MMA_K) / MIN_SHARE;
+        const uint32_t top = tiles_of(piece, MMA_K) / least;
         uint32_t rounds = 1;
         for (uint32_t r = 1; rest && r <= MAX_ROUNDS; r++) {
             uint32_t k = r * pairs / rest;
@@ -531,9 +538,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     const uint32_t n = a.meta->n;
     const uint32_t M = P == D_WEIGHT ? a.columns : n, N = LOGITS ? a.columns : a.hidden;
     const uint32_t K = P == D_HIDDEN ? a.columns : P == D_WEIGHT ? n : a.hidden;
-    const uint32_t mt = tiles_of(M, MMA_M), nt = tiles_of(N, MMA_N), steps = tiles_of(K, MMA_K);
+    const uint32_t wide = LOGITS ? a.width : MMA_N;
+    const uint32_t mt = tiles_of(M, MMA_M), nt = tiles_of(N, wide), steps = tiles_of(K, MMA_K);
     const bool skip = P == LOGITS_GRAD && a.keep && a.meta->kept;  // k_head_grad_kept has made G from the logits that are kept
-    const Split split(n, a.hidden, a.piece, gridDim.x / 2);
+    const Split split(n, a.hidden, a.piece, gridDim.x / 2, min_share(sizeof(T)));
     struct Tile {
         uint32_t m0, n0, width, half, k0, steps, share;
     };
@@ -559,8 +567,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             m = t / nt;
         }
         r.m0 = m * MMA_M;
-        r.n0 = c * MMA_N;
-        r.width = min(MMA_N, (N - r.n0 + 31) & ~31u);
+        r.n0 = c * wide;
+        r.width = min(wide, (N - r.n0 + 31) & ~31u);
         r.half = r.width / 2;
         return r;
     };
@@ -653,8 +661,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
             // column of the tile that the target has; far outside it where another tile has it
             const uint32_t target = LOGITS && in ? row.target - a.first - c.n0 : 0xffffffffu;
             const ExpFrom<F32> ex(row.m);
-            const uint32_t valid = min(MMA_N, N - c.n0);  // columns of the tile that exist
-            const uint32_t from = side * 128, to = min(from + 128, P == LOGITS_GRAD ? (valid + 63) & ~63u : valid);
+            const uint32_t valid = min(wide, N - c.n0);  // columns of the tile that exist
+            const uint32_t from = side * (wide / 2), to = min(from + wide / 2, P == LOGITS_GRAD ? (valid + 63) & ~63u : valid);
             // the tile's 128 columns of this warp leave tensor memory at once, which frees the accumulator for the next tile
             float acc[4][32];
             auto run_done = [&]() {  // a run is in the accumulator buffer
@@ -702,6 +710,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                 if (!ok) break;
             }
             const int32_t line = (int32_t)(c.m0 + rank * 128 + quarter * 32);  // the warp's first row
+            // lines of the logits that no product reads: d_weight reads G up to the next step of K, and d_hidden's lines past the last
+            // scored row are not read themselves
+            const bool idle = LOGITS && (uint32_t)line >= (P == LOGITS_GRAD ? (n + 63) & ~63u : n);
             // 128 bytes of each of the warp's rows go out as one box: 16-byte pieces in the order of the 128-byte swizzle, no two lanes of
             // a quarter warp in one bank
             auto box = [&](const CUtensorMap& map, int32_t x, int32_t y, int32_t z, const uint32_t (&w)[32], bool add) {
@@ -729,7 +740,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const uint32_t c0 = from + 32 * q;
-                    if (kept && c0 < to) {
+                    if (c0 >= to || idle) break;
+                    if (kept) {
                         uint32_t w[32];
                         words(q, w);
                         box(map_out, (int32_t)(c.n0 + c0), line, 0, w, false);
@@ -740,10 +752,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                         for (int j = 0; j < 32; j++) tl = target - c0 == (uint32_t)j ? acc[q][j] : tl;
                         a.target_logit[i] = tl;
                     }
-                    if (c0 + 32 > valid) {
+                    if (c0 + 32 > to) {
 #pragma unroll
                         for (int j = 0; j < 32; j++)
-                            if (c0 + j >= valid) acc[q][j] = -INFINITY;  // no word of the vocabulary
+                            if (c0 + j >= to) acc[q][j] = -INFINITY;  // no word of the vocabulary
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j++) m8[j & 7] = fmaxf(m8[j & 7], acc[q][j]);
@@ -755,16 +767,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < 4; k++) s4[k] = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int q = 0; q < 4; q++)
+                for (int q = 0; q < 4; q++) {
+                    if (from + 32 * q >= to || idle) break;
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) s4[j / 2 & 3] = add2(s4[j / 2 & 3], e(make_float2(acc[q][j], acc[q][j + 1])));
+                }
                 const float2 s1 = add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])), run_stats = make_float2(m, s1.x + s1.y);
-                if (in) a.part[(uint64_t)(2 * (c.n0 / MMA_N) + side) * a.pitch + i] = run_stats;
+                if (in) a.part[(uint64_t)(2 * (c.n0 / wide) + side) * a.pitch + i] = run_stats;
             } else if constexpr (P == LOGITS_GRAD) {
 #pragma unroll
                 for (int q = 0; q < 4; q += 2) {
                     const uint32_t c0 = from + 32 * q;
-                    if (c0 >= to) break;
+                    if (c0 >= to || idle) break;
 #pragma unroll
                     for (int e = 0; e < 2; e++)
                         logits_to_g(acc[q + e], ex, row.s, row.factor, target - c0 - 32 * e, valid - min(valid, c0 + 32 * e), in);
@@ -840,7 +854,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
 }
 
 // ---- a piece of G from logits that the losses have kept, the same bits as the product would give. A thread takes 32 columns of a
-// scored row; the rows up to the next multiple of a tile are zeros, as every line of G that a product reads.
+// scored row; the rows up to the next step of d_weight's K are zeros.
 template <typename T, typename S, int PARTS>
 __global__ void __launch_bounds__(256) k_head_grad_kept(const ProductArgs a) {
     let_next();
@@ -848,7 +862,7 @@ __global__ void __launch_bounds__(256) k_head_grad_kept(const ProductArgs a) {
     const uint32_t n = a.meta->n, kept = a.meta->kept;
     if (kept == 0 || n == 0) return;
     const uint32_t per = ((a.columns + 63) & ~63u) / 32;
-    const uint64_t total = (uint64_t)tiles_of(n, MMA_M) * MMA_M * per;
+    const uint64_t total = (uint64_t)((n + 63) & ~63u) * per;
     for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
         const uint32_t slot = (uint32_t)(e / per), c0 = (uint32_t)(e - (uint64_t)slot * per) * 32;
         const bool in = slot < n;
@@ -878,43 +892,66 @@ __global__ void __launch_bounds__(256) k_head_grad_kept(const ProductArgs a) {
 }
 
 // ---- d_hidden: the scored rows' sums, their shares in order, times the scale, rounded; zeros for the others
-// N columns a thread: four, so that a small d_hidden spreads over the SMs, or one where rows are not aligned
-template <typename T, int N>
+// N columns a thread: four, so that a small d_hidden spreads over the SMs, or one where rows are not aligned. GROUPS warps of a block
+// share the shares of 32 x N elements, in order, and are joined in order: a small d_hidden has many shares and few elements, and a thread
+// alone would wait for one load after the other (122 x 128, 73 shares: 15 us, 6 in 8 groups).
+template <typename T, int N, int GROUPS>
 __global__ void __launch_bounds__(256) k_head_d_hidden(uint32_t rows, uint32_t hidden, uint32_t dx_pitch, uint64_t piece, uint32_t pairs,
                                                        const int32_t* __restrict__ slot_of, const float* __restrict__ dx,
                                                        const float* __restrict__ dx_shares, const HeadMeta* __restrict__ meta, float scale, T* out,
                                                        uint64_t stride) {
+    static_assert(GROUPS == 1 || GROUPS == 8, "warps of a block");
+    __shared__ float joined[GROUPS > 1 ? 8 : 1][32 * N];
     let_next();
     after_previous();
     scale *= meta->down;
-    const Split split(meta->n, hidden, piece, pairs);
-    const uint32_t per = (hidden + N - 1) / N, nt = tiles_of(hidden, MMA_N);
+    const Split split(meta->n, hidden, piece, pairs, min_share(sizeof(T)));
+    const uint32_t per = (hidden + N - 1) / N, nt = tiles_of(hidden, MMA_N), group = GROUPS > 1 ? threadIdx.x / 32 : 0;
     const uint64_t total = (uint64_t)rows * per;
-    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
-        const uint32_t row = (uint32_t)(e / per), col = (uint32_t)(e - (uint64_t)row * per) * N;
-        const int32_t slot = slot_of[row];
+    constexpr uint32_t AT_ONCE = 256 / GROUPS;  // elements of N columns a block takes
+    for (uint64_t e0 = (uint64_t)blockIdx.x * AT_ONCE; e0 < total; e0 += (uint64_t)gridDim.x * AT_ONCE) {
+        const uint64_t e = e0 + threadIdx.x % AT_ONCE;
+        const bool here = e < total;
+        const uint32_t row = here ? (uint32_t)(e / per) : 0, col = here ? (uint32_t)(e - (uint64_t)row * per) * N : 0;
+        const int32_t slot = here ? slot_of[row] : -1;
         Vec<float, N> sum;
 #pragma unroll
         for (int j = 0; j < N; j++) sum.e[j] = 0.f;
         if (slot >= 0) {
-            sum.load(dx + (uint64_t)slot * dx_pitch + col);
             const uint32_t tile = slot / MMA_M * nt + col / MMA_N;
             const float* from = dx_shares + ((uint64_t)tile - split.whole) * (MMA_M * MMA_N) + slot % MMA_M * MMA_N + col % MMA_N;
-            const uint32_t shares = tile >= split.whole ? split.shares : 1;
+            const uint32_t shares = tile >= split.whole ? split.shares : 1, each = (shares + GROUPS - 1) / GROUPS;
+            uint32_t k = group * each;
+            const uint32_t end = min(shares, k + each);
+            if (k == 0) {
+                sum.load(dx + (uint64_t)slot * dx_pitch + col);
+                k = 1;
+            }
             constexpr int AHEAD = 8;
-            for (uint32_t k = 1; k < shares; k += AHEAD) {
+            for (; k < end; k += AHEAD) {
                 Vec<float, N> v[AHEAD];
 #pragma unroll
                 for (int a = 0; a < AHEAD; a++)
-                    if (k + a < shares) v[a].load(from + (uint64_t)(k + a - 1) * split.rest * (MMA_M * MMA_N));
+                    if (k + a < end) v[a].load(from + (uint64_t)(k + a - 1) * split.rest * (MMA_M * MMA_N));
 #pragma unroll
                 for (int a = 0; a < AHEAD; a++)
-                    if (k + a < shares) {
+                    if (k + a < end) {
 #pragma unroll
                         for (int j = 0; j < N; j++) sum.e[j] += v[a].e[j];
                     }
             }
         }
+        if constexpr (GROUPS > 1) {
+            __syncthreads();  // the sums of the round before have been read
+#pragma unroll
+            for (int j = 0; j < N; j++) joined[group][threadIdx.x % 32 + 32 * j] = sum.e[j];
+            __syncthreads();
+            if (group) continue;
+            for (int g = 1; g < GROUPS; g++)
+#pragma unroll
+                for (int j = 0; j < N; j++) sum.e[j] += joined[g][threadIdx.x + 32 * j];
+        }
+        if (!here) continue;
         Vec<T, N> o;
 #pragma unroll
         for (int j = 0; j < N; j++) o.e[j] = from_f32<T>(slot < 0 ? 0.f : sum.e[j] * scale);
@@ -953,12 +990,21 @@ int32_t tensor_map(CUtensorMap* m, int32_t dtype, const void* base, uint64_t pit
     return OXZ_OK;
 }
 
+// Width of the logits' tiles: halved while all of them still run at once (the losses of 149 x 1088 x 2918 f32: 61 us with 12 tiles of 256
+// columns, 54 with 46 of 64). To fill the last of several rounds it does not pay, since a narrow tile loads as much of X as a wide one
+// (2048 x 2048 x 2500 bf16: 43 us with 80 tiles of 256, 51 with 160 of 128).
+uint32_t tile_width(const oxz_head* h, uint64_t rows, uint64_t columns, uint32_t least) {
+    uint32_t w = MMA_N;
+    while (w > least && (uint64_t)tiles_of(rows, MMA_M) * tiles_of(columns, w / 2) <= (uint64_t)h->clusters) w /= 2;
+    return w;
+}
+
 template <typename T, typename S, typename G, int PARTS>
 struct Products {
     template <int P>
     static int32_t launch(const oxz_head* h, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& out, const CUtensorMap& shares,
                           const ProductArgs& a, uint64_t m, uint64_t n, cudaStream_t s) {
-        const uint64_t tiles = (uint64_t)tiles_of(m, MMA_M) * tiles_of(n, MMA_N);
+        const uint64_t tiles = (uint64_t)tiles_of(m, MMA_M) * tiles_of(n, P == LOGITS_STATS || P == LOGITS_GRAD ? a.width : MMA_N);
         // the cut of D_HIDDEN goes by the number of pairs: always all of them
         const unsigned pairs = P == D_HIDDEN ? (unsigned)h->clusters : (unsigned)std::min<uint64_t>(tiles, h->clusters);
         if (tiles) OXZ_CUDA(launch_after(true, k_head_product<T, S, G, P, PARTS>, 2 * pairs, MMA_THREADS, MMA_SMEM, s, ma, mb, out, shares, a));
@@ -1062,7 +1108,7 @@ struct Products {
         a.meta = h->meta;
         a.row_of = h->row_of;
         a.hidden = (uint32_t)d.hidden;
-        a.pitch = (uint32_t)d.max_rows;
+        a.pitch = (uint32_t)b.rows;
         a.dx_pitch = h->dx_pitch;
         a.targets = b.targets;
         a.mask = b.loss_mask;
@@ -1089,11 +1135,14 @@ struct Products {
         pairs(1);
         if (want_loss) {
             a.columns = (uint32_t)d.vocab;
+            a.width = tile_width(h, b.rows, d.vocab, 64);
             CUtensorMap ml = mx;  // not used where nothing is kept
             if (a.keep) OXZ_TRY(tensor_map(&ml, OXZ_F32, h->l, h->kept_pitch, h->l_elems / h->kept_pitch, 1, h->l_elems / h->kept_pitch * h->kept_pitch, 32));
             OXZ_TRY(launch<LOGITS_STATS>(h, mx, mw, ml, ml, a, b.rows, d.vocab, s));
-            const unsigned blocks = std::max<unsigned>(1, (unsigned)((b.rows + FINISH_ROWS - 1) / FINISH_ROWS));
-            OXZ_CUDA(launch_after(true, k_head_finish, blocks, 1024, 0, s, (uint32_t)b.rows, a.pitch, 2 * tiles_of(d.vocab, MMA_N), h->slot_of, h->part,
+            const bool many_rows = b.rows > (uint64_t)h->sms * FINISH_ROWS / 2;
+            const unsigned per = many_rows ? 32 : FINISH_ROWS, blocks = std::max<unsigned>(1, (unsigned)((b.rows + per - 1) / per)), halves = 2 * tiles_of(d.vocab, a.width);
+            const unsigned threads = many_rows ? 1024 : std::min(1024u, std::max(256u, (halves / 4 * per + 255) / 256 * 256));
+            OXZ_CUDA(launch_after(true, many_rows ? k_head_finish<32> : k_head_finish<FINISH_ROWS>, blocks, threads, 0, s, (uint32_t)b.rows, a.pitch, halves, h->slot_of, h->part,
                                   h->target_logit, b.loss_mask, stats, row_loss, h->loss_part, h->meta, totals));
         }
         if (!gr) return OXZ_OK;
@@ -1116,6 +1165,7 @@ struct Products {
             a.first = (uint32_t)v;
             a.columns = (uint32_t)std::min(h->piece, d.vocab - v);
             a.add = v > 0;
+            a.width = tile_width(h, b.rows, a.columns, 128);  // G leaves in boxes of 64 columns
             pairs(1);
             // the scored rows' count decides on the device which of the two has work
             if (a.keep && b.rows) OXZ_CUDA(launch_after(true, k_head_grad_kept<T, S, PARTS>, many, 256, 0, s, a));
@@ -1129,9 +1179,13 @@ struct Products {
         if (gr->d_hidden && b.rows) {
             constexpr int N = 4;
             const bool wide = !misaligned(gr->d_hidden, N * es) && gr->d_hidden_stride % N == 0 && d.hidden % N == 0;
-            auto k = wide ? k_head_d_hidden<T, N> : k_head_d_hidden<T, 1>;
-            OXZ_CUDA(launch_after(true, k, (unsigned)std::min<uint64_t>((b.rows * d.hidden / (wide ? N : 1) + 255) / 256, many), 256, 0, s, (uint32_t)b.rows,
-                                  (uint32_t)d.hidden, h->dx_pitch, h->piece, (uint32_t)h->clusters, h->slot_of, h->dx, h->dx_shares, h->meta, a.scale,
+            // elements a thread, or a group of eight; eight where they fill the SMs' blocks at most once
+            const uint64_t elements = b.rows * ((d.hidden + (wide ? N : 1) - 1) / (wide ? N : 1));
+            const bool grouped = elements <= (uint64_t)many * 32;
+            auto k = wide ? (grouped ? k_head_d_hidden<T, N, 8> : k_head_d_hidden<T, N, 1>) : (grouped ? k_head_d_hidden<T, 1, 8> : k_head_d_hidden<T, 1, 1>);
+            const uint64_t blocks = (elements + (grouped ? 31 : 255)) / (grouped ? 32 : 256);
+            OXZ_CUDA(launch_after(true, k, (unsigned)std::min<uint64_t>(blocks, many), 256, 0, s, (uint32_t)b.rows, (uint32_t)d.hidden, h->dx_pitch, h->piece,
+                                  (uint32_t)h->clusters, h->slot_of, h->dx, h->dx_shares, h->meta, a.scale,
                                   static_cast<T*>(gr->d_hidden), gr->d_hidden_stride));
         }
         return OXZ_OK;
@@ -1245,7 +1299,7 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             };
             OXZ_TRY(get(&h->row_of, d.max_rows * 4));
             OXZ_TRY(get(&h->slot_of, d.max_rows * 4));
-            OXZ_TRY(get(&h->part, 2 * (all / MMA_N) * d.max_rows * 8));
+            OXZ_TRY(get(&h->part, 2 * std::max<uint64_t>((all / MMA_N) * d.max_rows, (uint64_t)h->clusters * MMA_M) * 8));
             OXZ_TRY(get(&h->target_logit, d.max_rows * 4));
             OXZ_TRY(get(&h->stats, d.max_rows * 8));
             OXZ_TRY(get(&h->loss_part, (d.max_rows + FINISH_ROWS - 1) / FINISH_ROWS * 8));
