@@ -34,7 +34,7 @@ constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_CLUSTER 
 constexpr int DIGIT_BITS = 9, BINS = 1 << DIGIT_BITS;
 constexpr uint32_t CHUNK = 16;  // sorted tokens a warp sums on its own
 constexpr uint32_t DIRECT = 1024;  // tokens that are summed without being sorted: see k_embed_direct
-constexpr uint32_t RANKED = 8192;  // tokens that are sorted by counting: see rank_tokens
+constexpr uint32_t RANKED = 8192;  // tokens that are sorted by counting: see k_embed_rank
 
 // ---- lookup: a warp takes a piece of 32 x 4 vectors of one row
 template <typename T, int N>
@@ -197,31 +197,44 @@ __global__ void __launch_bounds__(SORT_THREADS) k_embed_sort(const int64_t* __re
 }
 
 // ---- gradient, first launch, up to RANKED tokens: a token's place is the count of tokens with a smaller id, and of equal ones before it.
-// A block takes 64 tokens, 16 threads each, every one of which counts over a sixteenth of all tokens in shared memory: 8192 tokens
-// take 7 us over all SMs, where the radix sort's barriers take 16.
-constexpr uint32_t RANK_TOKENS = 64;
-__global__ void __launch_bounds__(SORT_THREADS) k_embed_rank(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, unsigned long long* sorted,
-                                                             uint32_t* touched) {
+// The tokens are dealt evenly to one block an SM; PARTS threads a token count over a share of all tokens in shared memory each, 32 while
+// a block has no more than 32 tokens. 8192 tokens take 7 us, where the radix sort's barriers take 16; see the sums for whole calls.
+template <int PARTS>
+__global__ void __launch_bounds__(SORT_THREADS) k_embed_rank(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, uint32_t tokens,
+                                                             unsigned long long* sorted, uint32_t* touched) {
     __shared__ __align__(16) uint32_t key[RANKED];
     let_next();
-    const uint32_t padded = (n + 63) & ~63u;
-    for (uint32_t i = threadIdx.x; i < padded; i += SORT_THREADS) {
+    const uint32_t padded = (n + 4 * PARTS - 1) / (4 * PARTS) * (4 * PARTS);
+    for (uint32_t i = threadIdx.x; i < padded; i += blockDim.x) {
         const int64_t id = i < n ? ids[i] : -1;
         key[i] = i < n ? ((uint64_t)id < vocab ? (uint32_t)id : vocab) : 0xffffffffu;
     }
     __syncthreads();
-    const uint32_t i = blockIdx.x * RANK_TOKENS + threadIdx.x / 16, part = threadIdx.x & 15;
-    const uint32_t mine = i < n ? key[i] : 0;
+    const uint32_t own = threadIdx.x / PARTS, part = threadIdx.x % PARTS;
+    const bool here = own < tokens && blockIdx.x * tokens + own < n;
+    const uint32_t i = here ? blockIdx.x * tokens + own : 0, mine = key[i];
     uint32_t count = 0;
-    for (uint32_t j = part * 4; j < padded; j += 64) {
-        const uint4 k = *reinterpret_cast<const uint4*>(key + j);
-        const uint32_t below = j + 4 <= i ? mine + 1 : mine;  // in front of the token equal ids count too
-        count += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
-        if (j < i && i < j + 4) count += (k.x == mine) + (j + 1 < i && k.y == mine) + (j + 2 < i && k.z == mine);
+    // in front of the token equal ids count too; its own four are looked at one by one
+    auto four = [&](uint32_t j) { return *reinterpret_cast<const uint4*>(key + j); };
+    const uint32_t its = i & ~3u;
+    uint32_t j = part * 4;
+#pragma unroll 4
+    for (; j < its; j += 4 * PARTS) {
+        const uint4 k = four(j);
+        count += (k.x <= mine) + (k.y <= mine) + (k.z <= mine) + (k.w <= mine);
+    }
+    if (j == its && here) {
+        for (uint32_t e = j; e < j + 4; e++) count += key[e] < mine + (e < i);
+        j += 4 * PARTS;
+    }
+#pragma unroll 4
+    for (; j < padded; j += 4 * PARTS) {
+        const uint4 k = four(j);
+        count += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
     }
 #pragma unroll
-    for (int o = 8; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
-    if (part == 0 && i < n) {
+    for (int o = PARTS / 2; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
+    if (part == 0 && here) {
         sorted[count] = (unsigned long long)mine << 32 | i;
         mark(touched, mine, vocab);
     }
@@ -243,31 +256,46 @@ __global__ void __launch_bounds__(SORT_THREADS) k_embed_fill(unsigned char* fill
 
 __device__ __forceinline__ uint32_t key_of(unsigned long long it) { return (uint32_t)(it >> 32); }
 
+// v: what the row holds, where it is added to
+template <typename G, int N>
+__device__ __forceinline__ void write_row(G* dst, Vec<G, N>& v, const float (&sum)[N], float scale, bool accumulate) {
+#pragma unroll
+    for (int j = 0; j < N; j++) v.e[j] = from_f32<G>(accumulate ? to_f32<G>(v.e[j]) + sum[j] * scale : sum[j] * scale);
+    v.store(dst);
+}
 template <typename G, int N>
 __device__ __forceinline__ void write_row(G* dst, const float (&sum)[N], float scale, bool accumulate) {
     Vec<G, N> v;
     if (accumulate) v.load_coherent(dst);
-#pragma unroll
-    for (int j = 0; j < N; j++) v.e[j] = from_f32<G>(accumulate ? to_f32<G>(v.e[j]) + sum[j] * scale : sum[j] * scale);
-    v.store(dst);
+    write_row<G, N>(dst, v, sum, scale, accumulate);
 }
 
 // ---- gradient, second launch: a warp sums one chunk of CHUNK sorted tokens for 32 x N columns. Tokens that lie inside the
 // chunk are written; the sums of a token that goes on from the chunk before or into the chunk after go to the carries:
 // carry[chunk][0] for the token the chunk begins with, carry[chunk][1] for one that begins in the chunk and leaves it.
 // Blocks from `summing` on write zeros to the rows that have no token: the sums wait on their loads, the zeros take the memory meanwhile
-// (a fill of all rows beside the sort, and the sums after it, took 133 us where this takes 124: 8192 x 2048 bf16, 128256 rows).
-template <typename T, typename G, int N>
+// (a fill of all rows beside the sort, and the sums after it, took 9 us more: 8192 x 2048 bf16, 128256 rows, 117 us now). Where rows are
+// added to (ADD), what they hold is asked for along with the rows that are summed: 39 us instead of 46 (4974 x 448: 20 instead of 25).
+template <typename T, typename G, int N, bool ADD>
 __global__ void __launch_bounds__(256) k_embed_sums(const unsigned long long* __restrict__ sorted, uint32_t n, uint32_t vocab,
                                                     const T* __restrict__ d_out, uint64_t stride, uint32_t hidden, G* d_table,
-                                                    float* __restrict__ carry, float scale, int accumulate, uint32_t slices,
-                                                    uint32_t summing, const uint32_t* __restrict__ touched) {
+                                                    float* __restrict__ carry, float scale, uint32_t slices, uint32_t summing,
+                                                    const uint32_t* __restrict__ touched) {
     let_next();
     after_previous();
     if (blockIdx.x >= summing) {
-        const uint64_t row_bytes = (uint64_t)hidden * sizeof(G), warps = (uint64_t)(gridDim.x - summing) * 8;
-        for (uint64_t row = (uint64_t)(blockIdx.x - summing) * 8 + threadIdx.x / 32; row < vocab; row += warps)
-            if (!(touched[row >> 5] >> (row & 31) & 1)) fill_row(reinterpret_cast<unsigned char*>(d_table) + row * row_bytes, row_bytes);
+        // a warp takes 8 rows, and asks for the next ones' bits before it writes
+        const uint64_t row_bytes = (uint64_t)hidden * sizeof(G), warps = (uint64_t)(gridDim.x - summing) * 8, eights = ((uint64_t)vocab + 7) / 8;
+        const unsigned char* bits_of = reinterpret_cast<const unsigned char*>(touched);
+        uint64_t u = (uint64_t)(blockIdx.x - summing) * 8 + threadIdx.x / 32;
+        uint32_t next = u < eights ? bits_of[u] : 0;
+        for (; u < eights; u += warps) {
+            const uint32_t bits = next;
+            if (u + warps < eights) next = bits_of[u + warps];
+            const uint32_t rows = (uint32_t)min((uint64_t)8, vocab - u * 8);
+            for (uint32_t r = 0; r < rows; r++)
+                if (!(bits >> r & 1)) fill_row(reinterpret_cast<unsigned char*>(d_table) + (u * 8 + r) * row_bytes, row_bytes);
+        }
         return;
     }
     const uint64_t chunks = (n + CHUNK - 1) / CHUNK;
@@ -287,13 +315,18 @@ __global__ void __launch_bounds__(256) k_embed_sums(const unsigned long long* __
 #pragma unroll
         for (int j = 0; j < N; j++) sum[j] = 0.f;
         uint32_t begin = 0;  // where the current token's run begins in the chunk
-        constexpr int AHEAD = 8;
+        constexpr int AHEAD = ADD ? 4 : 8;
         for (uint32_t k0 = 0; k0 < count; k0 += AHEAD) {
             Vec<T, N> v[AHEAD];
+            Vec<G, N> old[ADD ? AHEAD : 1];
 #pragma unroll
             for (int a = 0; a < AHEAD; a++) {
                 const unsigned long long x = __shfl_sync(0xffffffffu, it, (k0 + a) & 31);
                 if (live && k0 + a < count && key_of(x) < vocab) v[a].load(d_out + (uint64_t)(uint32_t)x * stride + col);
+                if constexpr (ADD) {  // the row a run of equal tokens ends in, which no other warp writes: asked for along with the sums' rows
+                    const uint32_t next = __shfl_sync(0xffffffffu, key_of(it), (k0 + a + 1) & 31);
+                    if (live && k0 + a < count && key_of(x) < vocab && next != key_of(x)) old[a].load_coherent(d_table + (uint64_t)key_of(x) * hidden + col);
+                }
             }
 #pragma unroll
             for (int a = 0; a < AHEAD; a++) {
@@ -309,7 +342,7 @@ __global__ void __launch_bounds__(256) k_embed_sums(const unsigned long long* __
                 const bool left = begin == 0 && from_left;
                 if (live) {
                     if (ends && !left) {
-                        write_row<G, N>(d_table + (uint64_t)key * hidden + col, sum, scale, accumulate != 0);
+                        write_row<G, N>(d_table + (uint64_t)key * hidden + col, old[ADD ? a : 0], sum, scale, ADD);
                     } else {
                         float* c = carry + ((uint64_t)chunk * 2 + (left ? 0 : 1)) * hidden + col;
 #pragma unroll
@@ -338,17 +371,19 @@ __global__ void __launch_bounds__(256) k_embed_join(const unsigned long long* __
     const uint32_t chunk = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const uint64_t c0 = (uint64_t)chunk * CHUNK, c1 = c0 + CHUNK;
     if (c1 >= n) return;  // nothing leaves the last chunk
-    const uint32_t key = key_of(sorted[c1 - 1]);
-    if (key >= vocab || key_of(sorted[c1]) != key) return;
-    if (key_of(sorted[c0]) == key && c0 > 0 && key_of(sorted[c0 - 1]) == key) return;  // began further left
-    // one past the token's last item
-    uint32_t lo = (uint32_t)c1, hi = n;
-    while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (key_of(sorted[mid]) <= key) lo = mid + 1;
-        else hi = mid;
+    const uint32_t key = key_of(sorted[c1 - 1]), beyond = key_of(sorted[c1]), head = key_of(sorted[c0]), front = c0 > 0 ? key_of(sorted[c0 - 1]) : vocab;
+    if (key >= vocab || beyond != key) return;
+    if (head == key && front == key) return;  // began further left
+    // the last chunk that begins with the token, 32 places asked at a time: it lies in [last, end)
+    uint32_t last = chunk + 1, end = (uint32_t)(((uint64_t)n + CHUNK - 1) / CHUNK);
+    while (end - last > 1) {
+        const uint32_t step = (end - last + 31) / 32;
+        const uint64_t probe = last + (uint64_t)(lane + 1) * step;
+        const bool same = probe < end && key_of(sorted[probe * CHUNK]) == key;
+        last += __popc(__ballot_sync(0xffffffffu, same)) * step;
+        end = min(end, last + step);
     }
-    const uint32_t last = (lo - 1) / CHUNK, parts = last - chunk;  // carries [0] of chunks chunk + 1 .. last
+    const uint32_t parts = last - chunk;  // carries [0] of chunks chunk + 1 .. last
     const uint32_t col = blockIdx.y * 32 * N + lane * N;
     const uint32_t each = (parts + 7) / 8, p0 = min(parts, warp * each), p1 = min(parts, p0 + each);
     float sum[N];
@@ -475,8 +510,8 @@ int32_t sums(oxz_embed* e, uint32_t n, const int64_t* ids, const unsigned long l
     const unsigned blocks = (unsigned)std::min<uint64_t>(((uint64_t)chunks * slices + 7) / 8, 1u << 30);
     uint32_t* touched = accumulate ? nullptr : e->touched;
     const unsigned fillers = accumulate ? 0 : (unsigned)std::min<uint64_t>(e->sms * 8, (d.vocab + 7) / 8);
-    OXZ_CUDA(launch_after(true, k_embed_sums<T, G, N>, blocks + fillers, 256, 0, s, sorted, n, vocab, static_cast<const T*>(d_out), stride, hidden,
-                          static_cast<G*>(d_table), e->carry, (float)d.scale, accumulate, slices, blocks, touched));
+    OXZ_CUDA(launch_after(true, accumulate ? k_embed_sums<T, G, N, true> : k_embed_sums<T, G, N, false>, blocks + fillers, 256, 0, s, sorted, n, vocab,
+                          static_cast<const T*>(d_out), stride, hidden, static_cast<G*>(d_table), e->carry, (float)d.scale, slices, blocks, touched));
     OXZ_CUDA(launch_after(true, k_embed_join<G, N>, dim3(chunks - 1, slices), 256, 0, s, sorted, n, vocab, hidden, static_cast<G*>(d_table), e->carry,
                           (float)d.scale, accumulate, touched));
     return OXZ_OK;
@@ -613,8 +648,9 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
             if (touched && !e->clean) OXZ_CUDA(cudaMemsetAsync(touched, 0, (d.vocab + 31) / 32 * 4, s));
             if (touched) e->clean = false;  // until every launch of this call has been made
             if (n <= RANKED) {
-                OXZ_CUDA(launch_after(false, k_embed_rank, ((unsigned)n + RANK_TOKENS - 1) / RANK_TOKENS, SORT_THREADS, 0, s, ids, (uint32_t)n, (uint32_t)d.vocab,
-                                      e->sorted[0], touched));
+                const uint32_t tokens = std::min<uint32_t>(64, ((uint32_t)n + e->sms - 1) / e->sms), parts = tokens <= 32 ? 32 : 16;
+                OXZ_CUDA(launch_after(false, parts == 32 ? k_embed_rank<32> : k_embed_rank<16>, ((unsigned)n + tokens - 1) / tokens, (tokens * parts + 31) / 32 * 32, 0,
+                                      s, ids, (uint32_t)n, (uint32_t)d.vocab, tokens, e->sorted[0], touched));
             } else {
                 // keys run to vocab itself (ids outside the table): as few passes of at most DIGIT_BITS bits as hold them, of equal width
                 int key_bits = 1;

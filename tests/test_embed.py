@@ -161,6 +161,28 @@ def test_gradient_is_the_sum_over_equal_tokens(dtype, grad, kind, n, hidden, voc
 
 
 @gpu
+@pytest.mark.parametrize("n", [1024, 1025, 2113, 4736, 4737, 8129, 8191, 8192, 8193])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradient_at_the_bounds_of_each_way_to_order_the_tokens(n, accumulate):
+    """Whole numbers, whose sums are exact: every token has to reach its row once, at the last count of each sort and the first of the
+    next, and where the tokens do not divide evenly among the blocks."""
+    import torch
+    hidden, vocab = 24, 2500
+    rng = np.random.default_rng(n)
+    ids = torch.from_numpy(make_ids("uniform", n, vocab, rng).astype(np.int64)).cuda()
+    d_out = torch.from_numpy(rng.integers(-4, 5, (n, hidden)).astype(np.float32)).cuda()
+    old = torch.from_numpy(rng.integers(-4, 5, (vocab, hidden)).astype(np.float32)).cuda()
+    table = old.clone() if accumulate else torch.full_like(old, float("nan"))
+    emb = ox.TokenEmbedding(vocab, hidden, n, dtype=ox.F32)
+    torch.cuda.synchronize()
+    emb.grads(ids.data_ptr(), n, d_out.data_ptr(), table.data_ptr(), accumulate=accumulate)
+    torch.cuda.synchronize()
+    want = torch.zeros_like(old).index_add_(0, ids, d_out) + (old if accumulate else 0)
+    assert torch.equal(table, want)
+    emb.destroy()
+
+
+@gpu
 def test_gradient_of_strided_rows_and_of_no_tokens():
     import torch
     n, hidden, vocab = 50, 24, 11
