@@ -166,19 +166,6 @@ __device__ void sort_tokens(cg::cluster_group& cl, SortShared& sh, const int64_t
     }
 }
 
-// Zeros over `bytes` at `fill`, by blocks first, first + step, ..
-__device__ __forceinline__ void fill_zeros(unsigned char* fill, uint64_t bytes, uint64_t first, uint64_t step) {
-    // up to 31 bytes either side of the 32-byte pieces (a table whose rows are not whole pieces)
-    unsigned char* lo = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fill) + 31) & ~(uintptr_t)31);
-    const uint64_t head = min((uint64_t)(lo - fill), bytes), pieces = (bytes - head) / 32, tail = bytes - head - pieces * 32;
-    if (first == 0) {
-        if (threadIdx.x < head) fill[threadIdx.x] = 0;
-        if (threadIdx.x < tail) lo[pieces * 32 + threadIdx.x] = 0;
-    }
-    const uint32_t zero[8] = {};
-    for (uint64_t i = first * blockDim.x + threadIdx.x; i < pieces; i += step * blockDim.x) store32(lo + 32 * i, zero);
-}
-
 // A table that is overwritten is filled with zeros where no token is: the first launch marks the rows that have one.
 __device__ __forceinline__ void mark(uint32_t* touched, uint32_t key, uint32_t vocab) {
     if (touched && key < vocab) atomicOr(&touched[key >> 5], 1u << (key & 31));
@@ -248,10 +235,6 @@ __device__ __forceinline__ void fill_row(unsigned char* row, uint64_t bytes) {
     for (uint64_t i = lane; i < pieces; i += 32) store32(lo + 32 * i, zero);
     if (lane < head) row[lane] = 0;
     if (lane < tail) lo[pieces * 32 + lane] = 0;
-}
-__global__ void __launch_bounds__(SORT_THREADS) k_embed_fill(unsigned char* fill, uint64_t fill_bytes) {
-    let_next();
-    fill_zeros(fill, fill_bytes, blockIdx.x, gridDim.x);
 }
 
 __device__ __forceinline__ uint32_t key_of(unsigned long long it) { return (uint32_t)(it >> 32); }
@@ -412,18 +395,72 @@ __global__ void __launch_bounds__(256) k_embed_join(const unsigned long long* __
     write_row<G, N>(d_table + (uint64_t)key * hidden + col, sum, scale, accumulate != 0);
 }
 
-// ---- gradient of up to DIRECT tokens in one launch (after the fill, when the table is overwritten). A block has one token and up to
-// 8 x 32 N columns: it leaves where an equal id stands before the token; else it lists the equal ones behind, in order, and sums their
-// rows, `splits` groups of warps a contiguous part of the list each, joined in order.
+// Zeros over the rows without a token of one of `blocks` stretches of the table, by the block of that number. Up to FILL_ROWS rows at a
+// time: the block marks the ones with a token in shared memory, then walks the stretch in aligned pieces of 32 bytes, whatever rows
+// they lie in; a piece that a row with a token, or the stretch's end, cuts goes by elements.
+constexpr uint32_t FILL_ROWS = 8192;
+template <typename G>
+__device__ void fill_without(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, unsigned char* table, uint32_t row_bytes, uint32_t block, uint32_t blocks) {
+    __shared__ uint32_t marks[FILL_ROWS / 32];
+    const uint64_t per = ((uint64_t)vocab + blocks - 1) / blocks, r0 = min(block * per, (uint64_t)vocab), r1 = min(r0 + per, (uint64_t)vocab);
+    const uint32_t at_once = min(FILL_ROWS, (1u << 31) / row_bytes);  // offsets within a stretch fit 32 bits
+    const uint32_t zero[8] = {};
+    for (uint64_t a = r0; a < r1; a += at_once) {
+        const uint64_t b = min(a + at_once, r1);
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < FILL_ROWS / 32; i += blockDim.x) marks[i] = 0;
+        __syncthreads();
+        for (uint32_t j = threadIdx.x; j < n; j += blockDim.x) {
+            const int64_t id = ids[j];
+            if (id >= (int64_t)a && id < (int64_t)b) atomicOr(&marks[(uint32_t)(id - a) >> 5], 1u << ((uint32_t)(id - a) & 31));
+        }
+        __syncthreads();
+        auto marked = [&](uint32_t row) { return marks[row >> 5] >> (row & 31) & 1; };
+        unsigned char* from = table + a * row_bytes;
+        const uint32_t bytes = (uint32_t)(b - a) * row_bytes, skew = (uint32_t)(reinterpret_cast<uintptr_t>(from) & 31);
+        const uint32_t pieces = (uint32_t)(((uint64_t)skew + bytes + 31) / 32);
+        for (uint32_t p = threadIdx.x; p < pieces; p += blockDim.x) {
+            const int64_t at = (int64_t)p * 32 - skew;  // of the piece, from the stretch's beginning
+            const uint32_t begin = at < 0 ? 0 : (uint32_t)at, stop = (uint32_t)min(at + 32, (int64_t)bytes);
+            uint32_t row = begin / row_bytes, row_end = (row + 1) * row_bytes;
+            bool some = false, all = stop - begin == 32;  // rows without a token lie in the piece; nothing else does
+            for (uint32_t r = row, end = row_end;; r++, end += row_bytes) {
+                if (marked(r)) all = false;
+                else some = true;
+                if (end >= stop) break;
+            }
+            if (all) {
+                store32(from + begin, zero);
+            } else if (some) {
+                for (uint32_t k = begin; k < stop; k += sizeof(G)) {
+                    if (k == row_end) {
+                        row++;
+                        row_end += row_bytes;
+                    }
+                    if (!marked(row)) *reinterpret_cast<G*>(from + k) = from_f32<G>(0.f);
+                }
+            }
+        }
+    }
+}
+
+// ---- gradient of up to DIRECT tokens in one launch. A block has one token and up to 8 x 32 N columns (`across` blocks a token): it
+// leaves where an equal id stands before the token; else it lists the equal ones behind, in order, and sums their rows, `splits` groups
+// of warps a contiguous part of the list each, joined in order. The blocks behind write zeros to the rows without a token, where the
+// table is overwritten: 590 x 128 bf16 of 4131 rows 4.6 us, 6.0 with a fill of the whole table in front; 786 x 837 f16 of 113836 rows 42 and
+// 43.5.
 template <typename T, typename G, int N>
 __global__ void __launch_bounds__(256) k_embed_direct(const int64_t* __restrict__ ids, uint32_t n, uint32_t vocab, const T* __restrict__ d_out,
-                                                      uint64_t stride, uint32_t hidden, G* d_table, float scale, int accumulate, uint32_t wide) {
+                                                      uint64_t stride, uint32_t hidden, G* d_table, float scale, int accumulate, uint32_t wide,
+                                                      uint32_t across) {
     __shared__ uint16_t list[DIRECT];
     __shared__ uint32_t counts[8];
     __shared__ float share[256 * N];
-    let_next();
-    after_previous();
-    const uint32_t i = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (blockIdx.x >= n * across) {
+        fill_without<G>(ids, n, vocab, reinterpret_cast<unsigned char*>(d_table), hidden * (uint32_t)sizeof(G), blockIdx.x - n * across, gridDim.x - n * across);
+        return;
+    }
+    const uint32_t i = blockIdx.x / across, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int64_t id = ids[i];
     if ((uint64_t)id >= vocab) return;
     bool before = false;
@@ -452,7 +489,7 @@ __global__ void __launch_bounds__(256) k_embed_direct(const int64_t* __restrict_
     }
     __syncthreads();
     // `wide` warps along a row, 8 / wide along the list
-    const uint32_t splits = 8 / wide, part = warp / wide, col = (blockIdx.y * wide + warp % wide) * 32 * N + lane * N;
+    const uint32_t splits = 8 / wide, part = warp / wide, col = ((blockIdx.x - i * across) * wide + warp % wide) * 32 * N + lane * N;
     const bool live = part < splits && col < hidden;
     float sum[N];
 #pragma unroll
@@ -501,9 +538,11 @@ int32_t sums(oxz_embed* e, uint32_t n, const int64_t* ids, const unsigned long l
     const oxz_embed_desc& d = e->d;
     const uint32_t slices = (uint32_t)((d.hidden + 32 * N - 1) / (32 * N)), vocab = (uint32_t)d.vocab, hidden = (uint32_t)d.hidden;
     if (n <= DIRECT) {
-        const uint32_t wide = std::min<uint32_t>(8, slices);
-        OXZ_CUDA(launch_after(!accumulate, k_embed_direct<T, G, N>, dim3(n, (slices + wide - 1) / wide), 256, 0, s, ids, n, vocab, static_cast<const T*>(d_out),
-                              stride, hidden, static_cast<G*>(d_table), (float)d.scale, accumulate, wide));
+        const uint32_t wide = std::min<uint32_t>(8, slices), across = (slices + wide - 1) / wide;
+        const uint64_t bytes = d.vocab * d.hidden * sizeof(G);
+        const unsigned fillers = accumulate ? 0 : (unsigned)std::min<uint64_t>(e->sms * 8, (bytes + (16 << 10) - 1) / (16 << 10));
+        OXZ_CUDA(launch_after(false, k_embed_direct<T, G, N>, n * across + fillers, 256, 0, s, ids, n, vocab, static_cast<const T*>(d_out), stride, hidden,
+                              static_cast<G*>(d_table), (float)d.scale, accumulate, wide, across));
         return OXZ_OK;
     }
     const uint32_t chunks = (n + CHUNK - 1) / CHUNK;
@@ -639,12 +678,7 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
         OXZ_TRY(e->order.begin(s));
         const unsigned long long* sorted = e->sorted[0];
         uint32_t* touched = accumulate ? nullptr : e->touched;
-        if (n <= DIRECT) {
-            const uint64_t bytes = d.vocab * d.hidden * gs;
-            if (!accumulate)  // blocks of 32 KiB at least
-                OXZ_CUDA(launch_after(false, k_embed_fill, (unsigned)std::min<uint64_t>(e->sms * 2, (bytes + (32 << 10) - 1) / (32 << 10)), SORT_THREADS, 0, s,
-                                      static_cast<unsigned char*>(d_table), bytes));
-        } else {
+        if (n > DIRECT) {
             if (touched && !e->clean) OXZ_CUDA(cudaMemsetAsync(touched, 0, (d.vocab + 31) / 32 * 4, s));
             if (touched) e->clean = false;  // until every launch of this call has been made
             if (n <= RANKED) {
@@ -670,7 +704,7 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
                 OXZ_CUDA(cudaLaunchKernelEx(&cfg, k_embed_sort, ids, (uint32_t)n, (uint32_t)d.vocab, passes, bits, e->sorted[0], e->sorted[1], touched));
             }
         }
-        if (n) {
+        {
             const bool wide = !misaligned(d_out, 16) && !misaligned(d_table, 16) && d.hidden * es % 16 == 0 && d_out_stride * es % 16 == 0;
             const uint32_t m = (uint32_t)n;
             const uint64_t st = d_out_stride;
