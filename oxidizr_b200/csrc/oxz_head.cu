@@ -1075,7 +1075,7 @@ struct Products {
                        const oxz_head_grads* gr, cudaStream_t s) {
         const oxz_head_desc& d = h->d;
         const bool on16 = !misaligned(b.hidden, 16) && b.hidden_stride * sizeof(T) % 16 == 0 && d.hidden * sizeof(T) % 16 == 0;
-        if (few_fits(b.rows, d.hidden, sizeof(T), on16))
+        if (few_fits(b.rows, d.hidden, d.vocab, sizeof(T), on16))
             return run_few(h, b, on16, row_loss, row_stats, want_loss, totals, gr, s);
         constexpr bool F32 = sizeof(T) == 4, BF16 = std::is_same<S, __nv_bfloat16>::value;
         const size_t es = sizeof(T);

@@ -767,7 +767,11 @@ inline size_t few_logit_bytes(int r, uint64_t hidden, size_t size, bool wide) {
     const uint64_t n = wide ? 16 / size : 1, pitch = (hidden + 32 * n - 1) / (32 * n) * (32 * n);
     return (size_t)r * pitch * 4 + (wide ? (size_t)(r == 4 ? 2 : r == 8 ? 3 : 4) * (64 / r) * FEW_THREADS * 16 : 0);
 }
-inline bool few_fits(uint64_t rows, uint64_t hidden, size_t size, bool wide) {
+// More than 8 rows of 16-bit values that do not lie on 16 bytes go this way only over a small weight: read by elements, 16 rows of
+// 345 x 20000 take 42 us for the losses and 91 with gradients, where the tiles take 24 and 67 (97 x 100000: 52 and 116, 38 and 123;
+// 97 x 2000: 13 and 27, 14 and 33).
+inline bool few_fits(uint64_t rows, uint64_t hidden, uint64_t vocab, size_t size, bool wide) {
+    if (size == 2 && !wide && rows > 8 && hidden * vocab > (1u << 20)) return false;
     return rows <= (uint64_t)FEW_ROWS && few_logit_bytes(few_kernel_rows(rows, size, wide), hidden, size, wide) + 8192 <= FEW_SHARED;
 }
 template <typename T, int R>

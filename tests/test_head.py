@@ -414,6 +414,27 @@ def test_a_handful_of_rows(dtype, grad, rows, hidden, vocab, mask, gap, accumula
 
 
 @gpu
+@pytest.mark.parametrize("dtype, grad", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("rows, hidden, vocab", [(8, 345, 4000), (9, 345, 4000), (16, 345, 4000), (9, 345, 3000), (16, 517, 2500)])
+def test_a_handful_of_odd_rows_over_a_larger_weight(dtype, grad, rows, hidden, vocab):
+    """Rows off 16-byte bounds on both sides of what goes by streams of the weight and by tiles; losses alone, then their gradients."""
+    import torch
+    pr = Problem(dtype, rows, hidden, vocab, "weights", seed=rows, grad=grad).solve(scale=0.5)
+    h = ox.LossHead(vocab, hidden, rows, dtype=NAMES[dtype], grad_dtype=NAMES[grad])
+    o = pr.outputs()
+    h.loss_and_grads(**pr.batch(), **ptrs(o), grad_scale=0.5)
+    torch.cuda.synchronize()
+    pr.check(o, o)
+    q = pr.outputs()
+    h.loss(**pr.batch(), row_loss=q["row_loss"].data_ptr(), row_stats=q["row_stats"].data_ptr(), totals=q["totals"].data_ptr())
+    h.grads(**pr.batch(), row_stats=q["row_stats"].data_ptr(), d_hidden=q["d_hidden"].data_ptr(), d_weight=q["d_weight"].data_ptr(), grad_scale=0.5)
+    torch.cuda.synchronize()
+    for k in o:
+        assert torch.equal(o[k], q[k]), k
+    h.destroy()
+
+
+@gpu
 @pytest.mark.parametrize("dtype, grad", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("f16", "f32")])
 @pytest.mark.parametrize("rows, hidden, vocab, piece_bytes", [(40, 1024, 1500, 0), (600, 1040, 2500, 0), (600, 1040, 2500, 4 << 20), (1300, 264, 3000, 5 << 20),
                                                              (2100, 72, 5000, 0), (1025, 512, 700, 1)])
