@@ -415,22 +415,24 @@ struct Split {
     __host__ __device__ uint32_t items() const { return whole + rest * shares; }
 };
 
-// exp(x - m). f32 results take the library's exponential. For 16-bit operands the unit's 2^x of one fused product is ample: it is
-// off by 2^-22 and by 2^-24 |m log2 e| relatively, where the operands themselves are rounded to 2^-9 or 2^-12.
+// exp(x - m). f32 results take the library's exponential. For 16-bit operands the unit's 2^x is ample: it is off by 2^-22, and the
+// rounding of its argument by 2^-24 |x - m| log2 e, relatively, where the operands themselves are rounded to 2^-9 or 2^-12. The
+// difference is formed first: the largest logit's own term is 1 and the sums hold f32's digits (x log2 e - m log2 e in one fused
+// product leaves the rounding of m log2 e in every term of a row: at logits of 200 a sure row's loss was up to 1e-5 off, and negative).
 constexpr float LOG2E = 1.4426950408889634f;
 template <bool EXACT> struct ExpFrom {
     float m;
-    __device__ __forceinline__ explicit ExpFrom(float at) : m(EXACT ? at : at * LOG2E) {}
+    __device__ __forceinline__ explicit ExpFrom(float at) : m(at) {}
     __device__ __forceinline__ float operator()(float x) const {
         if constexpr (EXACT) return expf(x - m);
         float r;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(x, LOG2E, -m)));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((x - m) * LOG2E));
         return r;
     }
     // of two, the same bits as of each
     __device__ __forceinline__ float2 operator()(float2 x) const {
         if constexpr (EXACT) return make_float2(expf(x.x - m), expf(x.y - m));
-        const float2 t = fma2(x, make_float2(LOG2E, LOG2E), make_float2(-m, -m));
+        const float2 t = mul2(add2(x, make_float2(-m, -m)), make_float2(LOG2E, LOG2E));
         float2 r;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(t.x));
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(t.y));
