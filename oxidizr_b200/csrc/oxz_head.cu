@@ -355,7 +355,9 @@ __global__ void __launch_bounds__(LISTED) k_head_list_pack(const int64_t* __rest
 // from tensor memory while the other of its two buffers fills.
 // The tensor cores cut, not round, what they add to an accumulator: over K = 2048 the logits lose 2e-6 of the loss, over the
 // vocabulary of an f32 gradient 1e-5. Where that shows (RUN > 0) an accumulator holds RUN steps of K only and the runs are added in
-// f32 registers, rounded; parts of a value are added the small ones first.
+// f32 registers, rounded; parts of a value are added the small ones first. A cut goes one way, so the batch's total keeps what its rows
+// lose: 16-bit logits of hidden 2048 by runs of 4 are 2e-7 of the loss off, rows and total (bf16; f16 2.6e-7); runs of 8 leave
+// 4.4e-7 (5.5e-7) in 1 to 2 % less time (8192 x 2048 x 128256 bf16 with gradients 13.69 ms, 13.84), runs of 2 1e-7 in 9 % more.
 //   LOGITS_STATS  l = X W^T: each row's {max, sum of exp} over half a tile's columns goes out, and the target's logit
 //   LOGITS_GRAD   the same tile, turned into G
 //   D_HIDDEN      G W, summed over the pieces in f32; its tiles are few and long (K is a piece of the vocabulary): see Split
@@ -500,8 +502,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
     constexpr bool A_LINES = P == D_WEIGHT, B_LINES = P == D_HIDDEN || P == D_WEIGHT, LOGITS = P == LOGITS_STATS || P == LOGITS_GRAD;
     constexpr bool F32 = sizeof(T) == 4;
     // steps of K that stay in an accumulator (0: all): see above. f32 operands add 6 products of 64 a step, the five small ones first;
-    // d_hidden and d_weight in 16 bits hide the cut
-    constexpr uint32_t RUN = F32 ? 2 : LOGITS ? 8 : P == D_WEIGHT && sizeof(G) == 4 ? 4 : 0;
+    // d_hidden and d_weight in 16 bits hide the cut. 16-bit logits of up to WHOLE steps stay in one: what they lose is small (8e-8 of the
+    // loss at hidden 384, 5e-8 by runs), and a way out more would cost the batch 4 % (8191 x 384 x 32000)
+    constexpr uint32_t RUN = F32 ? 2 : LOGITS || (P == D_WEIGHT && sizeof(G) == 4) ? 4 : 0, WHOLE = LOGITS && !F32 ? 8 : 0;
+    auto run_of = [](uint32_t steps) { return RUN == 0 || steps <= WHOLE ? steps : RUN; };
     extern __shared__ __align__(16) unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
     const uint32_t bars = base + STAGES * STAGE_BYTES + EPILOGUE_WARPS * OUT_BYTES;
@@ -581,7 +585,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         bool ok = true;
         for (uint32_t t = blockIdx.x / 2; t < items && ok; t += pairs) {
             const Tile c = tile_at(t);
-            const uint32_t b_boxes = c.half > 64 ? 2 : 1, run = RUN ? RUN : c.steps;
+            const uint32_t b_boxes = c.half > 64 ? 2 : 1, run = run_of(c.steps);
             for (uint32_t k1 = 0; k1 < c.steps && ok; k1 += run) {
                 for (uint32_t p = 0; p < (uint32_t)a.n_pairs && ok; p++) {
                     const int32_t za = a.pair_a[p], zb = a.pair_b[p];
@@ -616,7 +620,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
         bool ok = true;
         for (uint32_t t = blockIdx.x / 2; t < items && ok; t += pairs) {
             const Tile c = tile_at(t);
-            const uint32_t idesc = instruction(a.bf16, A_LINES, B_LINES, MMA_M, c.width), run = RUN ? RUN : c.steps;
+            const uint32_t idesc = instruction(a.bf16, A_LINES, B_LINES, MMA_M, c.width), run = run_of(c.steps);
             for (uint32_t k1 = 0; k1 < c.steps && ok; k1 += run, round++) {
                 const uint32_t total = min(run, c.steps - k1) * a.n_pairs, buf = round & 1, d = tmem + buf * 256;
                 if (!(ok = mbar_wait(taken(buf), ((round >> 1) & 1) ^ 1, ws))) break;
@@ -695,7 +699,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                     for (int j = 0; j < 32; j++) acc[q][j] = 0.f;
             }
             if constexpr (RUN > 0) {
-                for (uint32_t k1 = RUN; k1 < c.steps; k1 += RUN) {
+                for (uint32_t k1 = run_of(c.steps); k1 < c.steps; k1 += RUN) {
                     const uint32_t at = run_done();
                     if (!ok) break;
 #pragma unroll
@@ -705,7 +709,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMA_THREADS, 1)
                         tmem_wait();
                         arrived(x);
 #pragma unroll
-                        for (int j = 0; j < 16; j++) acc[e / 2][16 * (e & 1) + j] += x[j];
+                        for (int j = 0; j < 16; j += 2) {
+                            float* to = &acc[e / 2][16 * (e & 1) + j];
+                            const float2 sum = add2(make_float2(to[0], to[1]), make_float2(x[j], x[j + 1]));
+                            to[0] = sum.x;
+                            to[1] = sum.y;
+                        }
                     }
                     run_taken();
                 }

@@ -67,3 +67,70 @@ def test_losses_of_sure_rows(dtype, rows, gap):
     assert not bad.any(), (int(bad.sum()), (np.abs(got - np.log1p(o)) / tol).max())
     assert abs(float(totals[0]) - np.log1p(o).sum()) <= tol.sum() + U * rows
     h.destroy()
+
+
+def cut_steps(X, W, t, run):
+    """What an accumulator of f32 that is cut, not rounded, at each 16 of K may lose of every row's logit of its target, the sums begun
+    anew each `run` steps of 64: (at most, on the mean) - a whole and a half step of the accumulator after each addition."""
+    most = np.zeros(len(X))
+    at = np.zeros(len(X))
+    for k in range(0, X.shape[1], 16):
+        if k % (64 * run) == 0:
+            at = np.zeros(len(X))
+        at = at + (X[:, k:k + 16] * W[t, k:k + 16]).sum(1)
+        most += np.exp2(np.floor(np.log2(np.abs(at))) - 23)
+    return most, most / 2
+
+
+@gpu
+@pytest.mark.parametrize("dtype, run", [("bf16", 4), ("f16", 4), ("f32", 2)])
+@pytest.mark.parametrize("hidden", [512, 2048])
+def test_long_sums_keep_their_digits(dtype, run, hidden):
+    """Logits near 40 whose products are all positive, beside a word whose logit, 46, is a single product: the loss is the
+    difference, and takes over whole what the sum of the products loses. 512 of K stay in one accumulator of 16-bit operands."""
+    import torch
+    t = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    rows, vocab, words = 512, 1000, 50
+    rng = np.random.default_rng(hidden)
+    x = rng.uniform(0.5, 1.5, (rows, hidden))
+    w = rng.uniform(-0.01, 0.01, (vocab, hidden))
+    w[:words] = rng.uniform(0.0, 80.0 / hidden, (words, hidden))
+    w[:, 0] = 0.0
+    w[words] = 0.0
+    x[:, 0], w[words, 0] = 1.0, 46.0
+    d_x, d_w = torch.from_numpy(x).cuda().to(t), torch.from_numpy(w).cuda().to(t)
+    targets = rng.integers(0, words, rows)
+    d_t = torch.from_numpy(targets).cuda()
+    X, W = d_x.double().cpu().numpy(), d_w.double().cpu().numpy()
+    logits = X @ W.T
+    m = logits.max(1)
+    want = np.log(np.exp(logits - m[:, None]).sum(1)) + m - logits[np.arange(rows), targets]
+    assert np.all(m == 46.0) and want.min() > 1.0
+    if dtype != "f32" and hidden <= 512:
+        run = 8
+    most, mean = cut_steps(X, W, targets, run)
+    if dtype == "f32":
+        # five more products of the parts stand in a run before the largest: below 2^-6 of it together, cut at the same places, and
+        # what the six products leave out is below 3 * 2^-24 of the sum
+        most, mean = most * (1 + 2.0 ** -6) + 3 * U * 60, mean * (1 + 2.0 ** -6) + 3 * U * 60
+    # runs are joined by rounded additions, U each of a sum below 64; the other terms of the loss as above
+    joins = hidden // 64 // run
+    if dtype == "f16":
+        # a product of two f16 has 22 bits (of two bf16 16). Here it is below 1.5 * 80 / hidden < 2^-2 (hidden 512) and its last bit
+        # 2^-21 of its first, while the sum's step is 2^-23 of a sum that passes 1 after a few instructions: bits of every product lie below
+        # the step, and each of an instruction's 16 products may be cut by up to a step as the accumulator is: 17 steps at most,
+        # half of them on the mean
+        most, mean = 17 * most, 17 * mean
+    most, rest = most + joins * 64 * U, 48 * U
+    h = ox.LossHead(vocab, hidden, rows, dtype=NAMES[dtype])
+    loss, totals = torch.empty(rows, device="cuda"), torch.empty(2, device="cuda")
+    torch.cuda.synchronize()
+    h.loss(rows, d_x.data_ptr(), d_w.data_ptr(), d_t.data_ptr(), row_loss=loss.data_ptr(), totals=totals.data_ptr())
+    torch.cuda.synchronize()
+    off = loss.double().cpu().numpy() - want
+    assert np.all(np.abs(off) <= most + rest), (np.abs(off) / (most + rest)).max()
+    # the cuts are spread evenly over a step: of 512 rows the mean is known to a few hundredths; 1.3 leaves room and is well below the
+    # 2 of runs twice as long
+    assert abs(off.mean()) <= 1.3 * mean.mean() + 8 * U, (off.mean(), mean.mean())
+    assert abs(float(totals[0]) - want.sum()) <= rows * (1.3 * mean.mean() + 8 * U) + U * want.sum()
+    h.destroy()
