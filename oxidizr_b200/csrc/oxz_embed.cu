@@ -525,11 +525,12 @@ __global__ void __launch_bounds__(256) k_embed_direct(const int64_t* __restrict_
 bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) % to) != 0; }
 
 template <typename T, int N>
-void lookup(const oxz_embed_desc& d, const int64_t* ids, uint64_t n, const void* table, void* out, uint64_t stride, cudaStream_t s) {
+int32_t lookup(const oxz_embed_desc& d, const int64_t* ids, uint64_t n, const void* table, void* out, uint64_t stride, cudaStream_t s) {
     const uint32_t pieces = (uint32_t)((d.hidden + 128 * N - 1) / (128 * N));
     const uint64_t blocks = std::min<uint64_t>((n * pieces + 7) / 8, 1u << 30);
-    k_embed_lookup<T, N><<<(unsigned)blocks, 256, 0, s>>>(ids, n, static_cast<const T*>(table), static_cast<T*>(out), stride,
-                                                         (uint32_t)d.hidden, d.vocab, (float)d.scale, pieces);
+    OXZ_CUDA(launch_after(false, k_embed_lookup<T, N>, (unsigned)blocks, 256, 0, s, ids, n, static_cast<const T*>(table), static_cast<T*>(out), stride,
+                          (uint32_t)d.hidden, d.vocab, (float)d.scale, pieces));
+    return OXZ_OK;
 }
 
 template <typename T, typename G, int N>
@@ -648,11 +649,9 @@ int32_t oxz_embed_lookup_async(const oxz_embed* e, const int64_t* ids, uint64_t 
         OXZ_TRY(dev.enter(d.device));
         cudaStream_t s = (cudaStream_t)stream;
         const bool wide = !misaligned(table, 16) && !misaligned(out, 16) && d.hidden * es % 16 == 0 && out_stride * es % 16 == 0;
-        if (d.dtype == OXZ_F32) wide ? lookup<float, 4>(d, ids, n, table, out, out_stride, s) : lookup<float, 1>(d, ids, n, table, out, out_stride, s);
-        else if (d.dtype == OXZ_BF16) wide ? lookup<__nv_bfloat16, 8>(d, ids, n, table, out, out_stride, s) : lookup<__nv_bfloat16, 1>(d, ids, n, table, out, out_stride, s);
-        else wide ? lookup<__half, 8>(d, ids, n, table, out, out_stride, s) : lookup<__half, 1>(d, ids, n, table, out, out_stride, s);
-        OXZ_CUDA(cudaGetLastError());
-        return OXZ_OK;
+        if (d.dtype == OXZ_F32) return wide ? lookup<float, 4>(d, ids, n, table, out, out_stride, s) : lookup<float, 1>(d, ids, n, table, out, out_stride, s);
+        if (d.dtype == OXZ_BF16) return wide ? lookup<__nv_bfloat16, 8>(d, ids, n, table, out, out_stride, s) : lookup<__nv_bfloat16, 1>(d, ids, n, table, out, out_stride, s);
+        return wide ? lookup<__half, 8>(d, ids, n, table, out, out_stride, s) : lookup<__half, 1>(d, ids, n, table, out, out_stride, s);
     });
 }
 
@@ -715,7 +714,6 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
             else if (!f32g) OXZ_TRY((wide ? sums<__half, __half, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__half, __half, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
             else OXZ_TRY((wide ? sums<__half, float, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__half, float, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
         }
-        OXZ_CUDA(cudaGetLastError());
         if (n > DIRECT && touched) e->clean = true;
         return e->order.end(s);
     });

@@ -1250,7 +1250,6 @@ int32_t call(const char* who, oxz_head* h, const oxz_head_batch* batch, float* r
     const oxz_head_grads* gp = want_grads ? &g : nullptr;
     const int32_t rc = with_types(d, [&](auto p) { return decltype(p)::run(h, b, row_loss, st, want_loss, totals, gp, s); });
     OXZ_TRY(rc);
-    OXZ_CUDA(cudaGetLastError());
     return h->order.end(s);
 }
 

@@ -34,12 +34,15 @@ inline int32_t guarded(const char* who, F&& body) noexcept {
     }
 }
 
+// An error is reported here once: the runtime is not left with it for a later call to find.
 #define OXZ_CUDA(expr)                                                                              \
     do {                                                                                            \
         cudaError_t e__ = (expr);                                                                   \
-        if (e__ != cudaSuccess)                                                                     \
+        if (e__ != cudaSuccess) {                                                                   \
+            (void)cudaGetLastError();                                                               \
             return ::oxz::fail(OXZ_ERR_CUDA, "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e__), \
                                __FILE__, __LINE__);                                                 \
+        }                                                                                           \
     } while (0)
 
 #define OXZ_TRY(expr)                  \

@@ -1,0 +1,103 @@
+// The token operators' calls on the host, over a runtime of notes (fake_cuda.hpp): what they enqueue, in what order, and what is left
+// when one of the runtime's calls fails in the middle.
+#include <cstring>
+#include <functional>
+
+#include "../../include/oxz_dpstep.h"
+#include "fake_cuda.hpp"
+
+static int failures = 0;
+#define EXPECT(c, ...)                                                          \
+    do {                                                                        \
+        if (!(c)) {                                                             \
+            std::printf("FAILED %s:%d: %s ", __FILE__, __LINE__, #c);           \
+            std::printf(" " __VA_ARGS__);                                       \
+            std::printf("\n");                                                  \
+            failures++;                                                         \
+        }                                                                       \
+    } while (0)
+
+static const cudaStream_t A = (cudaStream_t)0x1000;
+static void* const p = (void*)(1 << 20);  // an address that no kernel reads here
+
+// A handle and the call it is tested with
+struct Operator {
+    const char* name;
+    std::function<void*()> make;
+    std::function<int32_t(void*, cudaStream_t)> call;
+    std::function<void(void*)> destroy;
+};
+
+static void* embed(uint64_t tokens) {
+    const oxz_embed_desc d{tokens, 64, 1000, 1.0, OXZ_BF16, OXZ_BF16, 0, 0};
+    oxz_embed* e = nullptr;
+    EXPECT(oxz_embed_create(&d, &e) == OXZ_OK);
+    EXPECT(oxz_embed_alloc(e, nullptr) == OXZ_OK);
+    return e;
+}
+static void* head(uint64_t rows, uint64_t vocab, uint64_t piece_bytes) {
+    const oxz_head_desc d{rows, 64, vocab, piece_bytes, OXZ_BF16, OXZ_BF16, 0, 0};
+    oxz_head* h = nullptr;
+    EXPECT(oxz_head_create(&d, &h) == OXZ_OK);
+    EXPECT(oxz_head_alloc(h, nullptr) == OXZ_OK);
+    return h;
+}
+static Operator embed_grads(const char* name, uint64_t n, int accumulate) {
+    return {name, [=] { return embed(n); },
+            [=](void* h, cudaStream_t s) { return oxz_embed_grads_async((oxz_embed*)h, (const int64_t*)p, n, p, 0, p, accumulate, s); },
+            [](void* h) { oxz_embed_destroy((oxz_embed*)h); }};
+}
+static Operator head_train(const char* name, uint64_t rows, uint64_t vocab, uint64_t piece_bytes) {
+    return {name, [=] { return head(rows, vocab, piece_bytes); },
+            [=](void* h, cudaStream_t s) {
+                const oxz_head_batch b{rows, p, 0, p, (const int64_t*)p, nullptr};
+                const oxz_head_grads g{p, 0, p, 1.0, 0, 0};
+                return oxz_head_loss_grads_async((oxz_head*)h, &b, (float*)p, (float*)p, (float*)p, &g, s);
+            },
+            [](void* h) { oxz_head_destroy((oxz_head*)h); }};
+}
+static std::vector<Operator> operators() {
+    return {embed_grads("embed 100", 100, 0), embed_grads("embed 2000", 2000, 0), embed_grads("embed 9000", 9000, 0), embed_grads("embed 9000 added", 9000, 1),
+            head_train("head 5", 5, 500, 0), head_train("head 40", 40, 500, 0), head_train("head 2000 in pieces", 2000, 3000, 1)};
+}
+// An error is the failing call's: what runs after it is not refused for it, on the same handle or another.
+static void an_error_is_reported_once() {
+    for (const Operator& op : operators()) {
+        void* h = op.make();
+        fake::memory = 1 << 10;
+        const oxz_head_desc d{40, 64, 500, 0, OXZ_F32, OXZ_F32, 0, 0};
+        oxz_head* large = nullptr;
+        EXPECT(oxz_head_create(&d, &large) == OXZ_OK);
+        EXPECT(oxz_head_alloc(large, nullptr) == OXZ_ERR_CUDA);
+        oxz_head_destroy(large);
+        fake::memory = ~size_t(0);
+        EXPECT(op.call(h, A) == OXZ_OK, "%s: %s", op.name, fake::message.c_str());
+        fake::last = cudaErrorInvalidValue;  // what some other part of the program left
+        EXPECT(op.call(h, A) == OXZ_OK, "%s: %s", op.name, fake::message.c_str());
+        fake::last = cudaSuccess;
+        fake::fail_at = 1;  // the first launch
+        EXPECT(op.call(h, A) == OXZ_ERR_CUDA, "%s", op.name);
+        EXPECT(op.call(h, A) == OXZ_OK, "%s: %s", op.name, fake::message.c_str());
+        op.destroy(h);
+    }
+    const oxz_embed_desc d{8, 64, 1000, 1.0, OXZ_BF16, OXZ_BF16, 0, 0};
+    oxz_embed* e = nullptr;
+    EXPECT(oxz_embed_create(&d, &e) == OXZ_OK);
+    fake::last = cudaErrorInvalidValue;
+    EXPECT(oxz_embed_lookup_async(e, (const int64_t*)p, 8, p, p, 0, A) == OXZ_OK, "%s", fake::message.c_str());
+    fake::fail_at = 0;
+    EXPECT(oxz_embed_lookup_async(e, (const int64_t*)p, 8, p, p, 0, A) == OXZ_ERR_CUDA);
+    EXPECT(oxz_embed_lookup_async(e, (const int64_t*)p, 8, p, p, 0, A) == OXZ_OK, "%s", fake::message.c_str());
+    fake::last = cudaSuccess;
+    oxz_embed_destroy(e);
+}
+
+int main(int argc, char** argv) {
+    const struct { const char* name; void (*run)(); } tests[] = {
+        {"error", an_error_is_reported_once},
+    };
+    for (const auto& t : tests)
+        if (argc < 2 || std::strcmp(argv[1], t.name) == 0) t.run();
+    std::printf(failures ? "%d failed\n" : "all passed\n", failures);
+    return failures != 0;
+}
