@@ -674,7 +674,8 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
         DeviceGuard dev;
         OXZ_TRY(dev.enter(d.device));
         cudaStream_t s = (cudaStream_t)stream;
-        OXZ_TRY(e->order.begin(s));
+        Turn turn(e->order);
+        OXZ_TRY(turn.begin(s));
         const unsigned long long* sorted = e->sorted[0];
         uint32_t* touched = accumulate ? nullptr : e->touched;
         if (n > DIRECT) {
@@ -715,7 +716,7 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
             else OXZ_TRY((wide ? sums<__half, float, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__half, float, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
         }
         if (n > DIRECT && touched) e->clean = true;
-        return e->order.end(s);
+        return turn.end();
     });
 }
 

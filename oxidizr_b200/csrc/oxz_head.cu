@@ -1245,12 +1245,13 @@ int32_t call(const char* who, oxz_head* h, const oxz_head_batch* batch, float* r
     DeviceGuard dev;
     OXZ_TRY(dev.enter(d.device));
     cudaStream_t s = (cudaStream_t)stream;
-    OXZ_TRY(h->order.begin(s));
+    Turn turn(h->order);
+    OXZ_TRY(turn.begin(s));
     float2* st = reinterpret_cast<float2*>(row_stats);
     const oxz_head_grads* gp = want_grads ? &g : nullptr;
     const int32_t rc = with_types(d, [&](auto p) { return decltype(p)::run(h, b, row_loss, st, want_loss, totals, gp, s); });
     OXZ_TRY(rc);
-    return h->order.end(s);
+    return turn.end();
 }
 
 }  // namespace

@@ -102,26 +102,39 @@ struct StreamOrder {
         if (done) cudaEventDestroy(done);
         done = nullptr;
     }
-    static int32_t capturing(cudaStream_t s, bool* yes) {
+};
+
+// One call's turn in its handle's order: from begin() to end(), or, where the call breaks off between the two, to the end of the scope.
+// What it has launched by then uses the workspace as a whole call does, and the next call waits for it.
+class Turn {
+  public:
+    explicit Turn(StreamOrder& order) : order_(order) {}
+    Turn(const Turn&) = delete;
+    Turn& operator=(const Turn&) = delete;
+    ~Turn() { (void)end(); }
+    int32_t begin(cudaStream_t s) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         OXZ_CUDA(cudaStreamIsCapturing(s, &st));
-        *yes = st != cudaStreamCaptureStatusNone;
+        captured_ = st != cudaStreamCaptureStatusNone;
+        if (captured_) return OXZ_OK;
+        if (order_.used) OXZ_CUDA(cudaStreamWaitEvent(s, order_.done, 0));
+        stream_ = s;
+        running_ = true;
         return OXZ_OK;
     }
-    int32_t begin(cudaStream_t s) {
-        bool captured = false;
-        OXZ_TRY(capturing(s, &captured));
-        if (!captured && used) OXZ_CUDA(cudaStreamWaitEvent(s, done, 0));
+    int32_t end() {
+        if (!running_) return OXZ_OK;
+        OXZ_CUDA(cudaEventRecord(order_.done, stream_));  // one that fails is tried again at the end of the scope
+        running_ = false;
+        order_.used = true;
         return OXZ_OK;
     }
-    int32_t end(cudaStream_t s) {
-        bool captured = false;
-        OXZ_TRY(capturing(s, &captured));
-        if (captured) return OXZ_OK;
-        OXZ_CUDA(cudaEventRecord(done, s));
-        used = true;
-        return OXZ_OK;
-    }
+    bool captured() const { return captured_; }
+
+  private:
+    StreamOrder& order_;
+    cudaStream_t stream_ = nullptr;
+    bool captured_ = false, running_ = false;
 };
 
 constexpr uint32_t TILE = 256;           // elements per tile: one 8-element vector per lane of a warp

@@ -17,7 +17,7 @@ static int failures = 0;
         }                                                                       \
     } while (0)
 
-static const cudaStream_t A = (cudaStream_t)0x1000;
+static const cudaStream_t A = (cudaStream_t)0x1000, B = (cudaStream_t)0x2000;
 static void* const p = (void*)(1 << 20);  // an address that no kernel reads here
 
 // A handle and the call it is tested with
@@ -92,9 +92,46 @@ static void an_error_is_reported_once() {
     oxz_embed_destroy(e);
 }
 
+static bool works(const fake::Op& o) { return o.kind == fake::LAUNCH || o.kind == fake::CLEAR; }
+
+// A call that breaks off has launched kernels that use the handle's workspace: the next call, on another stream, waits for them.
+static void the_next_call_waits_for_one_that_broke_off() {
+    for (const Operator& op : operators()) {
+        for (int k = 0;; k++) {
+            void* h = op.make();
+            EXPECT(op.call(h, A) == OXZ_OK, "%s", op.name);
+            fake::ops.clear();
+            fake::fail_at = k;
+            const int32_t rc = op.call(h, A);
+            const bool reached = fake::fail_at < 0;
+            fake::fail_at = -1;
+            if (!reached) {
+                EXPECT(rc == OXZ_OK && k > 2, "%s: %d calls", op.name, k);
+                op.destroy(h);
+                break;
+            }
+            EXPECT(rc == OXZ_ERR_CUDA, "%s: call %d failed", op.name, k);
+            int work = -1, record = -1;
+            for (int i = 0; i < (int)fake::ops.size(); i++) {
+                if (works(fake::ops[i])) work = i;
+                if (fake::ops[i].kind == fake::RECORD) record = i;
+            }
+            const size_t before = fake::ops.size();
+            EXPECT(op.call(h, B) == OXZ_OK, "%s: after call %d failed: %s", op.name, k, fake::message.c_str());
+            if (work >= 0 && rc != OXZ_OK) {
+                EXPECT(record > work, "%s: call %d failed, nothing marks the end of what was launched", op.name, k);
+                EXPECT(fake::ops[before].kind == fake::WAIT && fake::ops[before].stream == B && record >= 0 && fake::ops[before].what == fake::ops[record].what,
+                       "%s: call %d failed, the next does not wait", op.name, k);
+            }
+            op.destroy(h);
+        }
+    }
+}
+
 int main(int argc, char** argv) {
     const struct { const char* name; void (*run)(); } tests[] = {
         {"error", an_error_is_reported_once},
+        {"broke_off", the_next_call_waits_for_one_that_broke_off},
     };
     for (const auto& t : tests)
         if (argc < 2 || std::strcmp(argv[1], t.name) == 0) t.run();

@@ -46,3 +46,7 @@ def run(name):
 
 def test_an_error_is_reported_once():
     run("error")
+
+
+def test_the_next_call_waits_for_one_that_broke_off():
+    run("broke_off")
