@@ -22,7 +22,7 @@ struct oxz_embed {
     unsigned long long* sorted[2] = {nullptr, nullptr};  // token << 32 | position, max_tokens each
     float* carry = nullptr;                              // [chunks][2][hidden]: partial sums of the tokens that cross chunks
     uint32_t* touched = nullptr;                         // a bit for every row of the table: it has a token. All 0 between calls
-    bool clean = false;                                  // ... unless a call broke off
+    bool clean = false;                                  // ... unless a call broke off, and clearing them failed as well
     int sms = 0;
     oxz::StreamOrder order;
 };
@@ -522,6 +522,25 @@ __global__ void __launch_bounds__(256) k_embed_direct(const int64_t* __restrict_
     if (live) write_row<G, N>(d_table + (uint64_t)id * hidden + col, sum, scale, accumulate != 0);
 }
 
+uint64_t mark_bytes(const oxz_embed_desc& d) { return (d.vocab + 31) / 32 * 4; }
+
+// From the first launch of a call that marks rows to the last, which takes the marks away. A call that breaks off in between clears them
+// itself: the next call relies on it, and so do graphs captured before. (A captured call runs nothing now and changes nothing.)
+struct Marking {
+    oxz_embed* e;
+    cudaStream_t s;
+    bool open = false;
+    void close() {
+        if (open) e->clean = true;
+        open = false;
+    }
+    ~Marking() {
+        if (!open) return;
+        e->clean = cudaMemsetAsync(e->touched, 0, mark_bytes(e->d), s) == cudaSuccess;
+        if (!e->clean) (void)cudaGetLastError();
+    }
+};
+
 bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) % to) != 0; }
 
 template <typename T, int N>
@@ -600,14 +619,14 @@ int32_t oxz_embed_alloc(oxz_embed* e, uint64_t* workspace_bytes) {
             for (int i = 0; i < 2; i++)
                 if (!e->sorted[i]) OXZ_CUDA(cudaMalloc((void**)&e->sorted[i], items));
             if (!e->carry) OXZ_CUDA(cudaMalloc((void**)&e->carry, carry));
-            if (!e->touched) OXZ_CUDA(cudaMalloc((void**)&e->touched, (e->d.vocab + 31) / 32 * 4));
-            OXZ_CUDA(cudaMemset(e->touched, 0, (e->d.vocab + 31) / 32 * 4));
+            if (!e->touched) OXZ_CUDA(cudaMalloc((void**)&e->touched, mark_bytes(e->d)));
+            OXZ_CUDA(cudaMemset(e->touched, 0, mark_bytes(e->d)));
             OXZ_CUDA(cudaDeviceSynchronize());
             e->clean = true;
             OXZ_CUDA(cudaDeviceGetAttribute(&e->sms, cudaDevAttrMultiProcessorCount, e->d.device));
             OXZ_TRY(e->order.create());
             OXZ_CUDA(cudaFuncSetAttribute(k_embed_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared)));
-            e->bytes = 2 * items + carry + (e->d.vocab + 31) / 32 * 4;
+            e->bytes = 2 * items + carry + mark_bytes(e->d);
             e->allocated = true;
         }
         if (workspace_bytes) *workspace_bytes = e->bytes;
@@ -678,9 +697,10 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
         OXZ_TRY(turn.begin(s));
         const unsigned long long* sorted = e->sorted[0];
         uint32_t* touched = accumulate ? nullptr : e->touched;
+        Marking marking{e, s};
         if (n > DIRECT) {
-            if (touched && !e->clean) OXZ_CUDA(cudaMemsetAsync(touched, 0, (d.vocab + 31) / 32 * 4, s));
-            if (touched) e->clean = false;  // until every launch of this call has been made
+            if (touched && !e->clean) OXZ_CUDA(cudaMemsetAsync(touched, 0, mark_bytes(d), s));
+            marking.open = touched && !turn.captured();
             if (n <= RANKED) {
                 const uint32_t tokens = std::min<uint32_t>(64, ((uint32_t)n + e->sms - 1) / e->sms), parts = tokens <= 32 ? 32 : 16;
                 OXZ_CUDA(launch_after(false, parts == 32 ? k_embed_rank<32> : k_embed_rank<16>, ((unsigned)n + tokens - 1) / tokens, (tokens * parts + 31) / 32 * 32, 0,
@@ -715,7 +735,7 @@ int32_t oxz_embed_grads_async(oxz_embed* e, const int64_t* ids, uint64_t n, cons
             else if (!f32g) OXZ_TRY((wide ? sums<__half, __half, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__half, __half, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
             else OXZ_TRY((wide ? sums<__half, float, 8>(e, m, ids, sorted, d_out, st, d_table, accumulate, s) : sums<__half, float, 1>(e, m, ids, sorted, d_out, st, d_table, accumulate, s)));
         }
-        if (n > DIRECT && touched) e->clean = true;
+        marking.close();
         return turn.end();
     });
 }

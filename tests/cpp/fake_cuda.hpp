@@ -26,7 +26,7 @@ struct Op {
 
 inline std::mutex lock;
 inline std::vector<Op> ops;             // what has been enqueued
-inline int fail_at = -1;                // this many enqueueing calls from now, one fails
+inline int fail_at = -1, fail_for = 1;  // this many enqueueing calls from now, so many in a row fail
 inline size_t memory = ~size_t(0);      // the largest allocation that succeeds
 inline std::set<cudaStream_t> capturing;
 inline thread_local cudaError_t last = cudaSuccess;
@@ -38,7 +38,11 @@ inline cudaError_t result(cudaError_t e) {
 }
 inline cudaError_t enqueue(Kind k, cudaStream_t s, const void* what) {
     std::lock_guard<std::mutex> hold(lock);
-    if (fail_at >= 0 && fail_at-- == 0) return result(cudaErrorLaunchOutOfResources);
+    if (fail_at == 0) {
+        if (--fail_for == 0) fail_at = -1, fail_for = 1;
+        return result(cudaErrorLaunchOutOfResources);
+    }
+    if (fail_at > 0) fail_at--;
     ops.push_back({k, s, what, capturing.count(s) != 0});
     return cudaSuccess;
 }

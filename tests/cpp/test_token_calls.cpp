@@ -17,7 +17,7 @@ static int failures = 0;
         }                                                                       \
     } while (0)
 
-static const cudaStream_t A = (cudaStream_t)0x1000, B = (cudaStream_t)0x2000;
+static const cudaStream_t A = (cudaStream_t)0x1000, B = (cudaStream_t)0x2000, C = (cudaStream_t)0x3000;
 static void* const p = (void*)(1 << 20);  // an address that no kernel reads here
 
 // A handle and the call it is tested with
@@ -128,10 +128,62 @@ static void the_next_call_waits_for_one_that_broke_off() {
     }
 }
 
+// The gradient that writes its table marks the rows that have a token, and its last kernel takes the marks away. A call that breaks off
+// between the two leaves marks: rows that the next call, or the replay of an older graph, would take for written.
+static void marks_are_taken_away_after_a_call_that_broke_off() {
+    const Operator op = embed_grads("embed 2000", 2000, 0);
+    for (int k : {2, 3}) {  // after the wait and the marks: the sums, or the kernel that takes the marks away
+        void* h = op.make();
+        EXPECT(op.call(h, A) == OXZ_OK);
+        // at once, for graphs that were captured while there were none
+        fake::ops.clear();
+        fake::fail_at = k;
+        EXPECT(op.call(h, A) == OXZ_ERR_CUDA);
+        int launch = -1, clear = -1;
+        for (int i = 0; i < (int)fake::ops.size(); i++) {
+            if (fake::ops[i].kind == fake::LAUNCH) launch = i;
+            if (fake::ops[i].kind == fake::CLEAR) clear = i;
+        }
+        EXPECT(launch >= 0 && clear > launch, "call %d failed, launches up to %d, marks cleared at %d", k, launch, clear);
+        // where that fails too: before the next call that runs, however many were captured meanwhile, and within each of those
+        fake::fail_at = k;
+        fake::fail_for = 2;
+        EXPECT(op.call(h, A) == OXZ_ERR_CUDA);
+        fake::capturing.insert(C);
+        for (int i = 0; i < 2; i++) {
+            fake::ops.clear();
+            EXPECT(op.call(h, C) == OXZ_OK);
+            EXPECT(!fake::ops.empty() && fake::ops[0].kind == fake::CLEAR && fake::ops[0].captured, "captured call %d", i);
+        }
+        fake::capturing.clear();
+        fake::ops.clear();
+        EXPECT(op.call(h, B) == OXZ_OK);
+        size_t first = 0;
+        while (first < fake::ops.size() && !works(fake::ops[first])) first++;
+        EXPECT(first < fake::ops.size() && fake::ops[first].kind == fake::CLEAR, "call %d failed, captures, then a call over old marks", k);
+        // and not again
+        fake::ops.clear();
+        EXPECT(op.call(h, B) == OXZ_OK);
+        for (const fake::Op& o : fake::ops) EXPECT(o.kind != fake::CLEAR);
+        op.destroy(h);
+    }
+    // a capture that breaks off has run nothing
+    void* h = op.make();
+    fake::capturing.insert(C);
+    fake::fail_at = 1;
+    EXPECT(op.call(h, C) == OXZ_ERR_CUDA);
+    fake::capturing.clear();
+    fake::ops.clear();
+    EXPECT(op.call(h, A) == OXZ_OK);
+    for (const fake::Op& o : fake::ops) EXPECT(o.kind != fake::CLEAR);
+    op.destroy(h);
+}
+
 int main(int argc, char** argv) {
     const struct { const char* name; void (*run)(); } tests[] = {
         {"error", an_error_is_reported_once},
         {"broke_off", the_next_call_waits_for_one_that_broke_off},
+        {"marks", marks_are_taken_away_after_a_call_that_broke_off},
     };
     for (const auto& t : tests)
         if (argc < 2 || std::strcmp(argv[1], t.name) == 0) t.run();

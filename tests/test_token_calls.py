@@ -50,3 +50,7 @@ def test_an_error_is_reported_once():
 
 def test_the_next_call_waits_for_one_that_broke_off():
     run("broke_off")
+
+
+def test_marks_are_taken_away_after_a_call_that_broke_off():
+    run("marks")
