@@ -8,6 +8,7 @@
 // follow while the piece is in the workspace. Rows that are not scored take no part: the scored ones are listed first, and
 // every product runs over the list.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -974,13 +975,15 @@ bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(
 
 using Encode = decltype(&cuTensorMapEncodeTiled);
 int32_t encoder(Encode* out) {
-    static Encode fn = nullptr;
+    static std::atomic<Encode> found{nullptr};  // handles of several threads ask; whoever comes first finds the same
+    Encode fn = found.load(std::memory_order_acquire);
     if (!fn) {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult st;
         OXZ_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &st));
         if (st != cudaDriverEntryPointSuccess || !p) return fail(OXZ_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
         fn = reinterpret_cast<Encode>(p);
+        found.store(fn, std::memory_order_release);
     }
     *out = fn;
     return OXZ_OK;

@@ -6,7 +6,6 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
-#include <mutex>
 #include <set>
 #include <string>
 #include <vector>
@@ -24,20 +23,19 @@ struct Op {
     bool captured;     // into a graph: nothing runs
 };
 
-inline std::mutex lock;
-inline std::vector<Op> ops;             // what has been enqueued
-inline int fail_at = -1, fail_for = 1;  // this many enqueueing calls from now, so many in a row fail
-inline size_t memory = ~size_t(0);      // the largest allocation that succeeds
-inline std::set<cudaStream_t> capturing;
+// One set for each thread: a lock here would order the threads, and hide what the library shares between them without one.
+inline thread_local std::vector<Op> ops;                // what has been enqueued
+inline thread_local int fail_at = -1, fail_for = 1;     // this many enqueueing calls from now, so many in a row fail
+inline thread_local size_t memory = ~size_t(0);         // the largest allocation that succeeds
+inline thread_local std::set<cudaStream_t> capturing;
 inline thread_local cudaError_t last = cudaSuccess;
-inline std::string message;             // of the library's last error
+inline thread_local std::string message;                // of the library's last error
 
 inline cudaError_t result(cudaError_t e) {
     if (e != cudaSuccess) last = e;
     return e;
 }
 inline cudaError_t enqueue(Kind k, cudaStream_t s, const void* what) {
-    std::lock_guard<std::mutex> hold(lock);
     if (fail_at == 0) {
         if (--fail_for == 0) fail_at = -1, fail_for = 1;
         return result(cudaErrorLaunchOutOfResources);
@@ -60,7 +58,6 @@ int32_t fail(int32_t status, const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(text, sizeof text, fmt, ap);
     va_end(ap);
-    std::lock_guard<std::mutex> hold(fake::lock);
     fake::message = text;
     return status;
 }
@@ -92,7 +89,6 @@ cudaError_t cudaGetDriverEntryPointByVersion(const char*, void** fn, unsigned, u
 cudaError_t cudaEventCreateWithFlags(cudaEvent_t* e, unsigned) { *e = (cudaEvent_t)malloc(1); return cudaSuccess; }
 cudaError_t cudaEventDestroy(cudaEvent_t e) { free((void*)e); return cudaSuccess; }
 cudaError_t cudaStreamIsCapturing(cudaStream_t s, cudaStreamCaptureStatus* st) {
-    std::lock_guard<std::mutex> hold(fake::lock);
     *st = fake::capturing.count(s) ? cudaStreamCaptureStatusActive : cudaStreamCaptureStatusNone;
     return cudaSuccess;
 }

@@ -1,12 +1,14 @@
 // The token operators' calls on the host, over a runtime of notes (fake_cuda.hpp): what they enqueue, in what order, and what is left
 // when one of the runtime's calls fails in the middle.
+#include <atomic>
 #include <cstring>
 #include <functional>
+#include <thread>
 
 #include "../../include/oxz_dpstep.h"
 #include "fake_cuda.hpp"
 
-static int failures = 0;
+static std::atomic<int> failures{0};
 #define EXPECT(c, ...)                                                          \
     do {                                                                        \
         if (!(c)) {                                                             \
@@ -179,14 +181,32 @@ static void marks_are_taken_away_after_a_call_that_broke_off() {
     op.destroy(h);
 }
 
+// Threads with a handle each share nothing that one of them writes: the thread sanitizer watches.
+static void threads_with_a_handle_each() {
+    for (const Operator& op : operators()) {
+        std::vector<std::thread> threads;
+        std::atomic<int> ready{0};
+        for (int k = 0; k < 4; k++)
+            threads.emplace_back([&, k] {
+                void* h = op.make();
+                ready++;
+                while (ready < 4) std::this_thread::yield();
+                for (int i = 0; i < 3; i++) EXPECT(op.call(h, (cudaStream_t)(uintptr_t)(0x10000 + 16 * k)) == OXZ_OK, "%s", op.name);
+                op.destroy(h);
+            });
+        for (std::thread& t : threads) t.join();
+    }
+}
+
 int main(int argc, char** argv) {
     const struct { const char* name; void (*run)(); } tests[] = {
         {"error", an_error_is_reported_once},
         {"broke_off", the_next_call_waits_for_one_that_broke_off},
         {"marks", marks_are_taken_away_after_a_call_that_broke_off},
+        {"threads", threads_with_a_handle_each},
     };
     for (const auto& t : tests)
         if (argc < 2 || std::strcmp(argv[1], t.name) == 0) t.run();
-    std::printf(failures ? "%d failed\n" : "all passed\n", failures);
+    std::printf(failures ? "%d failed\n" : "all passed\n", failures.load());
     return failures != 0;
 }

@@ -54,3 +54,7 @@ def test_the_next_call_waits_for_one_that_broke_off():
 
 def test_marks_are_taken_away_after_a_call_that_broke_off():
     run("marks")
+
+
+def test_threads_with_a_handle_each_share_nothing_that_is_written():
+    run("threads")
