@@ -1112,15 +1112,29 @@ class LitTrainerStep:
 
     # -- the two ends of the model that touch tokens, over the optimizer's own buffers (src/trainer.rs:309-316, 373-482). The work
     # is enqueued on `stream`: order it before the step (set_stream, or a synchronisation), as any backward's.
+    def _addresses(self, operator: "TokenEmbedding | LossHead", tensor: int, reads: bool = True, writes: bool = True) -> tuple[int, int]:
+        """The tensor's addresses for an operator that reads its weights, or writes its gradient: the buffers have no types or bounds of
+        their own, so an operator that does not fit them is refused here."""
+        opt, who = self.optimizer, type(operator).__name__
+        if operator.vocab * operator.hidden > opt.numel[tensor]:
+            raise ValueError(f"{who}: {operator.vocab} x {operator.hidden} elements do not fit tensor {tensor}, which has {opt.numel[tensor]}")
+        if reads and operator.dtype != opt.param_dtype:
+            raise ValueError(f"{who} works in dtype {operator.dtype}, the optimizer's weights have {opt.param_dtype}")
+        if writes and operator.grad_dtype != opt.grad_dtype:
+            raise ValueError(f"{who} writes gradients of dtype {operator.grad_dtype}, the optimizer's have {opt.grad_dtype}")
+        if operator.device != opt.device:
+            raise ValueError(f"{who} is on device {operator.device}, the optimizer on {opt.device}")
+        return opt.tensor_addresses(tensor)
+
     def embed(self, embedding: TokenEmbedding, tensor: int, ids: int, n: int, out: int, out_stride: int = 0, stream: int | None = None) -> None:
         """The hidden states of a micro-batch's inputs, from the working weights of embed_tokens (`tensor`)."""
-        embedding.lookup(ids, n, self.optimizer.tensor_addresses(tensor)[0], out, out_stride, stream)
+        embedding.lookup(ids, n, self._addresses(embedding, tensor, writes=False)[0], out, out_stride, stream)
 
     def embed_grads(self, embedding: TokenEmbedding, tensor: int, ids: int, n: int, d_out: int, accumulate: bool, d_out_stride: int = 0,
                     stream: int | None = None) -> None:
         """The gradient of ``embed`` into the flat buffer. ``accumulate`` False on the first micro-batch of a step, unless the tensor is
         tied to the head's, whose gradient is there already."""
-        embedding.grads(ids, n, d_out, self.optimizer.tensor_addresses(tensor)[1], accumulate, d_out_stride, stream)
+        embedding.grads(ids, n, d_out, self._addresses(embedding, tensor, reads=False)[1], accumulate, d_out_stride, stream)
 
     def loss_weight(self, rows: int, micro_batches: int, scored: int | None = None) -> float:
         """What a micro-batch's summed losses count in the step's loss (src/step_loss.rs:79-112): one over the step's scored tokens when
@@ -1136,7 +1150,7 @@ class LitTrainerStep:
         ``tensor`` (lm_head, or embed_tokens where the two are tied), both times the loss scale. Returns the weight of ``totals[0]`` in
         the step's loss: the local loss ``training_step`` takes is the sum over the micro-batches of weight * totals[0]."""
         weight = self.loss_weight(rows, micro_batches, scored)
-        work, grad = self.optimizer.tensor_addresses(tensor)
+        work, grad = self._addresses(head, tensor)
         head.loss_and_grads(rows, hidden, work, targets, loss_mask=loss_mask, row_loss=row_loss, totals=totals, d_hidden=d_hidden, d_weight=grad,
                             grad_scale=weight * (self.loss_scaler.scale() if self.loss_scaler else 1.0), accumulate=accumulate,
                             hidden_stride=hidden_stride, d_hidden_stride=d_hidden_stride, stream=stream)

@@ -171,3 +171,29 @@ def test_two_handles_on_two_streams_and_two_graphs_of_one():
     del graphs, g
     for job in jobs:
         job["head"].destroy()
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(vocab=31), "31 x 8 elements do not fit tensor 0, which has 240"), (dict(dtype=ox.F16, grad_dtype=ox.F16), "works in dtype 2, the optimizer's weights have 1"),
+    (dict(grad_dtype=ox.F32), "writes gradients of dtype 0, the optimizer's have 1"), (dict(device=1), "is on device 1, the optimizer on 0"),
+])
+@pytest.mark.parametrize("operator", ["embedding", "head"])
+def test_operators_that_do_not_fit_the_optimizers_buffers_are_refused(kw, text, operator):
+    """Before anything is enqueued: types and sizes that differ would be read and written as if they did not."""
+    trainer = ox.LitTrainerStep(ox.TrainerConfig(), ox.DpOptimizer([240, 8], allocate=False))
+    p = 1 << 20  # an address that is only looked at
+    given = {**dict(vocab=30, hidden=8, dtype=ox.BF16, allocate=False), **kw}
+    if operator == "embedding":
+        op = ox.TokenEmbedding(max_tokens=4, **given)
+        # the lookup reads the weights, its gradient does not
+        calls = [] if "dtype" in kw else [lambda: trainer.embed_grads(op, 0, p, 2, p, accumulate=False)]
+        if kw != dict(grad_dtype=ox.F32):
+            calls.append(lambda: trainer.embed(op, 0, p, 2, p))
+    else:
+        op = ox.LossHead(max_rows=4, **given)
+        calls = [lambda: trainer.loss_and_grads(op, 0, 2, p, p, p, p)]
+    for call in calls:
+        with pytest.raises(ValueError) as e:
+            call()
+        assert text in str(e.value)
+    op.destroy()
