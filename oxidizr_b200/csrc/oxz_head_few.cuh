@@ -262,10 +262,11 @@ __global__ void __launch_bounds__(LOGIT_THREADS) k_few_logits_16(const FewArgs a
     few_finish(a, by_warp);
 }
 
-// Any type and alignment: a warp takes WORDS words, lanes along hidden; the rows of x are in shared memory as f32. A lane has 16 bytes of
-// a word at a time, by asynchronous copies as above (WIDE), or one element.
+// f32, and 16-bit rows off 16 bytes: a warp takes WORDS words, lanes along hidden; the rows of x are in shared memory as f32. A lane has 16
+// bytes of a word at a time, by asynchronous copies as above (WIDE: f32 rows on 16 bytes), or one element.
 template <typename T, int R, bool WIDE>
 __global__ void __launch_bounds__(FEW_THREADS) k_few_logits(const FewArgs a) {
+    static_assert(!WIDE || sizeof(T) == 4, "16-bit rows on 16 bytes go by warp products");
     constexpr int N = WIDE ? 16 / (int)sizeof(T) : 1, WORDS = 64 / R;
     constexpr int DEPTH = R == 4 ? 2 : R == 8 ? 3 : 4;
     extern __shared__ __align__(16) float xs[];  // [R][pitch], then (WIDE) the ring [DEPTH][WORDS][threads] 16 bytes
@@ -785,7 +786,10 @@ int32_t few_logits(const FewArgs& a, bool wide, int sms, cudaStream_t s) {
             return OXZ_OK;
         }
     }
-    auto k = wide ? k_few_logits<T, R, true> : k_few_logits<T, R, false>;
+    auto k = k_few_logits<T, R, false>;
+    if constexpr (sizeof(T) == 4) {  // 16-bit rows on 16 bytes have gone the other way
+        if (wide) k = k_few_logits<T, R, true>;
+    }
     OXZ_CUDA(launch_after(false, k, blocks(64 / R), FEW_THREADS, shared, s, a));
     return OXZ_OK;
 }
@@ -831,7 +835,7 @@ int32_t few_run(const FewArgs& a, bool wide, bool out_wide, bool grads, int sms,
 // The shared memory that the kernels may need, granted once.
 template <typename T, typename G, int R>
 int32_t few_prepare_rows() {
-    OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 4096));
+    if constexpr (sizeof(T) == 4) OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 4096));
     OXZ_CUDA(cudaFuncSetAttribute(k_few_logits<T, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SHARED - 4096));
     OXZ_CUDA(cudaFuncSetAttribute(k_few_grads<T, G, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_GRAD_BYTES));
     OXZ_CUDA(cudaFuncSetAttribute(k_few_grads<T, G, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_GRAD_BYTES));
