@@ -45,11 +45,22 @@ struct WaitState {
     volatile uint32_t* dead;
     int32_t* expired;
 };
-constexpr uint32_t WAIT_TRIES = 1u << 24;  // each try suspends the thread for a while: seconds in all
+// A wait gives up after WAIT_NS of waiting that are at least LEAST_TRIES tries: what a try takes depends on the rest of its warp (2 us where
+// all of it waits, 25 ns where other lanes are elsewhere, both measured), so tries alone would bound it to anything from a twentieth of a
+// second to minutes; time alone would count what the block spends off the SM. The clock is not read in a wait of fewer than 256 tries.
+constexpr uint64_t WAIT_NS = 4000000000ull;
+constexpr uint32_t LEAST_TRIES = 1u << 16, MOST_TRIES = 1u << 30;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const WaitState& w) {
-    for (uint32_t i = 0; i < WAIT_TRIES; i++) {
+    uint64_t from = 0;
+    for (uint32_t i = 0; i < MOST_TRIES; i++) {
         if (mbar_try(bar, parity)) return true;
-        if ((i & 255) == 255 && *w.dead) return false;
+        if ((i & 255) == 255) {
+            if (*w.dead) return false;
+            uint64_t now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (from == 0) from = now;
+            if (i >= LEAST_TRIES && now - from > WAIT_NS) break;
+        }
     }
     *w.dead = 1;
     *reinterpret_cast<volatile int32_t*>(w.expired) = 1;
