@@ -398,7 +398,21 @@ impl TokenEmbedding {
     /// # Safety
     /// `ids`, `table` and `out` are device memory of the sizes the description and `n` give.
     pub unsafe fn lookup(&self, ids: *const i64, n: u64, table: *const c_void, out: *mut c_void, stream: *mut c_void) -> Result<()> {
-        check(sys::oxz_embed_lookup_async(self.raw, ids, n, table, out, 0, stream))
+        self.lookup_strided(ids, n, table, out, 0, stream)
+    }
+
+    /// # Safety
+    /// As `lookup`; the rows of `out` are `out_stride` elements apart (0: without gaps).
+    pub unsafe fn lookup_strided(
+        &self,
+        ids: *const i64,
+        n: u64,
+        table: *const c_void,
+        out: *mut c_void,
+        out_stride: u64,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        check(sys::oxz_embed_lookup_async(self.raw, ids, n, table, out, out_stride, stream))
     }
 
     /// # Safety
@@ -412,7 +426,23 @@ impl TokenEmbedding {
         accumulate: bool,
         stream: *mut c_void,
     ) -> Result<()> {
-        check(sys::oxz_embed_grads_async(self.raw, ids, n, d_out, 0, d_table, accumulate as i32, stream))
+        self.grads_strided(ids, n, d_out, 0, d_table, accumulate, stream)
+    }
+
+    /// # Safety
+    /// As `grads`; the rows of `d_out` are `d_out_stride` elements apart (0: without gaps).
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn grads_strided(
+        &mut self,
+        ids: *const i64,
+        n: u64,
+        d_out: *const c_void,
+        d_out_stride: u64,
+        d_table: *mut c_void,
+        accumulate: bool,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        check(sys::oxz_embed_grads_async(self.raw, ids, n, d_out, d_out_stride, d_table, accumulate as i32, stream))
     }
 }
 
@@ -439,7 +469,32 @@ impl LossHead {
     /// # Safety
     /// The batch's pointers and the outputs are device memory of the sizes the description and the batch give.
     pub unsafe fn loss(&mut self, batch: &sys::oxz_head_batch, row_loss: *mut f32, totals: *mut f32, stream: *mut c_void) -> Result<()> {
-        check(sys::oxz_head_loss_async(self.raw, batch, row_loss, ptr::null_mut(), totals, stream))
+        self.loss_with_stats(batch, row_loss, ptr::null_mut(), totals, stream)
+    }
+
+    /// # Safety
+    /// As `loss`; `row_stats` receives what `grads` needs of the same batch.
+    pub unsafe fn loss_with_stats(
+        &mut self,
+        batch: &sys::oxz_head_batch,
+        row_loss: *mut f32,
+        row_stats: *mut f32,
+        totals: *mut f32,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        check(sys::oxz_head_loss_async(self.raw, batch, row_loss, row_stats, totals, stream))
+    }
+
+    /// # Safety
+    /// As `loss`; `row_stats` was written by `loss_with_stats` for the same batch, `grads` names the gradients' memory.
+    pub unsafe fn grads(
+        &mut self,
+        batch: &sys::oxz_head_batch,
+        row_stats: *const f32,
+        grads: &sys::oxz_head_grads,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        check(sys::oxz_head_grads_async(self.raw, batch, row_stats, grads, stream))
     }
 
     /// # Safety
@@ -452,7 +507,21 @@ impl LossHead {
         grads: &sys::oxz_head_grads,
         stream: *mut c_void,
     ) -> Result<()> {
-        check(sys::oxz_head_loss_grads_async(self.raw, batch, row_loss, ptr::null_mut(), totals, grads, stream))
+        self.loss_and_grads_with_stats(batch, row_loss, ptr::null_mut(), totals, grads, stream)
+    }
+
+    /// # Safety
+    /// As `loss_and_grads`; `row_stats` receives the rows' statistics as well.
+    pub unsafe fn loss_and_grads_with_stats(
+        &mut self,
+        batch: &sys::oxz_head_batch,
+        row_loss: *mut f32,
+        row_stats: *mut f32,
+        totals: *mut f32,
+        grads: &sys::oxz_head_grads,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        check(sys::oxz_head_loss_grads_async(self.raw, batch, row_loss, row_stats, totals, grads, stream))
     }
 }
 

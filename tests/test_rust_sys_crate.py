@@ -183,3 +183,17 @@ def test_the_safe_wrapper_calls_only_declared_entry_points():
     for needed in ("oxz_plan_create", "oxz_state_alloc", "oxz_grads_flatten_async", "oxz_step", "oxz_scaler_record_step",
                    "oxz_lr_at", "oxz_spike_judge", "oxz_decay_excludes", "oxz_comm_abort", "oxz_grad_norms_per_tensor"):
         assert needed in used, needed
+
+
+def test_the_safe_wrapper_reaches_every_argument_of_the_token_operators():
+    """What the C++ and Python layers offer - strides, statistics, gradients apart from the losses - the safe layer offers as well: each
+    parameter of each call is handed through by some wrapper, not only given as a constant."""
+    _, hf, _ = parse_header()
+    text = re.sub(r"//[^\n]*", " ", open(os.path.join(CRATE, "src", "safe.rs")).read())
+    for name in ("oxz_embed_lookup_async", "oxz_embed_grads_async", "oxz_head_loss_async", "oxz_head_grads_async", "oxz_head_loss_grads_async"):
+        calls = [[a.strip() for a in m.group(1).split(",")] for m in re.finditer(r"sys::" + name + r"\(([^;]*?)\)\s*(?:\)|;)", text)]
+        assert calls, name
+        for k, (param, _) in enumerate(hf[name][0]):
+            assert all(len(c) == len(hf[name][0]) for c in calls), (name, calls)
+            given = {c[k] for c in calls}
+            assert any(re.match(r"(self\.raw|%s)\b" % param, g) for g in given), (name, param, given)
