@@ -537,14 +537,14 @@ int32_t oxz_loader_next_batch_async(oxz_loader* loader, void* stream, int64_t** 
  *   gradient   d_table[v] = scale * sum over i with ids[i] = v of d_out[i]      (+ what d_table held, when accumulating)
  *
  * Sums run in f32, in an order that the tokens alone decide: equal inputs give equal bits. Each result is rounded once to its
- * type. An id outside [0, vocab) reads as a row of zeros and receives no gradient.
+ * type. An id outside [0, vocab) reads as a row of zeros and receives no gradient. Strides are at most 2^31 elements.
  * The handle holds the workspace of the gradient. It is used by one thread at a time; calls on different streams are ordered by
  * the handle, but graphs captured from its gradient calls share the workspace, so their replays must not overlap each other or
  * other gradient calls of the handle. No call allocates, synchronises or copies to the host. */
 typedef struct oxz_embed oxz_embed;
 typedef struct oxz_embed_desc {
     uint64_t max_tokens;  /* the most tokens of one call, below 2^31 */
-    uint64_t hidden;      /* elements of a row */
+    uint64_t hidden;      /* elements of a row, at most 2^20 */
     uint64_t vocab;       /* rows of the table, below 2^31 */
     double scale;         /* factor of the embedding (1: none); applied in f32 */
     int32_t dtype;        /* oxz_dtype of the table, the rows looked up and their gradients */
@@ -581,15 +581,21 @@ int32_t oxz_embed_grads_async(oxz_embed* embed, const int64_t* ids, uint64_t n, 
  *
  * A row is scored when its loss_mask is not zero and its target lies in [0, vocab). Nothing of another row is used - not its
  * hidden state either, which may hold anything - and it gets loss 0, statistics 0 and a gradient of zeros.
- * Products are summed in f32 and softmax statistics kept in f32. g is rounded to dtype before it is multiplied (f16: scaled by a
- * power of two into its range first; with an f32 d_weight, for that gradient, to 24 bits; with up to 8 rows to twice the digits or more);
- * d_hidden and d_weight are rounded once. The order of every sum is fixed: equal inputs give equal bits. 16-bit weights with hidden
- * a multiple of 8 are read where they lie; others, and f32 ones, are first copied into the workspace in 16-bit parts.
+ * Products are summed in f32 and softmax statistics kept in f32; the order of every sum is fixed: equal inputs give equal bits.
+ * Batches of up to 16 rows stream the weight, as long as the rows fit a block's shared memory: up to 2816 elements of 9 to 16 rows and
+ * 5760 of up to 8 in 16 bits, 2432 of 9 to 16 rows, 3840 of 5 to 8 and 5760 of up to 4 in f32 (more where they do not lie on 16 bytes;
+ * 9 to 16 rows of 16 bits that do not only over a weight of up to 2^20 elements). Others go by tiles on the tensor cores, which cut
+ * what they add, one way: they are emptied into rounded sums so often that losses and their total keep 2e-7 to 3e-7 of themselves off at hidden 2048.
+ * There, 16-bit weights with hidden a multiple of 8 are read where they lie; others, and f32 ones, are first copied into the workspace
+ * in 16-bit parts.
+ * g is rounded to dtype before it is multiplied: f16 scaled by a power of two into its range first; with an f32 d_weight, for that
+ * gradient, to 24 bits; of up to 8 streamed rows to twice the digits or more. Its entry at the target is a difference from one, off by
+ * some 2^-22 of loss_mask (f32: 2^-24) however small it is. d_hidden and d_weight are rounded once. Strides are at most 2^31 elements.
  * d_hidden may be the memory of hidden itself.
  * The handle holds the workspace. It is used by one thread at a time; calls on different streams are ordered by the handle, but
  * graphs captured from its calls share the workspace, so their replays must not overlap each other or other calls of the
  * handle. No call allocates, synchronises or copies to the host. OXZ_ERR_TIMEOUT: a bounded wait inside a kernel of an earlier call
- * ran out, its results are not valid, and the handle serves no further call. */
+ * ran out (after four seconds), its results are not valid, and the handle serves no further call. */
 typedef struct oxz_head oxz_head;
 typedef struct oxz_head_desc {
     uint64_t max_rows;     /* the most tokens of one call, at most 2^30 */
@@ -605,7 +611,8 @@ typedef struct oxz_head_desc {
     int32_t reserved;      /* 0 */
 } oxz_head_desc;
 int32_t oxz_head_create(const oxz_head_desc* desc, oxz_head** out); /* host only: runs without a GPU */
-/* Allocates the workspace on the device; *workspace_bytes (may be NULL) receives its size. */
+/* Allocates the workspace on the device, that of the gradients included whatever the handle is used for; *workspace_bytes (may be NULL)
+ * receives its size. */
 int32_t oxz_head_alloc(oxz_head* head, uint64_t* workspace_bytes);
 int32_t oxz_head_destroy(oxz_head* head);
 /* One batch. All pointers are device memory, aligned to their element (weight: to 16 bytes, as every tensor of a plan is). */

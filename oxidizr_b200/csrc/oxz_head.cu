@@ -1322,8 +1322,9 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             if (d.dtype == OXZ_F32 || d.hidden % 8) OXZ_TRY(get(&h->w, d.vocab * h->pitch * h->parts * 2));
             OXZ_TRY(get(&h->g, h->cap * h->piece * h->g_parts * 2));
             h->kept_pitch = all;
-            // Kept logits are written and read once (10 bytes of traffic an element with G's 2: 1.6 ps measured); forming them again
-            // takes 2 x hidden operations on the tensor cores, six times that for f32 (0.85 ps at hidden 384, 2.9 at 2048, 16 bits).
+            // Kept logits are written and read once (10 bytes of traffic an element with G's 2); forming them again takes 2 x hidden
+            // operations on the tensor cores, six times that for f32. Losses with gradients of 2048 rows over 65536 words, bf16, kept
+            // and formed again: 579 and 461 us at hidden 384, 839 and 764 at 768, 1033 and 1003 at 1024, 1682 and 1870 at 2048.
             // A batch of few logits keeps them at any width: its time is launches, and G from them takes a light one
             // (100 x 360 x 12300 bf16: 42 us, 48 when they are formed again).
             h->keep_large = d.hidden * (d.dtype == OXZ_F32 ? 6 : 1) >= 1024;
