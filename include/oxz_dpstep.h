@@ -585,7 +585,7 @@ int32_t oxz_embed_grads_async(oxz_embed* embed, const int64_t* ids, uint64_t n, 
  * Batches of up to 16 rows stream the weight, as long as the rows fit a block's shared memory: up to 2816 elements of 9 to 16 rows and
  * 5760 of up to 8 in 16 bits, 2432 of 9 to 16 rows, 3840 of 5 to 8 and 5760 of up to 4 in f32 (more where they do not lie on 16 bytes;
  * 9 to 16 rows of 16 bits that do not only over a weight of up to 2^20 elements). Others go by tiles on the tensor cores, which cut
- * what they add, one way: they are emptied into rounded sums so often that losses and their total keep 2e-7 to 3e-7 of themselves off at hidden 2048.
+ * what they add, one way: they are emptied into rounded sums so often that losses and their total are off by 2e-7 to 3e-7 of themselves at hidden 2048.
  * There, 16-bit weights with hidden a multiple of 8 are read where they lie; others, and f32 ones, are first copied into the workspace
  * in 16-bit parts.
  * g is rounded to dtype before it is multiplied: f16 scaled by a power of two into its range first; with an f32 d_weight, for that

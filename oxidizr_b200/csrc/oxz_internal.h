@@ -111,7 +111,9 @@ class Turn {
     explicit Turn(StreamOrder& order) : order_(order) {}
     Turn(const Turn&) = delete;
     Turn& operator=(const Turn&) = delete;
-    ~Turn() { (void)end(); }
+    ~Turn() {  // what made the call break off has been reported
+        if (running_ && record() != cudaSuccess) (void)cudaGetLastError();
+    }
     int32_t begin(cudaStream_t s) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         OXZ_CUDA(cudaStreamIsCapturing(s, &st));
@@ -123,15 +125,20 @@ class Turn {
         return OXZ_OK;
     }
     int32_t end() {
-        if (!running_) return OXZ_OK;
-        OXZ_CUDA(cudaEventRecord(order_.done, stream_));  // one that fails is tried again at the end of the scope
-        running_ = false;
-        order_.used = true;
+        if (running_) OXZ_CUDA(record());  // one that fails is tried again at the end of the scope
         return OXZ_OK;
     }
     bool captured() const { return captured_; }
 
   private:
+    cudaError_t record() {
+        const cudaError_t e = cudaEventRecord(order_.done, stream_);
+        if (e == cudaSuccess) {
+            running_ = false;
+            order_.used = true;
+        }
+        return e;
+    }
     StreamOrder& order_;
     cudaStream_t stream_ = nullptr;
     bool captured_ = false, running_ = false;

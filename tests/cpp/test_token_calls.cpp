@@ -130,6 +130,22 @@ static void the_next_call_waits_for_one_that_broke_off() {
     }
 }
 
+// Where what is done about a failure fails as well, the first one is reported.
+static void the_first_failure_is_the_one_reported() {
+    for (const Operator& op : operators()) {
+        void* h = op.make();
+        EXPECT(op.call(h, A) == OXZ_OK);
+        fake::fail_at = 1;  // the first launch, and all that follows
+        fake::fail_for = 1000;
+        EXPECT(op.call(h, A) == OXZ_ERR_CUDA);
+        EXPECT(fake::message.find("launch_after") == 0, "%s: %s", op.name, fake::message.c_str());
+        fake::fail_at = -1;
+        fake::fail_for = 1;
+        EXPECT(op.call(h, A) == OXZ_OK, "%s: %s", op.name, fake::message.c_str());
+        op.destroy(h);
+    }
+}
+
 // The gradient that writes its table marks the rows that have a token, and its last kernel takes the marks away. A call that breaks off
 // between the two leaves marks: rows that the next call, or the replay of an older graph, would take for written.
 static void marks_are_taken_away_after_a_call_that_broke_off() {
@@ -202,6 +218,7 @@ int main(int argc, char** argv) {
     const struct { const char* name; void (*run)(); } tests[] = {
         {"error", an_error_is_reported_once},
         {"broke_off", the_next_call_waits_for_one_that_broke_off},
+        {"first", the_first_failure_is_the_one_reported},
         {"marks", marks_are_taken_away_after_a_call_that_broke_off},
         {"threads", threads_with_a_handle_each},
     };

@@ -52,6 +52,10 @@ def test_the_next_call_waits_for_one_that_broke_off():
     run("broke_off")
 
 
+def test_the_first_failure_is_the_one_reported():
+    run("first")
+
+
 def test_marks_are_taken_away_after_a_call_that_broke_off():
     run("marks")
 
