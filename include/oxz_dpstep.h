@@ -611,8 +611,8 @@ typedef struct oxz_head_desc {
     int32_t reserved;      /* 0 */
 } oxz_head_desc;
 int32_t oxz_head_create(const oxz_head_desc* desc, oxz_head** out); /* host only: runs without a GPU */
-/* Allocates the workspace on the device, that of the gradients included whatever the handle is used for; *workspace_bytes (may be NULL)
- * receives its size. */
+/* Allocates the workspace on the device, that of the gradients included whatever the handle is used for, and that of the tiles where a
+ * batch may need them; *workspace_bytes (may be NULL) receives its size. */
 int32_t oxz_head_alloc(oxz_head* head, uint64_t* workspace_bytes);
 int32_t oxz_head_destroy(oxz_head* head);
 /* One batch. All pointers are device memory, aligned to their element (weight: to 16 bytes, as every tensor of a plan is). */

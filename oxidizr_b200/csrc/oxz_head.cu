@@ -58,7 +58,7 @@ struct oxz_head {
     float* dx = nullptr;             // [scored rows][dx_pitch] sums over the pieces
     float* dx_shares = nullptr;      // tiles of 256 x 256: the shares after the first of the tiles that are cut
     int sms = 0;
-    float* few_logits = nullptr;     // [vocab][FEW_ROWS] and less: the path for a handful of rows
+    float* few_logits = nullptr;     // [vocab][R]: the path for a handful of rows
     float2* few_part = nullptr;
     float* few_dx = nullptr;
     uint32_t* few_done = nullptr;
@@ -1311,16 +1311,11 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
                 bytes += n;
                 return OXZ_OK;
             };
-            OXZ_TRY(get(&h->row_of, d.max_rows * 4));
-            OXZ_TRY(get(&h->slot_of, d.max_rows * 4));
-            OXZ_TRY(get(&h->part, 2 * std::max<uint64_t>((all / MMA_N) * d.max_rows, (uint64_t)h->clusters * MMA_M) * 8));
-            OXZ_TRY(get(&h->target_logit, d.max_rows * 4));
             OXZ_TRY(get(&h->stats, d.max_rows * 8));
-            OXZ_TRY(get(&h->loss_part, (d.max_rows + FINISH_ROWS - 1) / FINISH_ROWS * 8));
-            OXZ_TRY(get(&h->meta, sizeof(HeadMeta)));
-            OXZ_TRY(get(&h->x, h->cap * h->pitch * h->parts * 2));
-            if (d.dtype == OXZ_F32 || d.hidden % 8) OXZ_TRY(get(&h->w, d.vocab * h->pitch * h->parts * 2));
-            OXZ_TRY(get(&h->g, h->cap * h->piece * h->g_parts * 2));
+            int few_rows = FEW_ROWS;
+            // A handle whose every batch streams the weight never comes to the tiles, and gets none of their workspace
+            const bool tiles = !few_always(d.max_rows, d.hidden, d.vocab, dtype_size(d.dtype), &few_rows);
+            if (tiles) few_rows = FEW_ROWS;
             h->kept_pitch = all;
             // Kept logits are written and read once (10 bytes of traffic an element with G's 2); forming them again takes 2 x hidden
             // operations on the tensor cores, six times that for f32. Losses with gradients of 2048 rows over 65536 words, bf16, kept
@@ -1330,13 +1325,24 @@ int32_t oxz_head_alloc(oxz_head* h, uint64_t* workspace_bytes) {
             h->keep_large = d.hidden * (d.dtype == OXZ_F32 ? 6 : 1) >= 1024;
             h->l_elems = std::min(budget / 3 * 2 / 4, std::min<uint64_t>(h->cap * all, h->keep_large ? ~uint64_t(0) : FEW_LOGITS));
             if (h->l_elems < all) h->l_elems = 0;  // not a single row
-            if (h->l_elems) OXZ_TRY(get(&h->l, h->l_elems * 4));
-            OXZ_TRY(get(&h->dx, h->cap * h->dx_pitch * 4));
-            // rest x shares is at most MAX_ROUNDS x pairs
-            OXZ_TRY(get(&h->dx_shares, (uint64_t)MAX_ROUNDS * h->clusters * MMA_M * MMA_N * 4));
-            OXZ_TRY(get(&h->few_logits, d.vocab * FEW_ROWS * 4));
-            OXZ_TRY(get(&h->few_part, (uint64_t)h->sms * FEW_LOGIT_BLOCKS * FEW_ROWS * 8));
-            OXZ_TRY(get(&h->few_dx, (uint64_t)std::max(few_parts(d.hidden, d.vocab, h->sms, 1), few_parts_16(d.hidden, d.vocab, h->sms)) * FEW_ROWS * d.hidden * 4));
+            if (tiles) {
+                OXZ_TRY(get(&h->row_of, d.max_rows * 4));
+                OXZ_TRY(get(&h->slot_of, d.max_rows * 4));
+                OXZ_TRY(get(&h->part, 2 * std::max<uint64_t>((all / MMA_N) * d.max_rows, (uint64_t)h->clusters * MMA_M) * 8));
+                OXZ_TRY(get(&h->target_logit, d.max_rows * 4));
+                OXZ_TRY(get(&h->loss_part, (d.max_rows + FINISH_ROWS - 1) / FINISH_ROWS * 8));
+                OXZ_TRY(get(&h->meta, sizeof(HeadMeta)));
+                OXZ_TRY(get(&h->x, h->cap * h->pitch * h->parts * 2));
+                if (d.dtype == OXZ_F32 || d.hidden % 8) OXZ_TRY(get(&h->w, d.vocab * h->pitch * h->parts * 2));
+                OXZ_TRY(get(&h->g, h->cap * h->piece * h->g_parts * 2));
+                if (h->l_elems) OXZ_TRY(get(&h->l, h->l_elems * 4));
+                OXZ_TRY(get(&h->dx, h->cap * h->dx_pitch * 4));
+                // rest x shares is at most MAX_ROUNDS x pairs
+                OXZ_TRY(get(&h->dx_shares, (uint64_t)MAX_ROUNDS * h->clusters * MMA_M * MMA_N * 4));
+            }
+            OXZ_TRY(get(&h->few_logits, d.vocab * few_rows * 4));
+            OXZ_TRY(get(&h->few_part, (uint64_t)h->sms * FEW_LOGIT_BLOCKS * few_rows * 8));
+            OXZ_TRY(get(&h->few_dx, (uint64_t)std::max(few_parts(d.hidden, d.vocab, h->sms, 1), few_parts_16(d.hidden, d.vocab, h->sms)) * few_rows * d.hidden * 4));
             OXZ_TRY(get(&h->few_done, 4));
             OXZ_CUDA(cudaMemset(h->few_done, 0, 4));
             OXZ_CUDA(cudaDeviceSynchronize());
@@ -1358,7 +1364,7 @@ int32_t oxz_head_destroy(oxz_head* h) {
     return guarded("oxz_head_destroy", [&]() -> int32_t {
         if (!h) return OXZ_OK;
         DeviceGuard dev;
-        if (h->row_of) dev.enter(h->d.device);
+        if (h->stats) dev.enter(h->d.device);
         h->order.destroy();
         for (void* p : {(void*)h->row_of, (void*)h->slot_of, (void*)h->part, (void*)h->target_logit, (void*)h->stats, (void*)h->loss_part,
                         (void*)h->meta, h->x, h->w, h->g, (void*)h->l, (void*)h->dx, (void*)h->dx_shares, (void*)h->few_logits,

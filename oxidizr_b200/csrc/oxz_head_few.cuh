@@ -777,6 +777,18 @@ inline bool few_fits(uint64_t rows, uint64_t hidden, uint64_t vocab, size_t size
     if (size == 2 && !wide && rows > 8 && hidden * vocab > (1u << 20)) return false;
     return rows <= (uint64_t)FEW_ROWS && few_logit_bytes(few_kernel_rows(rows, size, wide), hidden, size, wide) + 8192 <= FEW_SHARED;
 }
+// Every batch of up to `rows` rows goes this way, wherever its rows lie; *most: the rows of the largest kernel among them.
+inline bool few_always(uint64_t rows, uint64_t hidden, uint64_t vocab, size_t size, int* most) {
+    *most = 0;
+    if (rows > (uint64_t)FEW_ROWS) return false;
+    for (uint64_t r = 0; r <= rows; r++)
+        for (const bool wide : {false, true}) {
+            if (wide && hidden * size % 16 != 0) continue;
+            if (!few_fits(r, hidden, vocab, size, wide)) return false;
+            *most = std::max(*most, few_kernel_rows(r, size, wide));
+        }
+    return true;
+}
 template <typename T, int R>
 int32_t few_logits(const FewArgs& a, bool wide, int sms, cudaStream_t s) {
     const size_t shared = few_logit_bytes(R, a.hidden, sizeof(T), wide);

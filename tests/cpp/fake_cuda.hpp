@@ -27,6 +27,7 @@ struct Op {
 inline thread_local std::vector<Op> ops;                // what has been enqueued
 inline thread_local int fail_at = -1, fail_for = 1;     // this many enqueueing calls from now, so many in a row fail
 inline thread_local size_t memory = ~size_t(0);         // the largest allocation that succeeds
+inline thread_local size_t allocated = 0;               // bytes asked for and got
 inline thread_local std::set<cudaStream_t> capturing;
 inline thread_local cudaError_t last = cudaSuccess;
 inline thread_local std::string message;                // of the library's last error
@@ -70,6 +71,7 @@ cudaError_t cudaGetLastError(void) { const cudaError_t e = fake::last; fake::las
 const char* cudaGetErrorString(cudaError_t) { return "fake error"; }
 cudaError_t cudaMalloc(void** p, size_t n) {
     if (n > fake::memory || !(*p = aligned_alloc(256, (n + 255) / 256 * 256))) return fake::result(cudaErrorMemoryAllocation);
+    fake::allocated += n;
     return cudaSuccess;
 }
 cudaError_t cudaFree(void* p) { free(p); return cudaSuccess; }

@@ -1,5 +1,6 @@
 // The token operators' calls on the host, over a runtime of notes (fake_cuda.hpp): what they enqueue, in what order, and what is left
 // when one of the runtime's calls fails in the middle.
+#include <algorithm>
 #include <atomic>
 #include <cstring>
 #include <functional>
@@ -214,11 +215,43 @@ static void threads_with_a_handle_each() {
     }
 }
 
+// A head whose every batch streams the weight has no workspace for tiles; one that may meet another batch has both.
+static void a_handful_of_rows_takes_no_workspace_for_tiles() {
+    const struct { uint64_t rows, hidden, vocab; int32_t dtype, grad; bool streams; } cases[] = {
+        {1, 512, 100315, OXZ_F32, OXZ_F32, true},    {16, 768, 39380, OXZ_F32, OXZ_F32, true},    {8, 1024, 32000, OXZ_BF16, OXZ_BF16, true},
+        {4, 5760, 32000, OXZ_F16, OXZ_F32, true},    {8, 345, 20000, OXZ_F16, OXZ_F16, true},     {16, 345, 3000, OXZ_BF16, OXZ_BF16, true},
+        {17, 512, 32000, OXZ_F32, OXZ_F32, false},   {16, 1024, 32000, OXZ_BF16, OXZ_BF16, false},  // a batch off 16 bytes would go by tiles
+        {8, 5768, 32000, OXZ_BF16, OXZ_BF16, false}, {16, 2436, 32000, OXZ_F32, OXZ_F32, false},  {16, 345, 3100, OXZ_BF16, OXZ_BF16, false},
+        {3, 5764, 32000, OXZ_F32, OXZ_F32, false},   {3, 5763, 32000, OXZ_F32, OXZ_F32, true},
+    };
+    for (const auto& c : cases) {
+        const oxz_head_desc d{c.rows, c.hidden, c.vocab, 0, c.dtype, c.grad, 0, 0};
+        oxz_head* h = nullptr;
+        uint64_t bytes = 0;
+        fake::allocated = 0;
+        EXPECT(oxz_head_create(&d, &h) == OXZ_OK);
+        EXPECT(oxz_head_alloc(h, &bytes) == OXZ_OK);
+        EXPECT(bytes <= fake::allocated && fake::allocated <= bytes + 4096, "%llu reported, %zu taken", (unsigned long long)bytes, fake::allocated);
+        // at most: the logits of 16 rows, d_hidden's sums of two blocks an SM of up to 1024 columns each, and small change
+        const uint64_t streaming = 64 * (c.vocab + 2 * 148 * std::min<uint64_t>(c.hidden, 1024) + c.hidden) + (1 << 20);
+        EXPECT((bytes <= streaming) == c.streams, "%llu rows of %llu over %llu: %llu bytes, streaming alone %llu", (unsigned long long)c.rows, (unsigned long long)c.hidden,
+               (unsigned long long)c.vocab, (unsigned long long)bytes, (unsigned long long)streaming);
+        for (uint64_t rows = 0; rows <= c.rows; rows++)
+            for (uint64_t off : {uint64_t(0), uint64_t(4)}) {
+                const oxz_head_batch b{rows, (char*)p + off, 0, p, (const int64_t*)p, nullptr};
+                const oxz_head_grads g{p, 0, p, 1.0, 0, 0};
+                EXPECT(oxz_head_loss_grads_async(h, &b, (float*)p, nullptr, (float*)p, &g, A) == OXZ_OK, "%s", fake::message.c_str());
+            }
+        oxz_head_destroy(h);
+    }
+}
+
 int main(int argc, char** argv) {
     const struct { const char* name; void (*run)(); } tests[] = {
         {"error", an_error_is_reported_once},
         {"broke_off", the_next_call_waits_for_one_that_broke_off},
         {"first", the_first_failure_is_the_one_reported},
+        {"handful", a_handful_of_rows_takes_no_workspace_for_tiles},
         {"marks", marks_are_taken_away_after_a_call_that_broke_off},
         {"threads", threads_with_a_handle_each},
     };

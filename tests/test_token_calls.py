@@ -62,3 +62,7 @@ def test_marks_are_taken_away_after_a_call_that_broke_off():
 
 def test_threads_with_a_handle_each_share_nothing_that_is_written():
     run("threads")
+
+
+def test_a_handful_of_rows_takes_no_workspace_for_tiles():
+    run("handful")
