@@ -589,7 +589,7 @@ int32_t oxz_embed_grads_async(oxz_embed* embed, const int64_t* ids, uint64_t n, 
  * There, 16-bit weights with hidden a multiple of 8 are read where they lie; others, and f32 ones, are first copied into the workspace
  * in 16-bit parts.
  * g is rounded to dtype before it is multiplied: f16 scaled by a power of two into its range first; with an f32 d_weight, for that
- * gradient, to 24 bits; of up to 8 streamed rows to twice the digits or more. Its entry at the target is a difference from one, off by
+ * gradient, to 24 bits; of streamed rows to twice the digits or more. Its entry at the target is a difference from one, off by
  * some 2^-22 of loss_mask (f32: 2^-24) however small it is. d_hidden and d_weight are rounded once. Strides are at most 2^31 elements.
  * d_hidden may be the memory of hidden itself.
  * The handle holds the workspace. It is used by one thread at a time; calls on different streams are ordered by the handle, but

@@ -10,8 +10,8 @@
 //
 // f32 rows, and 16-bit ones off 16 bytes, are f32 arithmetic in registers, and G is not rounded. 16-bit rows on 16 bytes use the
 // 16 x 8 x 16 warp product (mma.sync): at 16 rows the pass is bound by the weight's way, not by the product's rate (128256 words of 2048:
-// logits 120 us, 4.4 TB/s; gradients 209 us, 4.85 TB/s). Their gradients take G in two 16-bit parts up to 8 rows and in one above
-// (k_few_grads_16); an f32 d_weight takes k_few_grads and G unrounded. R, the rows a kernel is made for, is 4, 8 or 16.
+// logits 120 us, 4.4 TB/s; gradients 209 us, 4.85 TB/s). Their gradients take G in two 16-bit parts (k_few_grads_16); an f32 d_weight
+// takes k_few_grads and G unrounded. R, the rows a kernel is made for, is 4, 8 or 16.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -544,8 +544,9 @@ __global__ void __launch_bounds__(FEW_THREADS) k_few_grads(const FewArgs a, uint
 
 // Gradients of 16-bit operands on 16 bytes, by warp products. A block has 64 x across columns, a warp 64 of them; `along` = 4 / across
 // warps share a stretch of 16 x along words. A stretch's piece of the weight (8 KiB) and its kept logits come by asynchronous copies
-// GRAD_DEPTH stretches ahead; the block turns the logits into G - of up to 8 rows in two 16-bit parts, the second in the place of rows
-// 8 .. 15 (2^-16 of it is lost, where one part leaves 2^-9, which so few rows do not average out) - and each warp multiplies
+// GRAD_DEPTH stretches ahead; the block turns the logits into G, in two 16-bit parts (2^-16 of it is lost; one part would leave 2^-9,
+// which so few rows do not average out: 0.0023 of the gradients of 16 rows instead of the 0.0017 that their own rounding is), of up to
+// 8 rows the second in the place of rows 8 .. 15, of more as a product of its own (nothing, to 3 % at 128 columns) - and each warp multiplies
 //   dX[i][h] += sum_v G[v][i] W[v][h]    A = G^T (words along K) and B = W, both through transposing loads
 //   dW[v][h]  = sum_i G[v][i] x[i][h]    A = G as it lies, B = x in registers for good
 // dW's columns are dealt to the product's so that a lane's 16 results of a word are neighbours, written as two pieces of 16 bytes.
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a) 
     constexpr uint32_t l_bytes = words * R * 4;
     unsigned char* wp = raw16;                                                 // [GRAD_DEPTH][words][64 * across], 16-byte chunks turned by the word
     float* lp = reinterpret_cast<float*>(raw16 + GRAD_DEPTH * PIECE);          // [GRAD_DEPTH][words][R]
-    T* gp = reinterpret_cast<T*>(raw16 + GRAD_DEPTH * (PIECE + l_bytes));      // [words][16]
+    T* gp = reinterpret_cast<T*>(raw16 + GRAD_DEPTH * (PIECE + l_bytes));      // [words][16], and of 16 rows the second parts behind
     __shared__ float row_m[16], row_f[16], row_s[16];
     __shared__ uint32_t row_t[16];
     let_next();
@@ -646,14 +647,18 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a) 
             }
             const T hi = from_f32<T>(y), lo = from_f32<T>(isfinite(y) ? y - to_f32<T>(hi) : 0.f);
             gp[d * 16 + i] = hi;
-            if (R == 8) gp[d * 16 + 8 + i] = lo;
+            gp[R == 8 ? d * 16 + 8 + i : (words + d) * 16 + i] = lo;
         }
         __syncthreads();
         if (col >= a.hidden) continue;
-        uint32_t gt[4], gn[4];  // G^T and G of the warp's 16 words
-        const T* from = gp + mine * 16 * 16;
-        load_matrices_turned(gt, smem_address(from + ((lane >> 4) * 8 + (lane & 7)) * 16 + ((lane >> 3) & 1) * 8));
-        load_matrices(gn, smem_address(from + (((lane >> 3) & 1) * 8 + (lane & 7)) * 16 + (lane >> 4) * 8));
+        constexpr int PARTS = R / 8;
+        uint32_t gt[PARTS][4], gn[PARTS][4];  // G^T and G of the warp's 16 words
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) {
+            const T* from = gp + (p * words + mine * 16) * 16;
+            load_matrices_turned(gt[p], smem_address(from + ((lane >> 4) * 8 + (lane & 7)) * 16 + ((lane >> 3) & 1) * 8));
+            load_matrices(gn[p], smem_address(from + (((lane >> 3) & 1) * 8 + (lane & 7)) * 16 + (lane >> 4) * 8));
+        }
         if (a.want_dx) {
             const unsigned char* piece = wp + st * PIECE;
             const uint32_t d = mine * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);  // the word this lane points at
@@ -662,8 +667,11 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a) 
                 uint32_t b[4];
                 const uint32_t c = j + (lane >> 4);
                 load_matrices_turned(b, smem_address(piece + d * 128 * across + group * 128 + (((c ^ d) & 7) << 4)));
-                warp_product<T>(dx[j], gt, b[0], b[1]);
-                warp_product<T>(dx[j + 1], gt, b[2], b[3]);
+#pragma unroll
+                for (int p = PARTS - 1; p >= 0; p--) {
+                    warp_product<T>(dx[j], gt[p], b[0], b[1]);
+                    warp_product<T>(dx[j + 1], gt[p], b[2], b[3]);
+                }
             }
         }
         if (dw) {
@@ -671,7 +679,8 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_few_grads_16(const FewArgs a) 
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 out[j][0] = out[j][1] = out[j][2] = out[j][3] = 0.f;
-                warp_product<T>(out[j], gn, xb[j][0], xb[j][1]);
+#pragma unroll
+                for (int p = PARTS - 1; p >= 0; p--) warp_product<T>(out[j], gn[p], xb[j][0], xb[j][1]);
             }
             const uint32_t h = col + 16 * q;
 #pragma unroll
@@ -821,7 +830,7 @@ int32_t few_run_rows(FewArgs a, bool wide, bool out_wide, bool grads, int sms, c
             parts = few_parts_16(a.hidden, a.vocab, sms);
             a.words = ((a.vocab + parts - 1) / parts + words - 1) / words * words;
             parts = (a.vocab + a.words - 1) / a.words;
-            const size_t shared = (size_t)GRAD_DEPTH * (8192 + words * R * 4) + words * 16 * 2;
+            const size_t shared = (size_t)GRAD_DEPTH * (8192 + words * R * 4) + words * 16 * 2 * (R / 8);
             auto k = across == 4 ? k_few_grads_16<T, G, R, 2> : across == 2 ? k_few_grads_16<T, G, R, 1> : k_few_grads_16<T, G, R, 0>;
             OXZ_CUDA(launch_after(true, k, dim3(parts, columns), GRAD_THREADS, shared, s, a));
             scaled = true;

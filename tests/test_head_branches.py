@@ -113,6 +113,26 @@ def test_the_widest_rows_of_a_handful(dtype, rows, last, first, over):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows, hidden, vocab, gap", [(9, 1024, 2000, 0), (16, 1024, 2000, 8), (16, 64, 3000, 0), (12, 128, 3000, 0), (8, 512, 2000, 0), (1, 256, 2000, 0),
+                                                      (16, 100, 900, 3), (7, 33, 900, 0)])
+def test_a_handful_of_rows_keeps_twice_the_digits_of_g(dtype, rows, hidden, vocab, gap):
+    import torch
+    pr = Problem(dtype, rows, hidden, vocab, "weights" if rows > 1 else None, seed=8, gap=gap).solve(scale=0.5)
+    h = ox.LossHead(vocab, hidden, rows, dtype=NAMES[dtype])
+    o = pr.outputs()
+    h.loss_and_grads(**pr.batch(), **ptrs(o), grad_scale=0.5)
+    torch.cuda.synchronize()
+    pr.check(o, o)
+    dh, dw = fine_tolerance(pr, 0.5)
+    off = np.abs(o["d_hidden"].double().cpu().numpy() - pr.d_hidden)[pr.scored] / dh[pr.scored]
+    assert np.all(off <= 1), off.max()
+    off = np.abs(o["d_weight"].double().cpu().numpy() - pr.d_weight) / dw
+    assert np.all(off <= 1), off.max()
+    h.destroy()
+
+
+@gpu
 @pytest.mark.parametrize("rows", [12, 200])
 def test_two_threads_with_a_handle_each(rows):
     import torch
